@@ -302,6 +302,97 @@ int ugbsa_decode(const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_
                  int64_t so_h, int64_t so_d, float* workspace, int64_t workspace_elems,
                  void* stream);
 
+/* ---- paged key-value cache ----------------------------------------------- */
+
+#define UGBSA_CACHE_MODEL 0 /* pages hold dtype */
+#define UGBSA_CACHE_E4M3 1  /* pages hold e4m3 codes, scales a byte per token and head */
+
+/* A cache of num_pages pages of 64 tokens (the key block), Hk heads of D.  A
+ * block table [B, max_pages] int32 (row stride st_b, entries contiguous) names
+ * the pages of each sequence: token i of sequence b is slot i % 64 of page
+ * table[b][i / 64].  Tables, lengths and lists are device data:
+ *  - a length counts as 0 below 0 and as 64 * max_pages above that;
+ *  - a table entry outside [0, num_pages) is an absent page: nothing is
+ *    written to it, it reads as zeros, and its keys take no part.
+ * Slots past a sequence's length may hold anything, NaN included. */
+typedef struct {
+  void* k_pages; /* [num_pages, Hk, 64, D] of dtype or e4m3, head_dim stride 1, */
+  void* v_pages; /* 16-byte aligned rows; the other strides in elements */
+  int64_t sk_p, sk_h, sk_n;
+  int64_t sv_p, sv_h, sv_n;
+  uint8_t* k_scale; /* [num_pages, Hk, 64] contiguous, e4m3 only: a value is */
+  uint8_t* v_scale; /* code * 2^(byte - 127) */
+  void* planes;     /* [num_pages, Hk, 2, D] of dtype, contiguous: K-max and K-min
+                       of each page (16-byte aligned), or NULL */
+  int num_pages, Hk, D;
+  int dtype;       /* UGBSA_DTYPE_* of q, k, v, out and planes */
+  int cache_dtype; /* UGBSA_CACHE_* */
+} ugbsa_paged_cache;
+
+/* New tokens into the cache: k, v [T, Hk, D] of dtype, packed; sequence b's are
+ * rows cu_new[b] .. cu_new[b + 1] - 1 (cu_new [B + 1] int32, ascending; NULL: row
+ * b, one token each, T >= B) and go to positions lens[b], lens[b] + 1, ... .  Rows
+ * behind the last sequence and tokens past the table are left out.  e4m3: a
+ * token's head is divided by the smallest power of two that brings its largest
+ * finite magnitude to 448 or less and rounded to nearest even; infinities and
+ * values that would read back infinite are held at the largest that does not,
+ * NaN stays NaN.  planes: K-max and K-min of a page start over with its slot 0
+ * and otherwise take the new keys in (from k as given, before any rounding; NaN
+ * is passed over).  A page must not be named by two of the sequences that write
+ * to it. */
+int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
+                      int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
+                      const int32_t* cu_new, const int32_t* lens, const int32_t* table,
+                      int64_t st_b, int B, int T, int max_pages, void* stream);
+
+/* Cached tokens back: k_out, v_out [B, Hk, N, D] of dtype (the prefill entry
+ * points' layout), row n of sequence b its token n, zeros from lens[b] on.
+ * Exact: e4m3 values are values of dtype. */
+int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const int32_t* table,
+                     int64_t st_b, int B, int max_pages, int N, void* k_out, int64_t sk_b,
+                     int64_t sk_h, int64_t sk_n, int64_t sk_d, void* v_out, int64_t sv_b,
+                     int64_t sv_h, int64_t sv_n, int64_t sv_d, void* stream);
+
+/* fp32 elements of a ugbsa_paged_select workspace (0 for sizes no call takes). */
+int64_t ugbsa_paged_select_workspace_elems(int B, int Hk, int max_pages);
+
+/* Pages for one new token of each sequence: q [B, H, 1, D] of dtype, lens with
+ * that token.  A page's score is the maximum over the KV head's query heads of
+ * the Quest bound sum_d (q_d >= 0 ? q_d kmax_d : q_d kmin_d), summed in fp64.
+ * Kept: the first and the last page and, of the others, the best by (score
+ * desc, page asc), k_base pages in all, or k_slots where the cut is uncertain:
+ * sigma < tau, sigma = min(max((s(k) - s(k + 1)) / max(s(1) - s(k + 1), 1e-9),
+ * 0), 2) with s(i) the i-th best of the others' scores times scaling and k =
+ * k_base - 2; 2 where no page is cut.  Out: kv_idx [B, Hk, k_slots] int32, page
+ * numbers within the sequence, ascending, then max_pages; counts [B, Hk] int32;
+ * sigma [B, Hk] fp32 and uncertain [B, Hk] uint8 (either may be NULL).
+ * 3 <= k_base <= k_slots; scaling positive and finite; workspace 8-byte
+ * aligned. */
+int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                       int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                       const int32_t* table, int64_t st_b, int B, int max_pages, float scaling,
+                       int k_base, int k_slots, float tau, int32_t* kv_idx, int32_t* counts,
+                       float* sigma, uint8_t* uncertain, float* workspace,
+                       int64_t workspace_elems, void* stream);
+
+/* fp32 elements of a ugbsa_paged_decode workspace (0: none is needed, or sizes no
+ * call takes).  units: max_pages, or k_slots of a call with lists. */
+int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units);
+
+/* Decode over pages — attention of one query row per head over the tokens below
+ * lens[b]: of every page (kv_idx NULL), or of the pages that kv_idx [B, Hk,
+ * k_slots] lists for the KV head, the first counts[b][h] entries (counts NULL:
+ * all k_slots).  Entries outside the sequence's pages are skipped; a page must
+ * not be listed twice.  q [B, H, 1, D], out [B, H, D] of dtype with any b and h
+ * strides; B, H <= 65535.  A row without a key, or whose every weight is 0, gives
+ * zeros. */
+int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                       int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                       const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
+                       const int32_t* kv_idx, const int32_t* counts, int k_slots, void* out,
+                       int64_t so_b, int64_t so_h, int64_t so_d, float* workspace,
+                       int64_t workspace_elems, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,120 @@
+"""The paged cache's argument checks and size queries, which need no GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+import _capi
+import paged_cache as pc
+
+
+def struct(**kw):
+    s = dict(k_pages=16, v_pages=16, sk_p=16384, sk_h=8192, sk_n=128, sv_p=16384, sv_h=8192, sv_n=128,
+             planes=16, num_pages=4, Hk=2, D=128, dtype=_capi.DTYPE_BF16, cache_dtype=_capi.CACHE_MODEL)
+    s.update(kw)
+    return _capi.PagedCacheStruct(**s)
+
+
+def decode(lib, c, B=1, H=4, pages=8, scale=0.1, q=16, kv=None, counts=None, slots=0, out=16, ws=16, n=1 << 30,
+           table=16, st=8):
+    return lib.ugbsa_paged_decode(ctypes.addressof(c) if c else None, q, 512, 128, 128, 1, H, 16, table, st, B,
+                                  pages, scale, kv, counts, slots, out, 512, 128, 1, ws, n, None)
+
+
+def select(lib, c, k_base=4, k_slots=8, scaling=0.1, tau=0.1, ws=16, n=1 << 30):
+    return lib.ugbsa_paged_select(ctypes.addressof(c), 16, 512, 128, 128, 1, 4, 16, 16, 8, 1, 8, scaling, k_base,
+                                  k_slots, tau, 16, 16, None, None, ws, n, None)
+
+
+def refused(lib, rc, code, word):
+    assert rc == code and word in lib.ugbsa_last_error().decode(), (rc, lib.ugbsa_last_error())
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _capi.lib()
+
+
+def test_decode_refusals(lib):
+    refused(lib, decode(lib, None), -1, "cache is null")
+    refused(lib, decode(lib, struct(D=96)), -1, "head_dim")
+    refused(lib, decode(lib, struct(dtype=7)), -3, "dtype")
+    refused(lib, decode(lib, struct(cache_dtype=9)), -3, "cache dtype")
+    refused(lib, decode(lib, struct(Hk=0)), -1, "positive")
+    refused(lib, decode(lib, struct(), H=5), -1, "multiple")
+    refused(lib, decode(lib, struct(num_pages=0)), -1, "num_pages")
+    refused(lib, decode(lib, struct(), pages=0), -1, "max_pages")
+    refused(lib, decode(lib, struct(), pages=(1 << 24) + 1), -1, "max_pages")
+    refused(lib, decode(lib, struct(), B=65536), -1, "65535")
+    refused(lib, decode(lib, struct(), table=None), -1, "null")
+    refused(lib, decode(lib, struct(), st=-8), -2, "stride")
+    refused(lib, decode(lib, struct(k_pages=None)), -1, "null")
+    refused(lib, decode(lib, struct(k_pages=8)), -2, "aligned")
+    refused(lib, decode(lib, struct(sv_n=132)), -2, "aligned")
+    refused(lib, decode(lib, struct(cache_dtype=_capi.CACHE_E4M3)), -1, "scale")
+    refused(lib, decode(lib, struct(cache_dtype=_capi.CACHE_E4M3, k_scale=16, v_scale=17)), -2, "aligned")
+    refused(lib, decode(lib, struct(cache_dtype=_capi.CACHE_E4M3, k_scale=16, v_scale=16, sk_n=136)), -2, "aligned")
+    refused(lib, decode(lib, struct(), q=None), -1, "q is null")
+    for scale in (float("nan"), float("inf")):
+        refused(lib, decode(lib, struct(), scale=scale), -1, "scale")
+    refused(lib, decode(lib, struct(), kv=16, slots=0), -1, "k_slots")
+    refused(lib, decode(lib, struct(), counts=16), -1, "counts")
+    refused(lib, decode(lib, struct(), out=None), -2, "out")
+    need = lib.ugbsa_paged_decode_workspace_elems(1, 4, 2, 128, 64)
+    assert need > 0
+    refused(lib, decode(lib, struct(), pages=64, n=need - 1), -1, "workspace")
+    refused(lib, decode(lib, struct(), pages=64, ws=None), -1, "workspace")
+
+
+def test_select_refusals(lib):
+    refused(lib, select(lib, struct(planes=None)), -1, "planes")
+    refused(lib, select(lib, struct(planes=24)), -1, "planes")
+    refused(lib, select(lib, struct(), k_base=2), -1, "k_base")
+    refused(lib, select(lib, struct(), k_slots=3), -1, "k_base")
+    for scaling in (0.0, -1.0, float("inf"), float("nan")):
+        refused(lib, select(lib, struct(), scaling=scaling), -1, "scaling")
+    refused(lib, select(lib, struct(), tau=float("nan")), -1, "tau")
+    need = lib.ugbsa_paged_select_workspace_elems(1, 2, 8)
+    refused(lib, select(lib, struct(), n=need - 1), -1, "workspace")
+    refused(lib, select(lib, struct(), ws=20), -2, "workspace")
+
+
+def test_write_and_read_refusals(lib):
+    c = struct()
+
+    def write(T=4, B=1, cu=16, k=16, sk=256):
+        return lib.ugbsa_paged_write(ctypes.addressof(c), k, sk, 128, 1, 16, 256, 128, 1, cu, 16, 16, 8, B, T, 8, None)
+    refused(lib, write(T=-1), -1, "T=")
+    refused(lib, write(T=3, B=4, cu=None), -1, "T=")
+    refused(lib, write(k=None), -1, "k is null")
+    refused(lib, write(k=18), -2, "aligned")
+    refused(lib, write(sk=250), -2, "strides")
+    assert write(T=0) == 0                      # nothing to write: no launch
+
+    def read(N=64, out=16, sd=1):
+        return lib.ugbsa_paged_read(ctypes.addressof(c), 16, 16, 8, 1, 8, N, out, 8192, 8192, 128, sd,
+                                    16, 8192, 8192, 128, 1, None)
+    refused(lib, read(N=0), -1, "N must")
+    refused(lib, read(N=(1 << 30) + 1), -1, "N must")
+    refused(lib, read(out=None), -1, "null")
+    refused(lib, read(sd=2), -2, "stride")
+
+
+def test_workspace_queries_of_sizes_no_call_takes(lib):
+    for B, H, Hk, D, units in ((0, 4, 2, 128, 8), (1, 0, 2, 128, 8), (1, 5, 2, 128, 8), (1, 4, 2, 96, 8),
+                               (1, 4, 2, 128, 0), (1, 4, 2, 128, -1)):
+        assert lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, units) == 0
+    assert lib.ugbsa_paged_select_workspace_elems(0, 2, 8) == lib.ugbsa_paged_select_workspace_elems(1, 2, 0) == 0
+
+
+def test_caches_of_host_tensors_are_refused():
+    pages = torch.zeros(2, 1, 64, 64, dtype=torch.bfloat16)
+    for make in (lambda: pc.PagedCache(pages, pages), lambda: pc.PagedCache(pages, None),
+                 lambda: pc.PagedCache(pages.float(), pages.float()),
+                 lambda: pc.PagedCache(pages[:, :, :32], pages[:, :, :32]),
+                 lambda: pc.PagedCache(pages, pages, planes=torch.zeros(2, 1, 2, 32, dtype=torch.bfloat16)),
+                 lambda: pc.PagedCache(pages.transpose(2, 3), pages.transpose(2, 3)),
+                 lambda: pc.PagedCache.empty(2, 1, 64, torch.bfloat16, "cpu", e4m3=True)):
+        with pytest.raises(AssertionError):
+            make()

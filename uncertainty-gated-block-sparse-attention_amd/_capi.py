@@ -27,6 +27,7 @@ GRAIN_CELL, GRAIN_ROW = 0, 1
 ROUTER_ABS, ROUTER_QUANTILE = 0, 1
 V1_TOPK, V1_BELIEF = 0, 1
 DECODE_ONE_SPLIT = 512
+CACHE_MODEL, CACHE_E4M3 = 0, 1
 
 # Every symbol include/ugbsa.h declares, with its ctypes signature.
 _i, _i64, _f, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -79,8 +80,28 @@ SIGNATURES = {
                           _p, _i64, _i64, _i64, _i64,
                           _p, _i64, _i64, _i64, _i64,
                           _i, _i, _i, _i, _i, _i, _f, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "ugbsa_paged_write": (_i, [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64,
+                               _i, _i, _i, _p]),
+    "ugbsa_paged_read": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p, _i64, _i64, _i64, _i64,
+                              _p, _i64, _i64, _i64, _i64, _p]),
+    "ugbsa_paged_select_workspace_elems": (_i64, [_i, _i, _i]),
+    "ugbsa_paged_select": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _i,
+                                _i, _f, _p, _p, _p, _p, _p, _i64, _p]),
+    "ugbsa_paged_decode_workspace_elems": (_i64, [_i, _i, _i, _i, _i]),
+    "ugbsa_paged_decode": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _p,
+                                _p, _i, _p, _i64, _i64, _i64, _p, _i64, _p]),
 }
 ABI_VERSION = 4
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """``ugbsa_paged_cache`` of the header."""
+    _fields_ = [("k_pages", _p), ("v_pages", _p),
+                ("sk_p", _i64), ("sk_h", _i64), ("sk_n", _i64),
+                ("sv_p", _i64), ("sv_h", _i64), ("sv_n", _i64),
+                ("k_scale", _p), ("v_scale", _p), ("planes", _p),
+                ("num_pages", _i), ("Hk", _i), ("D", _i), ("dtype", _i), ("cache_dtype", _i)]
+
 
 _LIB = None
 

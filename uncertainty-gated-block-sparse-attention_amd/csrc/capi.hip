@@ -62,6 +62,50 @@ int64_t kv_copy_elems(int B, int Hk, int N, int D) {
   return 2 * static_cast<int64_t>(B) * Hk * nb * ugbsa::kBlock * D;
 }
 
+// A paged cache whose pages the kernels can read, and the table that names them.
+int check_paged(const ugbsa_paged_cache* c, int H, const int32_t* lens, const int32_t* table,
+                int64_t st_b, int B, int max_pages) {
+  if (c == nullptr) return fail(UGBSA_EARG, "cache is null");
+  int rc = check_dims(B, H, c->Hk, c->D, c->dtype);
+  if (rc) return rc;
+  if (c->cache_dtype != UGBSA_CACHE_MODEL && c->cache_dtype != UGBSA_CACHE_E4M3)
+    return fail(UGBSA_EDTYPE, "unknown cache dtype %d", c->cache_dtype);
+  if (B > 65535 || H > 65535) return fail(UGBSA_EARG, "B and H must be at most 65535 (B=%d, H=%d)", B, H);
+  if (c->num_pages < 1) return fail(UGBSA_EARG, "num_pages must be positive");
+  if (max_pages < 1 || max_pages > 1 << 24)
+    return fail(UGBSA_EARG, "max_pages must lie in [1, 2^24] (%d)", max_pages);
+  if (lens == nullptr || table == nullptr) return fail(UGBSA_EARG, "lens or table is null");
+  if (st_b < 0) return fail(UGBSA_ELAYOUT, "table: negative row stride");
+  return UGBSA_OK;
+}
+
+int check_pages(const ugbsa_paged_cache* c) {
+  const bool e4m3 = c->cache_dtype == UGBSA_CACHE_E4M3;
+  const int64_t unit = e4m3 ? 16 : 8;      // elements of a 16-byte load
+  if (c->k_pages == nullptr || c->v_pages == nullptr) return fail(UGBSA_EARG, "k_pages or v_pages is null");
+  if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || c->sk_p % unit || c->sk_h % unit ||
+      c->sk_n % unit || c->sv_p % unit || c->sv_h % unit || c->sv_n % unit)
+    return fail(UGBSA_ELAYOUT, "pages must have 16-byte aligned rows");
+  if (e4m3 && (c->k_scale == nullptr || c->v_scale == nullptr))
+    return fail(UGBSA_EARG, "an e4m3 cache needs k_scale and v_scale");
+  if (e4m3 && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 7)
+    return fail(UGBSA_ELAYOUT, "scales must be 8-byte aligned");
+  if (!aligned16(c->planes)) return fail(UGBSA_ELAYOUT, "planes must be 16-byte aligned");
+  return UGBSA_OK;
+}
+
+ugbsa::PagedCache paged_cache(const ugbsa_paged_cache* c) {
+  ugbsa::PagedCache p;
+  p.k = c->k_pages, p.v = c->v_pages;
+  p.sk_p = c->sk_p, p.sk_h = c->sk_h, p.sk_n = c->sk_n;
+  p.sv_p = c->sv_p, p.sv_h = c->sv_h, p.sv_n = c->sv_n;
+  p.k_scale = c->k_scale, p.v_scale = c->v_scale;
+  p.planes = static_cast<uint16_t*>(c->planes);
+  p.num_pages = c->num_pages, p.Hk = c->Hk, p.D = c->D, p.elem = c->dtype;
+  p.e4m3 = c->cache_dtype == UGBSA_CACHE_E4M3;
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -563,6 +607,110 @@ int ugbsa_decode(const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_
                                          Hk, N, D, dtype, scale, static_cast<uint16_t*>(out), so_b,
                                          so_h, workspace, static_cast<hipStream_t>(stream)),
                     "decode");
+}
+
+int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
+                      int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
+                      const int32_t* cu_new, const int32_t* lens, const int32_t* table,
+                      int64_t st_b, int B, int T, int max_pages, void* stream) {
+  int rc = check_paged(cache, cache ? cache->Hk : 1, lens, table, st_b, B, max_pages);
+  if (rc || (rc = check_pages(cache))) return rc;
+  if (T < 0 || (cu_new == nullptr && T < B))
+    return fail(UGBSA_EARG, "T=%d: one token a sequence needs at least B=%d rows", T, B);
+  if (T == 0) return hip_result(hipSuccess, "paged_write");
+  if ((rc = check_bf16_operand("k", k, 0, sk_h, sk_t, sk_d))) return rc;
+  if ((rc = check_bf16_operand("v", v, 0, sv_h, sv_t, sv_d))) return rc;
+  if (ugbsa::paged_write_units(B, T, cu_new != nullptr) >= 1 << 24)
+    return fail(UGBSA_EARG, "more than 2^24 pages in one write (T=%d, B=%d)", T, B);
+  return hip_result(ugbsa::launch_paged_write(paged_cache(cache), static_cast<const uint16_t*>(k), sk_t,
+                                              sk_h, static_cast<const uint16_t*>(v), sv_t, sv_h, cu_new,
+                                              lens, table, st_b, B, T, max_pages,
+                                              static_cast<hipStream_t>(stream)),
+                    "paged_write");
+}
+
+int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const int32_t* table,
+                     int64_t st_b, int B, int max_pages, int N, void* k_out, int64_t sk_b,
+                     int64_t sk_h, int64_t sk_n, int64_t sk_d, void* v_out, int64_t sv_b,
+                     int64_t sv_h, int64_t sv_n, int64_t sv_d, void* stream) {
+  int rc = check_paged(cache, cache ? cache->Hk : 1, lens, table, st_b, B, max_pages);
+  if (rc || (rc = check_pages(cache))) return rc;
+  if ((rc = check_bf16_operand("k_out", k_out, sk_b, sk_h, sk_n, sk_d))) return rc;
+  if ((rc = check_bf16_operand("v_out", v_out, sv_b, sv_h, sv_n, sv_d))) return rc;
+  if (N < 1 || N > 1 << 30) return fail(UGBSA_EARG, "N must lie in [1, 2^30] (%d)", N);
+  return hip_result(ugbsa::launch_paged_read(paged_cache(cache), lens, table, st_b, B, max_pages, N,
+                                             static_cast<uint16_t*>(k_out), sk_b, sk_h, sk_n,
+                                             static_cast<uint16_t*>(v_out), sv_b, sv_h, sv_n,
+                                             static_cast<hipStream_t>(stream)),
+                    "paged_read");
+}
+
+int64_t ugbsa_paged_select_workspace_elems(int B, int Hk, int max_pages) {
+  if (B < 1 || Hk < 1 || max_pages < 1) return 0;
+  return 2 * static_cast<int64_t>(B) * Hk * max_pages;      // an fp64 score a page
+}
+
+int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                       int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                       const int32_t* table, int64_t st_b, int B, int max_pages, float scaling,
+                       int k_base, int k_slots, float tau, int32_t* kv_idx, int32_t* counts,
+                       float* sigma, uint8_t* uncertain, float* workspace,
+                       int64_t workspace_elems, void* stream) {
+  int rc = check_paged(cache, H, lens, table, st_b, B, max_pages);
+  if (rc) return rc;
+  if (cache->planes == nullptr || !aligned16(cache->planes))
+    return fail(UGBSA_EARG, "the selection needs 16-byte aligned planes");
+  if ((rc = check_bf16_operand("q", q, sq_b, sq_h, sq_m, sq_d))) return rc;
+  if (k_base < 3 || k_slots < k_base || k_slots > 1 << 24)
+    return fail(UGBSA_EARG, "3 <= k_base <= k_slots <= 2^24 needed (k_base=%d, k_slots=%d)", k_base, k_slots);
+  if (!(scaling > 0.f && scaling <= 3.4e38f)) return fail(UGBSA_EARG, "scaling must be positive and finite");
+  if (tau != tau) return fail(UGBSA_EARG, "tau is NaN");
+  if (kv_idx == nullptr || counts == nullptr) return fail(UGBSA_EARG, "kv_idx or counts is null");
+  const int64_t need = ugbsa_paged_select_workspace_elems(B, cache->Hk, max_pages);
+  if (workspace == nullptr || workspace_elems < need)
+    return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_select_workspace_elems (%lld)",
+                (long long)workspace_elems, (long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 7) return fail(UGBSA_ELAYOUT, "workspace must be 8-byte aligned");
+  if (static_cast<int64_t>(B) * cache->Hk >= 1 << 24) return fail(UGBSA_EARG, "B * Hk must be below 2^24");
+  return hip_result(ugbsa::launch_paged_select(paged_cache(cache), static_cast<const uint16_t*>(q), sq_b,
+                                               sq_h, B, H, lens, table, st_b, max_pages, scaling, k_base,
+                                               k_slots, tau, kv_idx, counts, sigma, uncertain,
+                                               reinterpret_cast<uint64_t*>(workspace),
+                                               static_cast<hipStream_t>(stream)),
+                    "paged_select");
+}
+
+int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units) {
+  if (check_dims(B, H, Hk, D, UGBSA_DTYPE_BF16) || units < 1) return 0;
+  const int64_t splits = ugbsa::paged_decode_splits(B, H, Hk, D, units);
+  return splits == 1 ? 0 : static_cast<int64_t>(B) * H * splits * (D + 2);
+}
+
+int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                       int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                       const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
+                       const int32_t* kv_idx, const int32_t* counts, int k_slots, void* out,
+                       int64_t so_b, int64_t so_h, int64_t so_d, float* workspace,
+                       int64_t workspace_elems, void* stream) {
+  int rc = check_paged(cache, H, lens, table, st_b, B, max_pages);
+  if (rc || (rc = check_pages(cache))) return rc;
+  if ((rc = check_bf16_operand("q", q, sq_b, sq_h, sq_m, sq_d))) return rc;
+  if (!(scale - scale == 0.f)) return fail(UGBSA_EARG, "scale must be finite");
+  if (kv_idx != nullptr && (k_slots < 1 || k_slots > 1 << 24))
+    return fail(UGBSA_EARG, "k_slots must lie in [1, 2^24] (%d)", k_slots);
+  if (kv_idx == nullptr && counts != nullptr) return fail(UGBSA_EARG, "counts without kv_idx");
+  if (out == nullptr || so_d != 1) return fail(UGBSA_ELAYOUT, "out must be non-null with unit head_dim stride");
+  if (static_cast<int64_t>(B) * H >= 1 << 24) return fail(UGBSA_EARG, "B * H must be below 2^24");
+  const int64_t need = ugbsa_paged_decode_workspace_elems(B, H, cache->Hk, cache->D,
+                                                          kv_idx != nullptr ? k_slots : max_pages);
+  if (need > 0 && (workspace == nullptr || workspace_elems < need))
+    return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_decode_workspace_elems (%lld)",
+                (long long)workspace_elems, (long long)need);
+  return hip_result(ugbsa::launch_paged_decode(paged_cache(cache), static_cast<const uint16_t*>(q), sq_b,
+                                               sq_h, B, H, lens, table, st_b, max_pages, kv_idx, counts,
+                                               k_slots, scale, static_cast<uint16_t*>(out), so_b, so_h,
+                                               workspace, static_cast<hipStream_t>(stream)),
+                    "paged_decode");
 }
 
 }  // extern "C"

@@ -158,4 +158,45 @@ hipError_t launch_decode(const uint16_t* q, int64_t sq_b, int64_t sq_h, const ui
                          float scale, uint16_t* out, int64_t so_b, int64_t so_h, float* ws,
                          hipStream_t stream);
 
+// The paged cache of a call (paged.h): element strides of K and V, the scales
+// and planes contiguous; elem as above, e4m3: K and V hold e4m3 bytes.
+struct PagedCache {
+  void* k = nullptr;
+  void* v = nullptr;
+  int64_t sk_p = 0, sk_h = 0, sk_n = 0, sv_p = 0, sv_h = 0, sv_n = 0;
+  uint8_t* k_scale = nullptr;
+  uint8_t* v_scale = nullptr;
+  uint16_t* planes = nullptr;
+  int num_pages = 0, Hk = 0, D = 0, elem = 0, e4m3 = 0;
+};
+
+// Workgroups per KV head of a write: B (cu_new null: a token a sequence) or a
+// bound on the pages that T ragged tokens touch.
+int64_t paged_write_units(int B, int T, bool ragged);
+hipError_t launch_paged_write(const PagedCache& c, const uint16_t* k, int64_t sk_t, int64_t sk_h,
+                              const uint16_t* v, int64_t sv_t, int64_t sv_h, const int32_t* cu_new,
+                              const int32_t* lens, const int32_t* table, int64_t st_b, int B, int T,
+                              int max_pages, hipStream_t stream);
+hipError_t launch_paged_read(const PagedCache& c, const int32_t* lens, const int32_t* table,
+                             int64_t st_b, int B, int max_pages, int N, uint16_t* ko, int64_t sok_b,
+                             int64_t sok_h, int64_t sok_n, uint16_t* vo, int64_t sov_b, int64_t sov_h,
+                             int64_t sov_n, hipStream_t stream);
+
+// Page selection of one new token; keys holds B * Hk * max_pages.
+hipError_t launch_paged_select(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h, int B,
+                               int H, const int32_t* lens, const int32_t* table, int64_t st_b,
+                               int max_pages, float scaling, int k_base, int k_slots, float tau,
+                               int32_t* kv_idx, int32_t* counts, float* sigma, uint8_t* uncertain,
+                               uint64_t* keys, hipStream_t stream);
+
+// Decode attention over pages: all of them (kv_idx null) or lists of k_slots;
+// ws holds B * H * paged_decode_splits() * (D + 2) fp32 when that is above 1
+// (units: max_pages or k_slots).
+int paged_decode_splits(int B, int H, int Hk, int D, int units);
+hipError_t launch_paged_decode(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h,
+                               int B, int H, const int32_t* lens, const int32_t* table, int64_t st_b,
+                               int max_pages, const int32_t* kv_idx, const int32_t* counts, int k_slots,
+                               float scale, uint16_t* out, int64_t so_b, int64_t so_h, float* ws,
+                               hipStream_t stream);
+
 }  // namespace ugbsa

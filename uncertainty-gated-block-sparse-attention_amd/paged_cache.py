@@ -1,0 +1,268 @@
+"""Paged key-value cache for serving: written, read back, selected from and decoded over.
+
+The dispatcher's decode attends to a contiguous ``[B, Hk, N, D]`` cache; a server keeps keys and
+values in pages of 64 tokens, the selection block, that a block table names.  Pages hold the
+model's dtype or e4m3 codes with a power-of-two scale per token and head, and beside them stands
+each page's Quest summary (K-max, K-min), kept up to date as tokens are written:
+
+    cache = PagedCache.empty(num_pages, Hk, D, torch.bfloat16, "cuda", e4m3=True)
+    paged_write(cache, k, v, block_table, seq_lens, cu_new=cu)     # prompts [T, Hk, D], packed
+    ...                                                            # per generated token:
+    paged_write(cache, k1, v1, block_table, seq_lens)              # [B, Hk, D], one token each
+    seq_lens += 1
+    sel = paged_select(q, cache, block_table, seq_lens, scale, k_base=64, k_slots=128, tau=0.01)
+    out = paged_decode(q, cache, block_table, seq_lens, scale, sel.kv_idx, sel.counts)
+    k, v = paged_read(cache, block_table, seq_lens, N)             # [B, Hk, N, D] for a prefill
+
+``block_table`` [B, max_pages] int32 and ``seq_lens`` [B] int32 live on the device: no call reads
+them on the host, and every call is asynchronous on the current stream and can be captured in a
+graph.  Lengths outside [0, 64 * max_pages] are taken as the nearer end; table entries outside the
+cache name absent pages, which are never written, read as zeros and take no part in attention.
+
+The operators have no backward pass: tensors that require gradients are refused where gradients
+are recorded.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+
+import torch
+
+import _capi
+
+PAGE = 64    # tokens per page: the selection block
+
+
+@dataclass(frozen=True)
+class PagedCache:
+    """Pages of one layer and their summaries.
+
+    k_pages, v_pages : [P, Hk, 64, D] in ``dtype`` or ``torch.float8_e4m3fn`` (unit stride on
+    head_dim, 16-byte aligned rows, any other strides)
+    k_scale, v_scale : [P, Hk, 64] uint8 contiguous, for e4m3 pages: a value is code * 2^(byte - 127)
+    planes : [P, Hk, 2, D] in ``dtype``, contiguous: K-max and K-min of each page.  Optional where
+    nothing is selected; a cache of planes alone (no pages) serves ``paged_select`` only.
+    dtype : bf16 or fp16, the format of q, k, v and of every result
+    """
+
+    k_pages: torch.Tensor | None
+    v_pages: torch.Tensor | None
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+    planes: torch.Tensor | None = None
+    dtype: torch.dtype | None = None
+    _struct: _capi.PagedCacheStruct = field(init=False, repr=False, compare=False, default=None)
+
+    def __post_init__(self):
+        k, v, planes = self.k_pages, self.v_pages, self.planes
+        assert (k is None) == (v is None), "k_pages and v_pages go together"
+        assert k is not None or planes is not None, "pages or planes required"
+        dtype = self.dtype
+        e4m3 = k is not None and k.dtype == torch.float8_e4m3fn
+        if dtype is None:
+            assert not e4m3 or planes is not None, "dtype required (e4m3 pages do not tell it)"
+            dtype = planes.dtype if planes is not None else k.dtype
+            object.__setattr__(self, "dtype", dtype)
+        code = _capi.dtype_code(dtype)
+        s = _capi.PagedCacheStruct(dtype=code,
+                                   cache_dtype=_capi.CACHE_E4M3 if e4m3 else _capi.CACHE_MODEL)
+        if k is not None:
+            assert k.dim() == 4 and k.shape == v.shape and k.shape[2] == PAGE, "pages [P, Hk, 64, D] expected"
+            assert k.dtype == v.dtype and (e4m3 or k.dtype == dtype), f"pages: {dtype} or e4m3 required"
+            s.num_pages, s.Hk, _, s.D = k.shape
+            unit = 16 // k.element_size()
+            for t in (k, v):
+                assert t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(x % unit for x in t.stride()[:3]), \
+                    "pages need unit head_dim stride and 16-byte aligned rows"
+            s.k_pages, s.v_pages = k.data_ptr(), v.data_ptr()
+            s.sk_p, s.sk_h, s.sk_n, _ = k.stride()
+            s.sv_p, s.sv_h, s.sv_n, _ = v.stride()
+            assert e4m3 == (self.k_scale is not None) == (self.v_scale is not None), \
+                "scales go with e4m3 pages"
+            if e4m3:
+                for t in (self.k_scale, self.v_scale):
+                    assert t.shape == k.shape[:3] and t.dtype == torch.uint8 and t.is_contiguous() \
+                        and t.data_ptr() % 8 == 0, "scales [P, Hk, 64] uint8 contiguous expected"
+                s.k_scale, s.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        if planes is not None:
+            if k is None:
+                assert planes.dim() == 4, "planes [P, Hk, 2, D] expected"
+                s.num_pages, s.Hk, _, s.D = planes.shape
+            assert tuple(planes.shape) == (s.num_pages, s.Hk, 2, s.D) and planes.dtype == dtype \
+                and planes.is_contiguous() and planes.data_ptr() % 16 == 0, "planes [P, Hk, 2, D] expected"
+            s.planes = planes.data_ptr()
+        assert s.D in (64, 128, 256), f"head_dim {s.D} not supported (64, 128, 256)"
+        tensors = [t for t in (k, v, self.k_scale, self.v_scale, planes) if t is not None]
+        assert all(t.is_cuda and t.device == tensors[0].device for t in tensors), "HIP tensors of one device required"
+        object.__setattr__(self, "_struct", s)
+
+    @classmethod
+    def empty(cls, num_pages, Hk, D, dtype, device, e4m3=False, summaries=True):
+        """Uninitialised pages: every slot a sequence reads is written first."""
+        shape = (num_pages, Hk, PAGE, D)
+        pages = torch.float8_e4m3fn if e4m3 else dtype
+        k, v = (torch.empty(shape, dtype=pages, device=device) for _ in range(2))
+        ks, vs = (torch.empty(shape[:3], dtype=torch.uint8, device=device) if e4m3 else None for _ in range(2))
+        planes = torch.empty(num_pages, Hk, 2, D, dtype=dtype, device=device) if summaries else None
+        return cls(k, v, ks, vs, planes, dtype)
+
+    @property
+    def device(self):
+        return (self.planes if self.k_pages is None else self.k_pages).device
+
+
+@dataclass
+class PagedSelection:
+    kv_idx: torch.Tensor       # int32 [B, Hk, k_slots] ascending pages of the sequence, then max_pages
+    counts: torch.Tensor       # int32 [B, Hk] pages listed
+    sigma: torch.Tensor        # fp32 [B, Hk] margin at the cut
+    uncertain: torch.Tensor    # uint8 [B, Hk]
+
+
+def _check_operand(name, t, cache, shape):
+    """A 16-bit tensor of the cache's dtype and device that the kernels read in place."""
+    assert t.dtype == cache.dtype, f"{name}: {cache.dtype} required, got {t.dtype}"
+    assert t.device == cache.device, f"{name} must be on the cache's device"
+    assert tuple(t.shape) == shape, f"{name} {list(shape)} expected, got {list(t.shape)}"
+    assert not (t.requires_grad and torch.is_grad_enabled()), "the paged operators have no backward pass"
+    if t.is_neg():
+        t = t.resolve_neg()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
+        t = t.contiguous()
+    return t
+
+
+def _check_table(cache, block_table, seq_lens):
+    """B of a call's table and lengths."""
+    assert block_table.dim() == 2 and block_table.dtype == torch.int32 and (
+        block_table.stride(1) == 1 or block_table.shape[1] == 1), "block_table [B, max_pages] int32 expected"
+    B = block_table.shape[0]
+    assert B >= 1 and block_table.shape[1] >= 1, "block_table is empty"
+    _check_ints("seq_lens", seq_lens, cache, (B,))
+    assert block_table.device == cache.device, "block_table must be on the cache's device"
+    return B
+
+
+def _check_ints(name, t, cache, shape):
+    assert t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(), \
+        f"{name} {list(shape)} int32 contiguous expected"
+    assert t.device == cache.device, f"{name} must be on the cache's device"
+
+
+def _call(cache, what, fn, *args):
+    """fn(cache, *args, stream) on the cache's device."""
+    device = cache.device
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(ctypes.addressof(cache._struct), *args, _capi.stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.addressof(cache._struct), *args, _capi.stream_ptr(device))
+    _capi.check(rc, what)
+
+
+def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
+    """New tokens into the cache, quantised if it holds e4m3, and its page summaries.
+
+    k, v : [T, Hk, D], the new tokens of all sequences, packed
+    cu_new : [B + 1] int32, sequence b's are rows cu_new[b] .. cu_new[b + 1] - 1; None: one token
+    each, row b
+    seq_lens : tokens cached before this call; the new ones follow them (the caller adds them up)
+
+    Rows behind the last sequence and tokens past the table are left out.  Two sequences may share
+    pages, but not ones that both write to.
+    """
+    assert cache.k_pages is not None, "a cache of planes alone has no pages"
+    B = _check_table(cache, block_table, seq_lens)
+    T, s = k.shape[0], cache._struct
+    k = _check_operand("k", k, cache, (T, s.Hk, s.D))
+    v = _check_operand("v", v, cache, (T, s.Hk, s.D))
+    if cu_new is not None:
+        _check_ints("cu_new", cu_new, cache, (B + 1,))
+    _call(cache, "paged_write", _capi.lib().ugbsa_paged_write, k.data_ptr(), *k.stride(),
+          v.data_ptr(), *v.stride(), _capi.ptr(cu_new), seq_lens.data_ptr(), block_table.data_ptr(),
+          block_table.stride(0), B, T, block_table.shape[1])
+
+
+def paged_read(cache, block_table, seq_lens, n, out=None):
+    """(k, v) [B, Hk, n, D] in ``cache.dtype``: the first n cached tokens of every sequence, zeros
+    past its length (``out``: a pair of such tensors to fill)."""
+    assert cache.k_pages is not None, "a cache of planes alone has no pages"
+    B, s = _check_table(cache, block_table, seq_lens), cache._struct
+    shape = (B, s.Hk, n, s.D)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
+    k, v = out
+    for t in out:
+        assert tuple(t.shape) == shape and t.dtype == cache.dtype and t.device == cache.device, \
+            f"out: a pair of {list(shape)} in {cache.dtype} expected"
+    _call(cache, "paged_read", _capi.lib().ugbsa_paged_read, seq_lens.data_ptr(), block_table.data_ptr(),
+          block_table.stride(0), B, block_table.shape[1], n, k.data_ptr(), *k.stride(),
+          v.data_ptr(), *v.stride())
+    return k, v
+
+
+def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=0.0):
+    """The pages one new token attends to, per sequence and KV head: the decode counterpart of the
+    v2 selector.
+
+    q : [B, H, 1, D]; seq_lens counts the new token.  A page's score is the Quest bound of its
+    summary, maximised over the KV head's query heads and summed in fp64.  The first and the last
+    page are kept, and the best others by (score desc, page asc) up to ``k_base`` pages, or
+    ``k_slots`` where the margin at the cut, sigma = clamp((s(k) - s(k + 1)) / max(s(1) - s(k + 1),
+    1e-9), 0, 2) over the scaled scores of the others, k = k_base - 2, is below ``tau``
+    (``Selector.router_tau``'s role; 0 keeps k_base throughout).  A sequence's list depends on no
+    other sequence of the batch.  Returns a ``PagedSelection`` for ``paged_decode``.
+    """
+    assert cache.planes is not None, "the cache keeps no page summaries"
+    B, s = _check_table(cache, block_table, seq_lens), cache._struct
+    H = q.shape[1] if q.dim() == 4 else 0
+    q = _check_operand("q", q, cache, (B, H, 1, s.D))
+    device, max_pages = cache.device, block_table.shape[1]
+    r = PagedSelection(torch.empty(B, s.Hk, k_slots, dtype=torch.int32, device=device),
+                       torch.empty(B, s.Hk, dtype=torch.int32, device=device),
+                       torch.empty(B, s.Hk, dtype=torch.float32, device=device),
+                       torch.empty(B, s.Hk, dtype=torch.uint8, device=device))
+    lib = _capi.lib()
+    n = lib.ugbsa_paged_select_workspace_elems(B, s.Hk, max_pages)
+    ws = torch.empty(n, dtype=torch.float32, device=device)
+    _call(cache, "paged_select", lib.ugbsa_paged_select, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
+          block_table.data_ptr(), block_table.stride(0), B, max_pages, float(scaling), k_base, k_slots,
+          float(tau), r.kv_idx.data_ptr(), r.counts.data_ptr(), r.sigma.data_ptr(), r.uncertain.data_ptr(),
+          ws.data_ptr(), n)
+    return r
+
+
+def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=None, out=None):
+    """Attention of one new token per sequence over its cached tokens, of every page or of the
+    listed ones.
+
+    q : [B, H, 1, D]; seq_lens counts the new token, which ``paged_write`` has put in the cache
+    kv_idx : [B, Hk, k_slots] int32, the pages (numbered within the sequence, each at most once)
+    that the KV head's query heads attend to; counts [B, Hk] int32: how many entries count (None:
+    all).  Entries that are no page of the sequence are skipped.
+    Returns [B, 1, H, D] contiguous, the dispatcher's layout (``out`` if given).  A sequence without
+    a key gives zeros.
+    """
+    assert cache.k_pages is not None, "a cache of planes alone has no pages"
+    B, s = _check_table(cache, block_table, seq_lens), cache._struct
+    H = q.shape[1] if q.dim() == 4 else 0
+    q = _check_operand("q", q, cache, (B, H, 1, s.D))
+    slots = 0
+    if kv_idx is not None:
+        slots = kv_idx.shape[-1]
+        _check_ints("kv_idx", kv_idx, cache, (B, s.Hk, slots))
+    if counts is not None:
+        _check_ints("counts", counts, cache, (B, s.Hk))
+    if out is None:
+        out = torch.empty(B, 1, H, s.D, dtype=cache.dtype, device=cache.device)
+    assert tuple(out.shape) == (B, 1, H, s.D) and out.dtype == cache.dtype and out.device == cache.device
+    lib = _capi.lib()
+    n = lib.ugbsa_paged_decode_workspace_elems(B, H, s.Hk, s.D, slots or block_table.shape[1])
+    ws = torch.empty(n, dtype=torch.float32, device=cache.device) if n else None
+    _call(cache, "paged_decode", lib.ugbsa_paged_decode, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
+          block_table.data_ptr(), block_table.stride(0), B, block_table.shape[1], float(scale),
+          _capi.ptr(kv_idx), _capi.ptr(counts), slots, out.data_ptr(), out.stride(0), out.stride(2),
+          out.stride(3), _capi.ptr(ws), n)
+    return out
