@@ -29,129 +29,299 @@ __device__ __forceinline__ double key_double(uint64_t k) {
   return __builtin_bit_cast(double, (k >> 63) ? (k ^ (1ull << 63)) : ~k);
 }
 
-// keys [B, Hk, max_pages] of the pages between the first and the last of each row:
-// one wavefront a page, D / 64 dims a lane.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const int lo = static_cast<int>(u), hi = static_cast<int>(u >> 32);
+  const uint32_t l = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(lo, CTRL, 0xF, 0xF, true));
+  const uint32_t h = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(hi, CTRL, 0xF, 0xF, true));
+  return x + __builtin_bit_cast(double, static_cast<uint64_t>(h) << 32 | l);
+}
+// Sum over groups of LP = 8, 16 or 32 lanes in the VALU (every lane gets it): lanes
+// xor 1 and 2, the mirrored half row, the mirrored row, the neighbouring row.
+template <int LP>
+__device__ __forceinline__ double group_sum(double x) {
+  x = dpp_add<0xB1>(x);
+  x = dpp_add<0x4E>(x);
+  x = dpp_add<0x141>(x);
+  if constexpr (LP >= 16) x = dpp_add<0x140>(x);
+  if constexpr (LP >= 32) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto l = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+    const auto h = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+    x = __builtin_bit_cast(double, static_cast<uint64_t>(h[0]) << 32 | l[0]) +
+        __builtin_bit_cast(double, static_cast<uint64_t>(h[1]) << 32 | l[1]);
+  }
+  return x;
+}
+
+// The score of one page by its definition, read from memory: for planes that hold
+// infinities or NaN, where the sums below are not the definition's.
 template <typename E, int D>
+__device__ double plain_score(const uint16_t* pl, const uint16_t* q) {
+  double s = 0.0;
+  for (int d = 0; d < D; ++d) {
+    const float x = E::to_f32(q[d]);
+    s += static_cast<double>(x) * E::to_f32(x >= 0.f ? pl[d] : pl[D + d]);
+  }
+  return s;
+}
+
+constexpr int kScoreAhead = 2;          // steps of a wavefront whose loads are in flight
+
+// keys [B, Hk, max_pages] of the pages between the first and the last of each row.
+//
+// D / 8 lanes take a page, 8 dims each, so a wavefront reads 64 / (D / 8) pages' whole
+// planes per step, two 16-byte loads a lane.  Twice the score is
+//   sum_d q_d (kmax_d + kmin_d) + |q_d| (kmax_d - kmin_d),
+// two fp64 FMAs a dim and head (|q| is a source modifier) and no select by the sign
+// of q; the sums and differences are shared by the GC heads of a pass, whose q stay
+// in registers as fp64.  fp64 FMAs run at the fp32 rate here, and the pass is
+// bound by them and the 4 D bytes a page about equally at five heads.
+template <typename E, int D, int GC>
 __global__ __launch_bounds__(256) void paged_score_kernel(
     PagedCache c, const uint16_t* __restrict__ q, int64_t sq_b, int64_t sq_h, int grp,
     const int32_t* __restrict__ lens, const int32_t* __restrict__ table, int64_t st_b, int max_pages,
-    uint64_t* __restrict__ keys) {
-  constexpr int L = D / 64;
+    int per_wave, uint64_t* __restrict__ keys) {
+  constexpr int LP = D / 8, NP = 64 / LP;        // lanes a page, pages a step
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int g = blockIdx.y, b = blockIdx.z;
+  const int g = blockIdx.x % c.Hk, b = blockIdx.y;   // a page's heads run side by side
   const int nb = (cached_len(lens, b, max_pages) + kBlock - 1) / kBlock;
-  const uint16_t* qb = q + b * sq_b + g * grp * sq_h + L * lane;
-  const int64_t row = static_cast<int64_t>(b) * c.Hk + g;
-  for (int j = blockIdx.x * 4 + wave; j < nb - 1; j += gridDim.x * 4) {
-    if (j == 0) continue;
-    const int page = table[b * st_b + j];
-    double best = -INFINITY;
-    if (page >= 0 && page < c.num_pages) {
-      const uint16_t* pl = c.planes + (static_cast<int64_t>(page) * c.Hk + g) * 2 * D + L * lane;
-      double hi[L], lo[L];
+  // this wavefront's pages [j0, j1), at most the 64 whose table entries its lanes hold
+  const int j0 = (blockIdx.x / c.Hk * 4 + wave) * per_wave, j1 = min(j0 + per_wave, nb);
+  if (j0 >= j1) return;
+  const int sub = lane / LP, d0 = 8 * (lane % LP);
+  const int mine = j0 + lane < j1 ? table[b * st_b + j0 + lane] : -1;
+  uint64_t* kr = keys + (static_cast<int64_t>(b) * c.Hk + g) * max_pages;
+
+  u32x4 his[kScoreAhead], los[kScoreAhead];
+  int pages[kScoreAhead];
+  auto load = [&](int j, u32x4& hi, u32x4& lo, int& page) {
+    page = __shfl(mine, j - j0 + sub, 64);
+    if (j + sub >= j1 || page < 0 || page >= c.num_pages) page = -1;
+    const uint16_t* pl = c.planes + (static_cast<int64_t>(max(page, 0)) * c.Hk + g) * 2 * D + d0;
+    hi = *reinterpret_cast<const u32x4*>(pl);
+    lo = *reinterpret_cast<const u32x4*>(pl + D);
+  };
+  for (int h0 = 0; h0 < grp; h0 += GC) {
+    double qd[GC][8];
+    const uint16_t* qh = q + b * sq_b + (g * grp + h0) * sq_h;
 #pragma unroll
-      for (int i = 0; i < L; ++i) hi[i] = E::to_f32(pl[i]), lo[i] = E::to_f32(pl[D + i]);
-      for (int h = 0; h < grp; ++h) {
-        double acc = 0.0;
+    for (int h = 0; h < GC; ++h) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(qh + min(h, grp - 1 - h0) * sq_h + d0);
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-          const float x = E::to_f32(qb[h * sq_h + i]);
-          acc += static_cast<double>(x) * (x >= 0.f ? hi[i] : lo[i]);
-        }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) acc += __shfl_xor(acc, off, 64);
-        best = (acc > best || acc != acc) ? acc : best;
+      for (int i = 0; i < 4; ++i) {
+        qd[h][2 * i] = E::to_f32(x[i] & 0xFFFFu);
+        qd[h][2 * i + 1] = E::to_f32(x[i] >> 16);
       }
     }
-    if (lane == 0) keys[row * max_pages + j] = double_key(best);
+    // the steps in flight: step s of a round of kScoreAhead in registers of its own
+#pragma unroll
+    for (int s = 0; s < kScoreAhead; ++s)
+      if (j0 + s * NP < j1) load(j0 + s * NP, his[s], los[s], pages[s]);
+    for (int jr = j0; jr < j1; jr += kScoreAhead * NP) {
+      static_for<kScoreAhead>([&](auto sc) {
+        constexpr int s = sc;
+        const int j = jr + s * NP;
+        if (j >= j1) return;
+        const u32x4 hi = his[s], lo = los[s];
+        const int at = pages[s];
+        double sum[8], dif[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double a = E::to_f32(hi[i] & 0xFFFFu), z = E::to_f32(lo[i] & 0xFFFFu);
+          const double a1 = E::to_f32(hi[i] >> 16), z1 = E::to_f32(lo[i] >> 16);
+          sum[2 * i] = a + z, dif[2 * i] = a - z;
+          sum[2 * i + 1] = a1 + z1, dif[2 * i + 1] = a1 - z1;
+        }
+        const int ahead = j + kScoreAhead * NP;
+        if (ahead < j1) load(ahead, his[s], los[s], pages[s]);
+        double best = -INFINITY;
+        bool odd = false;
+#pragma unroll
+        for (int h = 0; h < GC; ++h) {
+          double acc = 0.0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            acc = __builtin_fma(qd[h][i], sum[i], acc);
+            acc = __builtin_fma(__builtin_fabs(qd[h][i]), dif[i], acc);
+          }
+          acc = group_sum<LP>(acc);
+          odd |= acc != acc;
+          best = acc > best ? acc : best;
+        }
+        best *= 0.5;
+        if (lane % LP != 0 || j + sub >= j1) return;
+        if (at < 0) {
+          best = -INFINITY;
+        } else if (odd || best == INFINITY || best == -INFINITY) {
+          best = -INFINITY;
+          const uint16_t* pl = c.planes + (static_cast<int64_t>(at) * c.Hk + g) * 2 * D;
+          for (int h = 0; h < min(GC, grp - h0); ++h) {
+            const double x = plain_score<E, D>(pl, qh + h * sq_h);
+            best = (x > best || x != x) ? x : best;
+          }
+        }
+        uint64_t key = double_key(best);
+        if (h0 > 0) {                                // the earlier heads' best, by this lane
+          const uint64_t before = kr[j + sub];
+          key = before > key ? before : key;
+        }
+        kr[j + sub] = key;
+      });
+    }
   }
 }
 
-// Sum over the workgroup (every thread gets it); red: 4 ints.
-__device__ __forceinline__ int wg_sum(int x, int* red) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
-}
-__device__ __forceinline__ uint64_t wg_max(uint64_t x, uint64_t* red) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const uint64_t y = __shfl_xor(static_cast<unsigned long long>(x), off, 64);
-    x = y > x ? y : x;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-  __syncthreads();
-  uint64_t a = red[0] > red[1] ? red[0] : red[1], z = red[2] > red[3] ? red[2] : red[3];
-  return a > z ? a : z;
-}
+constexpr int kPickKeys = 8;            // keys a thread holds in registers
 
-// One workgroup per row: cut, margin, gate and the ascending list.
-__global__ __launch_bounds__(256) void paged_pick_kernel(
+// One workgroup of NT threads per row: cut, margin, gate and the ascending list.
+// REG: rows of up to 8 NT pages, whose keys stay in registers.
+//
+// The k-th largest key: the keys between the row's extremes go into 4 NT bins of
+// equal width, the bin that holds rank k is found by a scan over the bins, and its
+// few keys are ranked against each other; a bin of more than NT is binned again.
+// Bins relative to the extremes matter: the digits of the keys as they stand share
+// their sign and most of the exponent.
+template <int NT, bool REG>
+__global__ __launch_bounds__(NT) void paged_pick_kernel(
     const uint64_t* __restrict__ keys, const int32_t* __restrict__ lens, int Hk, int max_pages,
     float scaling, int k_base, int k_slots, float tau, int32_t* __restrict__ kv_idx,
     int32_t* __restrict__ counts, float* __restrict__ sigma, uint8_t* __restrict__ uncertain) {
-  __shared__ int hist[256];
-  __shared__ int red[4];
-  __shared__ uint64_t red64[4];
-  __shared__ uint64_t s_prefix;
-  __shared__ int s_left;
-  const int tid = threadIdx.x;
+  constexpr int kBits = 31 - __builtin_clz(4 * NT);
+  __shared__ int hist[4 * NT];
+  __shared__ uint64_t cand[NT];
+  __shared__ uint64_t s_max[NT / 64], s_min[NT / 64];
+  __shared__ int s_cnt[NT / 64], s_cnt2[NT / 64];
+  __shared__ uint64_t s_kth;
+  __shared__ int s_bin, s_left, s_in, s_cands;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const int b = static_cast<int>(row / Hk);
   const int nb = (cached_len(lens, b, max_pages) + kBlock - 1) / kBlock;
   const uint64_t* kr = keys + row * max_pages;
   int32_t* list = kv_idx + row * k_slots;
-
-  // the k-th largest key of pages 1 .. nb - 2 (1 <= k <= nb - 2): digit by digit
-  auto kth = [&](int k) {
-    uint64_t prefix = 0;
-    int left = k;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      __syncthreads();
-      hist[tid] = 0;
-      __syncthreads();
-      for (int j = 1 + tid; j < nb - 1; j += 256) {
-        const uint64_t x = kr[j];
-        if (shift == 56 || (x >> (shift + 8)) == (prefix >> (shift + 8)))
-          atomicAdd(&hist[(x >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255;
-        while (hist[d] < left) left -= hist[d--];
-        s_prefix = prefix | (static_cast<uint64_t>(d) << shift);
-        s_left = left;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      left = s_left;
-    }
-    return prefix;
-  };
-
+  int keep = min(k_base, nb);
   float sg = 2.f;
   bool unsure = false;
-  uint64_t cut = 0;
-  int keep = min(k_base, nb);
-  if (nb > k_base) {
-    const int k = k_base - 2;
-    const uint64_t a = kth(k);
-    int not_below = 0;
-    uint64_t below = 0, top = 0;
-    for (int j = 1 + tid; j < nb - 1; j += 256) {
-      const uint64_t x = kr[j];
-      if (x >= a) ++not_below;
-      else if (x > below) below = x;
-      if (x > top) top = x;
+
+  // thread t has pages [t chunk, (t + 1) chunk); key 0: no competitor
+  const int chunk = (nb + NT - 1) / NT, j0 = tid * chunk;
+  auto read = [&](int i) -> uint64_t {
+    const int j = j0 + i;
+    return i < chunk && j > 0 && j < nb - 1 ? kr[j] : 0;
+  };
+  uint64_t held[kPickKeys];
+  if (REG && nb > k_base) {
+#pragma unroll
+    for (int i = 0; i < kPickKeys; ++i) held[i] = read(i);
+  }
+  auto each = [&](auto&& f) {
+    if constexpr (REG) {
+#pragma unroll
+      for (int i = 0; i < kPickKeys; ++i)
+        if (i < chunk) f(i, held[i]);
+    } else {
+      for (int i = 0; i < chunk; ++i) f(i, read(i));
     }
-    const uint64_t next = wg_sum(not_below, red) > k ? a : 0;
-    below = wg_max(below, red64);
-    top = wg_max(top, red64);
-    const double sc = scaling, c = key_double(next ? next : below) * sc;
+  };
+  // maximum and (of the nonzero keys) minimum over the workgroup, and a count
+  auto reduce = [&](uint64_t mx, uint64_t mn, int n, uint64_t& all_mx, uint64_t& all_mn, int& all_n) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      const uint64_t a = __shfl_xor(static_cast<unsigned long long>(mx), off, 64);
+      const uint64_t z = __shfl_xor(static_cast<unsigned long long>(mn), off, 64);
+      mx = a > mx ? a : mx;
+      mn = z < mn ? z : mn;
+      n += __shfl_xor(n, off, 64);
+    }
+    __syncthreads();
+    if (lane == 0) s_max[wave] = mx, s_min[wave] = mn, s_cnt[wave] = n;
+    __syncthreads();
+    all_mx = 0, all_mn = ~0ull, all_n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+      all_mx = s_max[w] > all_mx ? s_max[w] : all_mx;
+      all_mn = s_min[w] < all_mn ? s_min[w] : all_mn;
+      all_n += s_cnt[w];
+    }
+  };
+  auto kth = [&](int left, uint64_t lo, uint64_t hi) -> uint64_t {
+    for (;;) {
+      if (lo == hi) return lo;
+      const int width = 64 - __builtin_clzll(hi - lo);
+      const int shift = width > kBits ? width - kBits : 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hist[NT * i + tid] = 0;
+      if (tid == 0) s_cands = 0;
+      __syncthreads();
+      each([&](int, uint64_t x) {
+        if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
+      });
+      __syncthreads();
+      // thread t: the four bins below 4 NT - 4 t, an inclusive scan from the top
+      const int top = 4 * NT - 1 - 4 * tid;
+      int n[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += n[i] = hist[top - i];
+      int incl = sum;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += y;
+      }
+      if (lane == 63) s_cnt[wave] = incl;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) incl += s_cnt[w];
+      if (incl - sum < left && left <= incl) {       // exactly one thread
+        int before = incl - sum, i = 0;
+        while (before + n[i] < left) before += n[i++];
+        s_bin = top - i;
+        s_left = left - before;
+        s_in = n[i];
+      }
+      __syncthreads();
+      lo += static_cast<uint64_t>(s_bin) << shift;
+      hi = lo + ((1ull << shift) - 1);
+      left = s_left;
+      if (shift == 0) return lo;
+      if (s_in <= NT) break;
+    }
+    each([&](int, uint64_t x) {
+      if (x >= lo && x <= hi) cand[atomicAdd(&s_cands, 1)] = x;
+    });
+    __syncthreads();
+    const int m = s_cands;
+    if (tid < m) {
+      const uint64_t x = cand[tid];
+      int above = 0, same = 0;
+      for (int i = 0; i < m; ++i) above += cand[i] > x, same += cand[i] == x;
+      if (above < left && left <= above + same) s_kth = x;     // equal keys write the same
+    }
+    __syncthreads();
+    return s_kth;
+  };
+
+  uint64_t cut = 0;
+  if (nb > k_base) {
+    uint64_t mx = 0, mn = ~0ull, top, low, unused;
+    int n = 0, all;
+    each([&](int, uint64_t x) {
+      mx = x > mx ? x : mx;
+      if (x != 0 && x < mn) mn = x;
+    });
+    reduce(mx, mn, 0, top, low, all);
+    const int k = k_base - 2;
+    const uint64_t a = kth(k, low, top);
+    mx = 0;
+    each([&](int, uint64_t x) {
+      n += x >= a;
+      if (x < a && x > mx) mx = x;
+    });
+    uint64_t below;
+    reduce(mx, ~0ull, n, below, unused, all);
+    const double sc = scaling, c = key_double(all > k ? a : below) * sc;
     const double reach = key_double(top) * sc - c, ratio = (key_double(a) * sc - c) / (reach > 1e-9 ? reach : 1e-9);
     const double clamped = ratio < 0.0 ? 0.0 : (ratio > 2.0 ? 2.0 : ratio);
     sg = static_cast<float>(clamped);
@@ -159,46 +329,46 @@ __global__ __launch_bounds__(256) void paged_pick_kernel(
     cut = a;
     if (unsure) {
       keep = min(k_slots, nb);
-      if (nb > keep) cut = kth(keep - 2);
+      if (nb > keep && keep > k_base) cut = kth(keep - 2, low, top);
     }
   }
-  // pages above the cut, and the lowest of those at it
-  int above = 0;
-  if (nb > keep) {
-    for (int j = 1 + tid; j < nb - 1; j += 256) above += kr[j] > cut;
-    above = wg_sum(above, red);
-  }
-  const int ties = keep - 2 - above;
-  int ties_before = 0, out_before = 0;
-  for (int j0 = 0; j0 < nb; j0 += 256) {
-    const int j = j0 + tid;
-    bool in = j < nb, tie = false;
-    if (in && nb > keep && j > 0 && j < nb - 1) {
-      const uint64_t x = kr[j];
-      in = x > cut;
-      tie = x == cut;
+  if (nb <= keep) {
+    for (int s = tid; s < k_slots; s += NT) list[s] = s < nb ? s : max_pages;
+  } else {
+    // kept: the first and the last page, those above the cut, and the lowest of
+    // those at it; a page's place is what is kept of the pages before it
+    int over = 0, ties = 0;
+    auto forced = [&](int i) { return j0 + i == 0 || j0 + i == nb - 1; };
+    each([&](int i, uint64_t x) {
+      if (j0 + i >= nb) return;
+      over += forced(i) || x > cut;
+      ties += !forced(i) && x == cut;
+    });
+    int o = over, e = ties;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(o, off, 64), z = __shfl_up(e, off, 64);
+      if (lane >= off) o += y, e += z;
     }
-    // ranks over the workgroup, ties first
-    for (int pass = 0; pass < 2; ++pass) {
-      const uint64_t bal = __ballot(pass == 0 ? tie : in);
-      __syncthreads();
-      if ((tid & 63) == 0) red[tid >> 6] = __popcll(bal);
-      __syncthreads();
-      int rank = lanes_below(bal), all = 0;
-      for (int w = 0; w < 4; ++w) {
-        if (w < (tid >> 6)) rank += red[w];
-        all += red[w];
-      }
-      if (pass == 0) {
-        if (tie) in = ties_before + rank < ties;
-        ties_before += all;
-      } else {
-        if (in) list[out_before + rank] = j;
-        out_before += all;
-      }
+    __syncthreads();
+    if (lane == 63) s_cnt[wave] = o, s_cnt2[wave] = e;
+    __syncthreads();
+    int all_over = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+      if (w < wave) o += s_cnt[w], e += s_cnt2[w];
+      all_over += s_cnt[w];
     }
+    o -= over, e -= ties;
+    const int room = keep - all_over;
+    each([&](int i, uint64_t x) {
+      if (j0 + i >= nb) return;
+      const bool tie = !forced(i) && x == cut;
+      if (forced(i) || x > cut || (tie && e < room)) list[o + min(e, room)] = j0 + i;
+      o += forced(i) || x > cut;
+      e += tie;
+    });
+    for (int s = keep + tid; s < k_slots; s += NT) list[s] = max_pages;
   }
-  for (int s = keep + tid; s < k_slots; s += 256) list[s] = max_pages;
   if (tid == 0) {
     counts[row] = keep;
     if (sigma != nullptr) sigma[row] = sg;
@@ -213,13 +383,40 @@ static hipError_t launch_paged_select_t(const PagedCache& c, const uint16_t* q, 
                                         int k_base, int k_slots, float tau, int32_t* kv_idx,
                                         int32_t* counts, float* sigma, uint8_t* uncertain, uint64_t* keys,
                                         hipStream_t stream) {
-  const dim3 grid(min((max_pages + 3) / 4, 256), c.Hk, B);
-  paged_score_kernel<E, D><<<grid, 256, 0, stream>>>(c, q, sq_b, sq_h, H / c.Hk, lens, table, st_b,
-                                                     max_pages, keys);
+  // heads a pass: an even share of the group, at most the 8 whose q fit the registers
+  const int grp = H / c.Hk, passes = (grp + 7) / 8, gc = (grp + passes - 1) / passes;
+  // pages a wavefront: as many as leave the card 4096 wavefronts, from one step to
+  // 16 (64 sequences of up to 128K tokens, both launches: 8 / 16 / 32 / 64 pages 62.7 /
+  // 56.4 / 62.1 / 79 us; with four steps' loads in flight instead of two, which cost a
+  // wavefront per SIMD, 78.8 / 67.1 / 75 / 88)
+  constexpr int NP = 512 / D;
+  const int64_t pages = static_cast<int64_t>(B) * c.Hk * max_pages;
+  int per = static_cast<int>(pages / 4096 < 16 ? pages / 4096 : 16) / NP * NP;
+  if (per < NP) per = NP;
+  const dim3 grid((max_pages + 4 * per - 1) / (4 * per) * c.Hk, B);
+#define UGBSA_SCORE(GC_)                                                                          \
+  paged_score_kernel<E, D, GC_><<<grid, 256, 0, stream>>>(c, q, sq_b, sq_h, grp, lens, table, st_b, \
+                                                          max_pages, per, keys)
+  if (gc == 1) UGBSA_SCORE(1);
+  else if (gc == 2) UGBSA_SCORE(2);
+  else if (gc <= 4) UGBSA_SCORE(4);
+  else if (gc == 5) UGBSA_SCORE(5);
+  else if (gc <= 7) UGBSA_SCORE(7);
+  else UGBSA_SCORE(8);
+#undef UGBSA_SCORE
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  paged_pick_kernel<<<dim3(B * c.Hk), 256, 0, stream>>>(keys, lens, c.Hk, max_pages, scaling, k_base,
-                                                        k_slots, tau, kv_idx, counts, sigma, uncertain);
+  // few threads for few keys, where barriers cost more than steps (one sequence of 512
+  // pages, both launches: 64 / 128 / 256 / 512 threads 12.2 / 11.3 / 11.3 / 12.4 us)
+#define UGBSA_PICK(NT_, REG_)                                                                         \
+  paged_pick_kernel<NT_, REG_><<<dim3(B * c.Hk), NT_, 0, stream>>>(keys, lens, c.Hk, max_pages, scaling, \
+                                                                   k_base, k_slots, tau, kv_idx, counts, \
+                                                                   sigma, uncertain)
+  if (max_pages <= 128 * kPickKeys) UGBSA_PICK(128, true);
+  else if (max_pages <= 256 * kPickKeys) UGBSA_PICK(256, true);
+  else if (max_pages <= 512 * kPickKeys) UGBSA_PICK(512, true);
+  else UGBSA_PICK(512, false);
+#undef UGBSA_PICK
   return hipGetLastError();
 }
 
