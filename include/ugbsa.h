@@ -317,7 +317,7 @@ int ugbsa_decode(const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_
  * Slots past a sequence's length may hold anything, NaN included. */
 typedef struct {
   void* k_pages; /* [num_pages, Hk, 64, D] of dtype or e4m3, head_dim stride 1, */
-  void* v_pages; /* 16-byte aligned rows; the other strides in elements */
+  void* v_pages; /* 16-byte aligned rows; the other strides in elements, a slot's at most 2^24 */
   int64_t sk_p, sk_h, sk_n;
   int64_t sv_p, sv_h, sv_n;
   uint8_t* k_scale; /* [num_pages, Hk, 64] contiguous, e4m3 only: a value is */
@@ -375,17 +375,19 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
                        float* sigma, uint8_t* uncertain, float* workspace,
                        int64_t workspace_elems, void* stream);
 
-/* fp32 elements of a ugbsa_paged_decode workspace (0: none is needed, or sizes no
- * call takes).  units: max_pages, or k_slots of a call with lists. */
+/* fp32 elements of a ugbsa_paged_decode workspace (0 for sizes no call takes).
+ * units: max_pages, or k_slots of a call with lists. */
 int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units);
 
 /* Decode over pages — attention of one query row per head over the tokens below
  * lens[b]: of every page (kv_idx NULL), or of the pages that kv_idx [B, Hk,
  * k_slots] lists for the KV head, the first counts[b][h] entries (counts NULL:
  * all k_slots).  Entries outside the sequence's pages are skipped; a page must
- * not be listed twice.  q [B, H, 1, D], out [B, H, D] of dtype with any b and h
- * strides; B, H <= 65535.  A row without a key, or whose every weight is 0, gives
- * zeros. */
+ * not be listed twice.  q [B, H, 1, D], out [B, H, D] of dtype with
+ * even strides (4-byte aligned rows); B, H <= 65535, B * H * max_pages (or k_slots)
+ * below 2^31 - 2^16.  A row without a key, or whose every weight is 0, gives
+ * zeros.  workspace (16-byte aligned) holds the pieces of rows that several
+ * workgroups share; its contents on entry do not matter. */
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
                        int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
                        const int32_t* table, int64_t st_b, int B, int max_pages, float scale,

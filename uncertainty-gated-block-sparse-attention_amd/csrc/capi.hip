@@ -86,6 +86,9 @@ int check_pages(const ugbsa_paged_cache* c) {
   if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || c->sk_p % unit || c->sk_h % unit ||
       c->sk_n % unit || c->sv_p % unit || c->sv_h % unit || c->sv_n % unit)
     return fail(UGBSA_ELAYOUT, "pages must have 16-byte aligned rows");
+  // lane offsets within a page are 32-bit
+  if (c->sk_n < 0 || c->sv_n < 0 || c->sk_n > 1 << 24 || c->sv_n > 1 << 24)
+    return fail(UGBSA_ELAYOUT, "the pages' slot strides must lie in [0, 2^24]");
   if (e4m3 && (c->k_scale == nullptr || c->v_scale == nullptr))
     return fail(UGBSA_EARG, "an e4m3 cache needs k_scale and v_scale");
   if (e4m3 && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 7)
@@ -682,8 +685,8 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
 
 int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units) {
   if (check_dims(B, H, Hk, D, UGBSA_DTYPE_BF16) || units < 1) return 0;
-  const int64_t splits = ugbsa::paged_decode_splits(B, H, Hk, D, units);
-  return splits == 1 ? 0 : static_cast<int64_t>(B) * H * splits * (D + 2);
+  // one size for both cache types: e4m3 keeps more workgroups resident
+  return ugbsa::paged_decode_ws_elems(B, H, Hk, D, true, units);
 }
 
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
@@ -698,14 +701,20 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
   if (!(scale - scale == 0.f)) return fail(UGBSA_EARG, "scale must be finite");
   if (kv_idx != nullptr && (k_slots < 1 || k_slots > 1 << 24))
     return fail(UGBSA_EARG, "k_slots must lie in [1, 2^24] (%d)", k_slots);
+  // the rows' pages are numbered end to end in 32 bits
+  if (static_cast<int64_t>(B) * H * (kv_idx != nullptr ? k_slots : max_pages) > INT32_MAX - 65536)
+    return fail(UGBSA_EARG, "B * H * pages a row must be below 2^31 - 2^16");
   if (kv_idx == nullptr && counts != nullptr) return fail(UGBSA_EARG, "counts without kv_idx");
   if (out == nullptr || so_d != 1) return fail(UGBSA_ELAYOUT, "out must be non-null with unit head_dim stride");
+  if ((reinterpret_cast<uintptr_t>(out) & 3) || so_b % 2 || so_h % 2)
+    return fail(UGBSA_ELAYOUT, "out must have 4-byte aligned rows");
   if (static_cast<int64_t>(B) * H >= 1 << 24) return fail(UGBSA_EARG, "B * H must be below 2^24");
   const int64_t need = ugbsa_paged_decode_workspace_elems(B, H, cache->Hk, cache->D,
                                                           kv_idx != nullptr ? k_slots : max_pages);
-  if (need > 0 && (workspace == nullptr || workspace_elems < need))
+  if (workspace == nullptr || workspace_elems < need)
     return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_decode_workspace_elems (%lld)",
                 (long long)workspace_elems, (long long)need);
+  if (!aligned16(workspace)) return fail(UGBSA_ELAYOUT, "workspace must be 16-byte aligned");
   return hip_result(ugbsa::launch_paged_decode(paged_cache(cache), static_cast<const uint16_t*>(q), sq_b,
                                                sq_h, B, H, lens, table, st_b, max_pages, kv_idx, counts,
                                                k_slots, scale, static_cast<uint16_t*>(out), so_b, so_h,

@@ -190,9 +190,8 @@ hipError_t launch_paged_select(const PagedCache& c, const uint16_t* q, int64_t s
                                uint64_t* keys, hipStream_t stream);
 
 // Decode attention over pages: all of them (kv_idx null) or lists of k_slots;
-// ws holds B * H * paged_decode_splits() * (D + 2) fp32 when that is above 1
-// (units: max_pages or k_slots).
-int paged_decode_splits(int B, int H, int Hk, int D, int units);
+// ws holds paged_decode_ws_elems fp32 (units: max_pages or k_slots).
+int64_t paged_decode_ws_elems(int B, int H, int Hk, int D, bool e4m3, int units);
 hipError_t launch_paged_decode(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h,
                                int B, int H, const int32_t* lens, const int32_t* table, int64_t st_b,
                                int max_pages, const int32_t* kv_idx, const int32_t* counts, int k_slots,

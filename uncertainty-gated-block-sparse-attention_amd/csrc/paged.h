@@ -24,6 +24,9 @@
 namespace ugbsa {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef const __attribute__((address_space(1))) u32x4 gu32x4;
+typedef const __attribute__((address_space(1))) u32x2 gu32x2;
+typedef const __attribute__((address_space(1))) uint32_t gu32;
 
 // Eight e4m3 codes (lo: dims 0-3, hi: 4-7) times 2^(byte - 127) in E's format (exact).
 template <typename E>

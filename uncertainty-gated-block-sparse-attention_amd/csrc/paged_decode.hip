@@ -16,7 +16,7 @@ constexpr int kPdStep = 32;       // keys per wavefront step: half a page
 // wavefronts' O of 16 heads would take 66 KiB of LDS.
 __host__ __device__ constexpr int pd_heads(int D) { return D > 128 ? 8 : 16; }
 
-// The row's pages a list or the block table names.
+// The pages that a call's lists or block table name.
 struct PagedRows {
   const int32_t* lens;
   const int32_t* table;
@@ -27,290 +27,451 @@ struct PagedRows {
   int k_slots;
 };
 
-// Pages (or list entries) of row (b, h).
-__device__ __forceinline__ int row_units(const PagedRows& r, int Hk, int b, int h, int len) {
+// The work of a call is its rows' pages (or list entries), laid end to end: a group
+// is a sequence, or with lists a (sequence, KV head), its members the (KV head,)
+// head chunks that visit its n pages, one row each.  Workgroup w takes units
+// [w per, (w + 1) per) of the line, however the batch's lengths are spread, so
+// rows begin and end inside workgroups.  A row that one workgroup holds is written
+// by it; the pieces of the others meet in paged_combine_kernel: piece 2 w of
+// workgroup w continues a row, piece 2 w + 1 begins one.
+constexpr int kPdUnits = 2;       // fewest units of a workgroup: a half page a wavefront
+
+struct PagedGroups {
+  int groups, members, Hk;
+};
+
+__device__ __forceinline__ int group_units(const PagedRows& r, int Hk, int i) {
+  const int b = r.kv_idx == nullptr ? i : i / Hk;
+  const int len = cached_len(r.lens, b, r.max_pages);
   if (r.kv_idx == nullptr) return (len + kBlock - 1) / kBlock;
-  if (len == 0) return 0;
-  const int n = r.counts == nullptr ? r.k_slots : r.counts[static_cast<int64_t>(b) * Hk + h];
-  return min(max(n, 0), r.k_slots);
+  const int n = r.counts == nullptr ? r.k_slots : r.counts[i];
+  return len == 0 ? 0 : min(max(n, 0), r.k_slots);
+}
+
+// Wavefronts per SIMD that the registers allow, which is also the workgroups per CU
+// that a call launches: a line cut into more than are resident leaves a second round
+// of them (us, 256 / 512 / 768 / 1024 workgroups: 24 sequences of up to 16K tokens,
+// 40/8 heads, bf16 86.1 / 78.4 / 88.1 / 80.1; 32 x 64K in e4m3 1127 / 758 / 727 / 858; 4
+// of up to 64K at 16/2 heads, head_dim 256 44.1 / 50.3 / 55.1 / 64.5).
+__host__ __device__ constexpr int pd_occupancy(int D, bool F8) {
+  return D == 64 ? 4 : (D == 128 ? (F8 ? 3 : 2) : (F8 ? 2 : 1));
 }
 
 template <typename E, int D, bool F8>
-__global__ __launch_bounds__(64 * kPdWaves) void paged_decode_kernel(
-    PagedCache c, PagedRows rows, const uint16_t* __restrict__ q, int64_t sq_b, int64_t sq_h, int grp,
-    int chunks, int splits, float scale_log2, uint16_t* __restrict__ out, int64_t so_b, int64_t so_h,
-    float* __restrict__ part, float* __restrict__ ml) {
+__global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_decode_kernel(
+    PagedCache c, PagedRows rows, PagedGroups gr, const uint16_t* __restrict__ q, int64_t sq_b,
+    int64_t sq_h, int grp, int chunks, float scale_log2, uint16_t* __restrict__ out, int64_t so_b,
+    int64_t so_h, int* __restrict__ starts, float* __restrict__ part, float* __restrict__ ml) {
   constexpr int KS = D / 32, DT = D / 16, NH = pd_heads(D);
   constexpr int DPL = D / 16;                    // dims a lane loads per key of V
   // 16-bit rows are read 8 dims a load, or 4 at head_dim 64 (VW = dims a load)
   constexpr int VW = F8 ? DPL : (D == 64 ? 4 : 8), VL = DPL / VW;
+  constexpr int SZ = F8 ? 1 : 2;
   __shared__ float s_o[kPdWaves][NH][D + 4];
   __shared__ float s_ml[kPdWaves][NH][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ int s_sum[kPdWaves], s_start[2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
-  const int split = blockIdx.x, ck = blockIdx.y % chunks, g = blockIdx.y / chunks, b = blockIdx.z;
-  const int heads = min(NH, grp - ck * NH);   // live columns
-  const int h0 = g * grp + ck * NH;
 
-  const int len = cached_len(rows.lens, b, rows.max_pages);
-  const int units = row_units(rows, c.Hk, b, g, len);
-  const int per = (units + splits - 1) / splits;
-  const int u0 = min(units, split * per), u1 = min(units, u0 + per);
-  const int32_t* table = rows.table + b * rows.st_b;
-  const int32_t* list = rows.kv_idx == nullptr
-                            ? nullptr
-                            : rows.kv_idx + (static_cast<int64_t>(b) * c.Hk + g) * rows.k_slots;
-
-  // Q^T columns (heads past the group are zero and never written).  Contraction
-  // slot 8 g4 + i of step ks is dim 32 ks + 8 g4 + i; e4m3 rows, 16 codes a load,
-  // take dim 64 (ks / 2) + 16 g4 + 8 (ks % 2) + i.
-  bf16x8 qf[KS];
+  // The line's length, and the row where this workgroup's units begin: up to 64
+  // groups lie in a wavefront's lanes, more in the workgroup's threads, some each.
+  const bool few = gr.groups <= 64;
+  const int each = few ? 1 : (gr.groups + 255) / 256, i0 = (few ? lane : threadIdx.x) * each;
+  int mine = 0;
+  for (int i = i0; i < min(i0 + each, gr.groups); ++i) mine += group_units(rows, gr.Hk, i);
+  mine *= gr.members;
+  int incl = mine;
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const int d = F8 ? 64 * (ks / 2) + 16 * g4 + 8 * (ks % 2) : 32 * ks + 8 * g4;
-    qf[ks] = r16 < heads ? load_bf16x8(q + b * sq_b + (h0 + r16) * sq_h + d) : zero_bf16x8();
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += y;
   }
+  int total = __builtin_amdgcn_readlane(incl, 63);
+  if (!few) {
+    if (lane == 63) s_sum[wave] = incl;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kPdWaves; ++w) {
+      if (w < wave) incl += s_sum[w];
+      total += s_sum[w];
+    }
+  }
+  const int per = max(kPdUnits, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
+  if (blockIdx.x == 0 && (!few || wave == 0)) {    // for the joining kernel
+    int s = incl - mine;
+    for (int i = i0; i < min(i0 + each, gr.groups); ++i) {
+      starts[i] = s;
+      s += group_units(rows, gr.Hk, i) * gr.members;
+    }
+    if (threadIdx.x == 0) starts[gr.groups] = total, starts[gr.groups + 1] = per;
+  }
+  if (static_cast<int64_t>(blockIdx.x) * per >= total) return;
+  int u = blockIdx.x * per;
+  const int u_end = min(u + per, total);
+  int group, n, off0;                              // off0: units of the group before u
+  if (few) {
+    group = __builtin_popcountll(__ballot(incl <= u));
+    const int units = __builtin_amdgcn_readlane(mine, group);
+    off0 = u - (__builtin_amdgcn_readlane(incl, group) - units);
+    n = static_cast<int>(static_cast<uint32_t>(units) / static_cast<uint32_t>(gr.members));
+  } else {
+    if (incl - mine <= u && u < incl) {            // one thread
+      int s = incl - mine;
+      for (int i = i0;; ++i) {
+        const int k = group_units(rows, gr.Hk, i) * gr.members;
+        if (u < s + k) {
+          s_start[0] = i;
+          s_start[1] = u - s;
+          break;
+        }
+        s += k;
+      }
+    }
+    __syncthreads();
+    group = __builtin_amdgcn_readfirstlane(s_start[0]);
+    off0 = __builtin_amdgcn_readfirstlane(s_start[1]);
+    n = __builtin_amdgcn_readfirstlane(group_units(rows, gr.Hk, group));
+  }
+  int member = static_cast<int>(static_cast<uint32_t>(off0) / static_cast<uint32_t>(n));
+  int p0 = off0 - member * n;
+
   // MFMA row R of S^T tile mt is key 8 (R >> 2) + 4 mt + (R & 3) of the step:
   // the lane then holds keys 8 g4 + 4 mt + i
   const int krow = 8 * (r16 >> 2) + (r16 & 3);
+  // byte offsets of the lane's K and V rows within a step (the strides fit, checked on the host)
+  const uint32_t k_lane = static_cast<uint32_t>((krow * c.sk_n + (F8 ? 16 : 8) * g4) * SZ);
+  const uint32_t v_lane = static_cast<uint32_t>((8 * g4 * c.sv_n + VW * r16) * SZ);
+  const uint32_t k_row = static_cast<uint32_t>(c.sk_n * SZ), v_row = static_cast<uint32_t>(c.sv_n * SZ);
 
-  // step st of the row: the half page's keys, how many of them exist, its page
-  struct Step { int64_t page; int base, left; };
-  auto step_at = [&](int st) {
-    const int u = st >> 1;
-    const int blk = list == nullptr ? u : list[u];
-    int page = -1;
-    if (blk >= 0 && blk < rows.max_pages && blk * kBlock < len) page = table[blk];
-    const bool there = page >= 0 && page < c.num_pages;
-    Step s;
-    s.page = there ? page : 0;               // an absent page: page 0's keys, none of them live
-    s.base = kPdStep * (st & 1);
-    s.left = there ? len - blk * kBlock - s.base : 0;
-    return s;
-  };
+  for (;;) {
+    // this workgroup's piece [p0, p1) of row (b, g, ck)
+    const int p1 = min(n, p0 + u_end - u);
+    const int b = rows.kv_idx == nullptr ? group : group / gr.Hk;
+    const int g = rows.kv_idx == nullptr ? member / chunks : group % gr.Hk;
+    const int ck = rows.kv_idx == nullptr ? member % chunks : member;
+    const int heads = min(NH, grp - ck * NH);    // live columns
+    const int h0 = g * grp + ck * NH;
+    const int len = cached_len(rows.lens, b, rows.max_pages);
+    const int32_t* table = rows.table + b * rows.st_b;
+    const int32_t* list = rows.kv_idx == nullptr
+                              ? nullptr
+                              : rows.kv_idx + (static_cast<int64_t>(b) * gr.Hk + g) * rows.k_slots;
 
-  u32x4 kf[2][F8 ? KS / 2 : KS];
-  float ksc[2], vsc[8];
-  uint32_t vr[8][F8 ? DPL / 4 : DPL / 2];    // V[8 g4 + i][the lane's dims]
-  auto load_k = [&](const Step& s) {
+    // Q^T columns (heads past the group are zero and never written).  Contraction
+    // slot 8 g4 + i of step ks is dim 32 ks + 8 g4 + i; e4m3 rows, 16 codes a load,
+    // take dim 64 (ks / 2) + 16 g4 + 8 (ks % 2) + i.
+    bf16x8 qf[KS];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const int slot = s.base + krow + 4 * mt;
-      const int64_t at = s.page * c.sk_p + g * c.sk_h + slot * c.sk_n;
-      if constexpr (F8) {
-        const uint8_t* row = static_cast<const uint8_t*>(c.k) + at + 16 * g4;
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = F8 ? 64 * (ks / 2) + 16 * g4 + 8 * (ks % 2) : 32 * ks + 8 * g4;
+      qf[ks] = r16 < heads ? load_bf16x8(q + b * sq_b + (h0 + r16) * sq_h + d) : zero_bf16x8();
+    }
+
+    gchar* const kg = (gchar*)c.k + g * c.sk_h * SZ;
+    gchar* const vg = (gchar*)c.v + g * c.sv_h * SZ;
+
+    // step st of the row: its half page's keys, how many of them exist, its page
+    struct Step { int64_t page; int base, left; };
+    auto step_at = [&](int st) {
+      const int x = st >> 1;
+      const int blk = list == nullptr ? x : list[x];
+      int page = -1;
+      if (blk >= 0 && blk < rows.max_pages && blk * kBlock < len) page = table[blk];
+      const bool there = page >= 0 && page < c.num_pages;
+      Step s;
+      s.page = there ? page : 0;             // an absent page: page 0's keys, none of them live
+      s.base = kPdStep * (st & 1);
+      s.left = there ? len - blk * kBlock - s.base : 0;
+      return s;
+    };
+
+    u32x4 kf[2][F8 ? KS / 2 : KS];
+    float ksc[2], vsc[8];
+    uint32_t vr[8][F8 ? DPL / 4 : DPL / 2];  // V[8 g4 + i][the lane's dims]
+    auto load_k = [&](const Step& s) {
+      gchar* half = kg + s.page * c.sk_p * SZ + static_cast<uint32_t>(s.base) * k_row;
 #pragma unroll
-        for (int j = 0; j < KS / 2; ++j) kf[mt][j] = *reinterpret_cast<const u32x4*>(row + 64 * j);
-        ksc[mt] = e8m0(c.k_scale[(s.page * c.Hk + g) * kBlock + slot]);
-      } else {
-        const uint16_t* row = static_cast<const uint16_t*>(c.k) + at + 8 * g4;
+      for (int mt = 0; mt < 2; ++mt) {
+        gchar* row = half + 4u * mt * k_row;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[mt][ks] = *reinterpret_cast<const u32x4*>(row + 32 * ks);
+        for (int j = 0; j < (F8 ? KS / 2 : KS); ++j)
+          kf[mt][j] = *reinterpret_cast<gu32x4*>(row + (k_lane + 64u * j));
+        if constexpr (F8)
+          ksc[mt] = e8m0(c.k_scale[(s.page * gr.Hk + g) * kBlock + s.base + krow + 4 * mt]);
       }
-    }
-  };
-  auto load_v = [&](const Step& s) {
-    if constexpr (F8) {
-      const u32x2 sc = *reinterpret_cast<const u32x2*>(
-          c.v_scale + (s.page * c.Hk + g) * kBlock + s.base + 8 * g4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) vsc[i] = e8m0((sc[i / 4] >> (8 * (i % 4))) & 0xFFu);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t at = s.page * c.sv_p + g * c.sv_h + (s.base + 8 * g4 + i) * c.sv_n + VW * r16;
+    };
+    auto load_v = [&](const Step& s) {
+      gchar* half = vg + s.page * c.sv_p * SZ + static_cast<uint32_t>(s.base) * v_row;
       if constexpr (F8) {
-        const uint8_t* row = static_cast<const uint8_t*>(c.v) + at;
-        if constexpr (DPL == 4) {
-          vr[i][0] = *reinterpret_cast<const uint32_t*>(row);
-        } else if constexpr (DPL == 8) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(row);
-          vr[i][0] = x[0], vr[i][1] = x[1];
-        } else {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(row);
+        const u32x2 sc = *reinterpret_cast<const u32x2*>(
+            c.v_scale + (s.page * gr.Hk + g) * kBlock + s.base + 8 * g4);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vr[i][j] = x[j];
-        }
-      } else {
-        const uint16_t* row = static_cast<const uint16_t*>(c.v) + at;
+        for (int i = 0; i < 8; ++i) vsc[i] = e8m0((sc[i / 4] >> (8 * (i % 4))) & 0xFFu);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        gchar* row = half + static_cast<uint32_t>(i) * v_row;
+        constexpr int LB = VW * SZ;          // bytes of a load
 #pragma unroll
         for (int l = 0; l < VL; ++l) {
-          if constexpr (VW == 8) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(row + 128 * l);
+          gchar* at = row + (v_lane + 256u * l);
+          if constexpr (LB == 16) {
+            const u32x4 x = *reinterpret_cast<gu32x4*>(at);
 #pragma unroll
             for (int j = 0; j < 4; ++j) vr[i][4 * l + j] = x[j];
-          } else {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(row);
+          } else if constexpr (LB == 8) {
+            const u32x2 x = *reinterpret_cast<gu32x2*>(at);
             vr[i][0] = x[0], vr[i][1] = x[1];
+          } else {
+            vr[i][0] = *reinterpret_cast<gu32*>(at);
           }
         }
       }
+    };
+
+    f32x4 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;  // of head r16; l over this lane's keys
+
+    const int st1 = 2 * p1;
+    int st = 2 * p0 + wave;
+    Step cur{}, nxt{}, far{};
+    if (st < st1) {
+      cur = step_at(st);
+      load_k(cur);
+      load_v(cur);
+      if (st + kPdWaves < st1) nxt = step_at(st + kPdWaves);
     }
-  };
-
-  f32x4 o[DT];
+    for (; st < st1; st += kPdWaves) {
+      const bool more = st + kPdWaves < st1;
+      // the page after the next one's: its number is on the way during this step
+      if (st + 2 * kPdWaves < st1) far = step_at(st + 2 * kPdWaves);
+      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;    // of head r16; l over this lane's keys
-
-  const int st1 = 2 * u1;
-  int st = 2 * u0 + wave;
-  Step cur{}, nxt{};
-  if (st < st1) {
-    cur = step_at(st);
-    load_k(cur);
-    load_v(cur);
-  }
-  for (; st < st1; st += kPdWaves) {
-    const bool more = st + kPdWaves < st1;
-    if (more) nxt = step_at(st + kPdWaves);
-    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        bf16x8 a;
-        if constexpr (F8)
-          a = e4m3_x8<E>(kf[mt][ks / 2][2 * (ks % 2)], kf[mt][ks / 2][2 * (ks % 2) + 1], ksc[mt]);
-        else
-          a = __builtin_bit_cast(bf16x8, kf[mt][ks]);
-        s[mt] = E::mfma(a, qf[ks], s[mt]);
-      }
-    if (more) load_k(nxt);
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * scale_log2;
-    if (cur.left < kPdStep) {       // keys past the end, or an absent page
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (8 * g4 + e >= cur.left) {
-          x[e] = -INFINITY;
-          if constexpr (F8) vsc[e] = 1.f;
-#pragma unroll
-          for (int j = 0; j < (F8 ? DPL / 4 : DPL / 2); ++j) vr[e][j] = 0u;
+        for (int mt = 0; mt < 2; ++mt) {
+          bf16x8 a;
+          if constexpr (F8)
+            a = e4m3_x8<E>(kf[mt][ks / 2][2 * (ks % 2)], kf[mt][ks / 2][2 * (ks % 2) + 1], ksc[mt]);
+          else
+            a = __builtin_bit_cast(bf16x8, kf[mt][ks]);
+          s[mt] = E::mfma(a, qf[ks], s[mt]);
         }
-    }
-    float mx = x[0];
+      if (more) load_k(nxt);
+      float x[8];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-    const float m_new = fmaxf(m, quad_rows_max(mx));
-    const float off = m_new == -INFINITY ? 0.f : m_new;   // no finite score so far: weights 0
-    const float alpha = __builtin_amdgcn_exp2f(m - off);
-    m = m_new;
-    float p[8], sum = 0.f;
+      for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * scale_log2;
+      if (cur.left < kPdStep) {     // keys past the end, or an absent page
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(x[e] - off);
-      sum += p[e];
-    }
-    l = l * alpha + sum;
+        for (int e = 0; e < 8; ++e)
+          if (8 * g4 + e >= cur.left) {
+            x[e] = -INFINITY;
+            if constexpr (F8) vsc[e] = 1.f;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-    // P rounded once to the element format, as the other attention kernels do
-    u32x4 pw;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) pw[j] = E::pack2(p[2 * j], p[2 * j + 1]);
-    const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
-    // operand dt: the lane's dim dt of the eight keys
-#pragma unroll
-    for (int d2 = 0; d2 < DT / 2; ++d2) {
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (F8) w[i] = e4m3_pair<E>(vr[i][d2 / 2], vsc[i], d2 % 2);
-        else w[i] = vr[i][d2];
+            for (int j = 0; j < (F8 ? DPL / 4 : DPL / 2); ++j) vr[e][j] = 0u;
+          }
       }
+      float mx = x[0];
 #pragma unroll
-      for (int odd = 0; odd < 2; ++odd) {
-        u32x4 a;
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+      const float m_new = fmaxf(m, quad_rows_max(mx));
+      const float off = m_new == -INFINITY ? 0.f : m_new;   // no finite score so far: weights 0
+      const float alpha = __builtin_amdgcn_exp2f(m - off);
+      m = m_new;
+      float p[8], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          a[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], odd ? 0x07060302u : 0x05040100u);
-        o[2 * d2 + odd] = E::mfma(__builtin_bit_cast(bf16x8, a), pb, o[2 * d2 + odd]);
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(x[e] - off);
+        sum += p[e];
       }
+      l = l * alpha + sum;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      // P rounded once to the element format, as the other attention kernels do
+      u32x4 pw;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pw[j] = E::pack2(p[2 * j], p[2 * j + 1]);
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
+      // operand dt: the lane's dim dt of the eight keys
+#pragma unroll
+      for (int d2 = 0; d2 < DT / 2; ++d2) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (F8) w[i] = e4m3_pair<E>(vr[i][d2 / 2], vsc[i], d2 % 2);
+          else w[i] = vr[i][d2];
+        }
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+          u32x4 a;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            a[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], odd ? 0x07060302u : 0x05040100u);
+          o[2 * d2 + odd] = E::mfma(__builtin_bit_cast(bf16x8, a), pb, o[2 * d2 + odd]);
+        }
+      }
+      if (more) load_v(nxt);
+      cur = nxt;
+      nxt = far;
     }
-    if (more) load_v(nxt);
-    cur = nxt;
-  }
-  l = quad_rows_sum(l);
+    l = quad_rows_sum(l);
 
-  // O^T row R = 4 g4 + i of operand dt is dim VW R + dt % VW of load dt / VW
-  // (128 dims a load)
-  if (r16 < heads) {
+    // O^T row R = 4 g4 + i of operand dt is dim VW R + dt % VW of load dt / VW
+    // (128 dims a load)
+    if (r16 < heads) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s_o[wave][r16][128 * (dt / VW) + VW * (4 * g4 + i) + dt % VW] = o[dt][i];
-    if (g4 == 0) {
-      s_ml[wave][r16][0] = m;
-      s_ml[wave][r16][1] = l;
-    }
-  }
-  __syncthreads();
-
-  const int H = c.Hk * grp;
-  for (int i = threadIdx.x; i < heads * D; i += 64 * kPdWaves) {
-    const int hh = i / D, d = i % D;
-    float mm = s_ml[0][hh][0];
-#pragma unroll
-    for (int w = 1; w < kPdWaves; ++w) mm = fmaxf(mm, s_ml[w][hh][0]);
-    const float off = mm == -INFINITY ? 0.f : mm;
-    float acc = 0.f, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < kPdWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(s_ml[w][hh][0] - off);
-      acc += s_o[w][hh][d] * f;
-      ll += s_ml[w][hh][1] * f;
-    }
-    const int64_t bh = static_cast<int64_t>(b) * H + h0 + hh;
-    if (splits == 1) {
-      // no key at all: zeros
-      out[b * so_b + (h0 + hh) * so_h + d] =
-          static_cast<uint16_t>(E::pack2(ll == 0.f ? 0.f : acc / ll, 0.f) & 0xFFFFu);
-    } else {
-      part[(bh * splits + split) * D + d] = acc;
-      if (d == 0) {
-        ml[(bh * splits + split) * 2] = mm;
-        ml[(bh * splits + split) * 2 + 1] = ll;
+        for (int i = 0; i < 4; ++i)
+          s_o[wave][r16][128 * (dt / VW) + VW * (4 * g4 + i) + dt % VW] = o[dt][i];
+      if (g4 == 0) {
+        s_ml[wave][r16][0] = m;
+        s_ml[wave][r16][1] = l;
       }
     }
+    __syncthreads();
+
+    const bool whole = p0 == 0 && p1 == n;
+    const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (p0 == 0 ? 1 : 0);
+    for (int i = threadIdx.x; i < heads * D; i += 64 * kPdWaves) {
+      const int hh = i / D, d = i % D;
+      float mm = s_ml[0][hh][0];
+#pragma unroll
+      for (int w = 1; w < kPdWaves; ++w) mm = fmaxf(mm, s_ml[w][hh][0]);
+      const float off = mm == -INFINITY ? 0.f : mm;
+      float acc = 0.f, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPdWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(s_ml[w][hh][0] - off);
+        acc += s_o[w][hh][d] * f;
+        ll += s_ml[w][hh][1] * f;
+      }
+      if (whole) {
+        // no key at all: zeros
+        out[b * so_b + (h0 + hh) * so_h + d] =
+            static_cast<uint16_t>(E::pack2(ll == 0.f ? 0.f : acc / ll, 0.f) & 0xFFFFu);
+      } else {
+        part[(piece * NH + hh) * D + d] = acc;
+        if (d == 0) {
+          ml[(piece * NH + hh) * 2] = mm;
+          ml[(piece * NH + hh) * 2 + 1] = ll;
+        }
+      }
+    }
+
+    u += p1 - p0;
+    if (u >= u_end) return;
+    // the next row with pages
+    p0 = 0;
+    if (++member == gr.members) {
+      member = 0;
+      for (++group;; group += 64) {
+        const int k = group + lane < gr.groups ? group_units(rows, gr.Hk, group + lane) : 0;
+        const uint64_t some = __ballot(k > 0);
+        if (some == 0) continue;                   // u < total: a later group has pages
+        const int f = __builtin_ctzll(some);
+        n = __builtin_amdgcn_readlane(k, f);
+        group += f;
+        break;
+      }
+    }
+    __syncthreads();                               // s_o is read by all before it is written again
   }
 }
 
-// out of one (b, head) from its splits.
-constexpr int kPdMaxSplits = 512;
+// out of the heads whose rows several workgroups hold, and zeros for rows without
+// pages: 256 threads a head, four dims each and the pieces in runs of 1024 / D.
+constexpr int kPdMaxWorkgroups = 1024;
+constexpr int kPdCombineThreads = 256;
 template <typename E, int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(const float* __restrict__ part,
-                                                            const float* __restrict__ ml, int H,
-                                                            int splits, uint16_t* __restrict__ out,
-                                                            int64_t so_b, int64_t so_h) {
-  __shared__ float s_w[kPdMaxSplits];
-  const int64_t bh = blockIdx.x;
-  const float* mlb = ml + bh * splits * 2;
-  float mx = -INFINITY;
-  for (int s = 0; s < splits; ++s) mx = fmaxf(mx, mlb[2 * s]);
+__global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
+    const int* __restrict__ starts, const float* __restrict__ part, const float* __restrict__ ml,
+    PagedGroups gr, int grp, int chunks, bool lists, uint16_t* __restrict__ out, int64_t so_b,
+    int64_t so_h) {
+  constexpr int RUNS = 4 * kPdCombineThreads / D, NH = pd_heads(D), PT = kPdMaxWorkgroups / kPdCombineThreads;
+  __shared__ float s_w[kPdMaxWorkgroups];
+  __shared__ float s_red[kPdCombineThreads / 64][2];
+  __shared__ f32x4 s_acc[RUNS][D / 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int H = gr.Hk * grp, b = blockIdx.x / H, h = blockIdx.x % H;
+  const int g = h / grp, ck = h % grp / NH, hh = h % grp % NH;
+  const int group = lists ? b * gr.Hk + g : b, member = lists ? ck : g * chunks + ck;
+  const uint32_t s0 = starts[group], s1 = starts[group + 1], per = starts[gr.groups + 1];
+  const uint32_t n = (s1 - s0) / static_cast<uint32_t>(gr.members), first = s0 + member * n;
+  uint16_t* o = out + b * so_b + h * so_h;
+  if (n == 0) {
+    if (tid < D) o[tid] = 0;
+    return;
+  }
+  const int wa = static_cast<int>(first / per);
+  const int pieces = static_cast<int>((first + n - 1) / per) - wa + 1;
+  if (pieces == 1) return;
+  auto at = [&](int i) { return (2 * (wa + i) + (i == 0 ? 1 : 0)) * NH + hh; };
+  float ms[PT], ls[PT], mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    const int x = kPdCombineThreads * i + tid;
+    ms[i] = x < pieces ? ml[2 * at(x)] : -INFINITY;
+    ls[i] = x < pieces ? ml[2 * at(x) + 1] : 0.f;
+    mx = fmaxf(mx, ms[i]);
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+  if (lane == 0) s_red[wave][0] = mx;
+  __syncthreads();
+  mx = s_red[0][0];
+#pragma unroll
+  for (int w = 1; w < kPdCombineThreads / 64; ++w) mx = fmaxf(mx, s_red[w][0]);
   const float off = mx == -INFINITY ? 0.f : mx;
-  for (int s = threadIdx.x; s < splits; s += 256) s_w[s] = __builtin_amdgcn_exp2f(mlb[2 * s] - off);
+  float lt = 0.f;
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    const float w = __builtin_amdgcn_exp2f(ms[i] - off);
+    if (kPdCombineThreads * i + tid < pieces) s_w[kPdCombineThreads * i + tid] = w;
+    lt += ls[i] * w;
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) lt += __shfl_xor(lt, s, 64);
+  if (lane == 0) s_red[wave][1] = lt;
   __syncthreads();
   float total = 0.f;
-  for (int s = 0; s < splits; ++s) total += mlb[2 * s + 1] * s_w[s];
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float acc = 0.f;
-    for (int s = 0; s < splits; ++s) acc += part[(bh * splits + s) * D + d] * s_w[s];
-    out[(bh / H) * so_b + (bh % H) * so_h + d] =
-        static_cast<uint16_t>(E::pack2(total == 0.f ? 0.f : acc / total, 0.f) & 0xFFFFu);
+#pragma unroll
+  for (int w = 0; w < kPdCombineThreads / 64; ++w) total += s_red[w][1];
+
+  const int run = tid / (D / 4), d4 = tid % (D / 4);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = run; i < pieces; i += RUNS)
+    acc += reinterpret_cast<const f32x4*>(part + static_cast<int64_t>(at(i)) * D)[d4] * s_w[i];
+  s_acc[run][d4] = acc;
+  __syncthreads();
+  if (tid < D / 4) {
+#pragma unroll
+    for (int r = 1; r < RUNS; ++r) acc += s_acc[r][tid];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = total == 0.f ? 0.f : acc[j] / total;
+    uint32_t* w = reinterpret_cast<uint32_t*>(o) + 2 * tid;
+    w[0] = E::pack2(acc[0], acc[1]);
+    w[1] = E::pack2(acc[2], acc[3]);
   }
 }
 
-// Splits of each row's pages: enough workgroups that every CU holds two, each
-// with a page a wavefront pair.
-int paged_decode_splits(int B, int H, int Hk, int D, int units) {
+// Workgroups of a call: as many as the card holds at once, unless the call's rows
+// cannot have kPdUnits for each.
+static int paged_decode_workgroups(int B, int H, int Hk, int D, bool e4m3, int units) {
   const int64_t rows = static_cast<int64_t>(B) * Hk * ((H / Hk + pd_heads(D) - 1) / pd_heads(D));
-  int64_t want = 512 / rows;
-  if (want > units / 2) want = units / 2;
-  if (want > kPdMaxSplits) want = kPdMaxSplits;
-  return want < 1 ? 1 : static_cast<int>(want);
+  const int64_t most = (rows * units + kPdUnits - 1) / kPdUnits;
+  const int64_t resident = 256 * pd_occupancy(D, e4m3);
+  return static_cast<int>(most < resident ? most : resident);
+}
+
+// The pieces, their (m, l), then starts [groups + 2] int32.
+int64_t paged_decode_ws_elems(int B, int H, int Hk, int D, bool e4m3, int units) {
+  const int64_t pieces = 2 * static_cast<int64_t>(paged_decode_workgroups(B, H, Hk, D, e4m3, units)) * pd_heads(D);
+  return pieces * (D + 2) + static_cast<int64_t>(B) * Hk + 2;
 }
 
 template <typename E, int D, bool F8>
@@ -319,14 +480,19 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
                                         uint16_t* out, int64_t so_b, int64_t so_h, float* ws,
                                         hipStream_t stream) {
   const int grp = H / c.Hk, chunks = (grp + pd_heads(D) - 1) / pd_heads(D);
-  const int splits = paged_decode_splits(B, H, c.Hk, D, rows.kv_idx ? rows.k_slots : rows.max_pages);
+  const bool lists = rows.kv_idx != nullptr;
+  const int wgs = paged_decode_workgroups(B, H, c.Hk, D, F8, lists ? rows.k_slots : rows.max_pages);
+  const PagedGroups gr{lists ? B * c.Hk : B, lists ? chunks : c.Hk * chunks, c.Hk};
+  const int64_t pieces = 2 * static_cast<int64_t>(wgs) * pd_heads(D);
   float* part = ws;
-  float* ml = ws + static_cast<int64_t>(B) * H * splits * D;
-  paged_decode_kernel<E, D, F8><<<dim3(splits, c.Hk * chunks, B), 64 * kPdWaves, 0, stream>>>(
-      c, rows, q, sq_b, sq_h, grp, chunks, splits, scale * kLog2e, out, so_b, so_h, part, ml);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || splits == 1) return e;
-  paged_combine_kernel<E, D><<<dim3(B * H), 256, 0, stream>>>(part, ml, H, splits, out, so_b, so_h);
+  float* ml = part + pieces * D;
+  int* starts = reinterpret_cast<int*>(ml + 2 * pieces);
+  paged_decode_kernel<E, D, F8><<<dim3(wgs), 64 * kPdWaves, 0, stream>>>(
+      c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out, so_b, so_h, starts, part, ml);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  paged_combine_kernel<E, D><<<dim3(B * H), kPdCombineThreads, 0, stream>>>(
+      starts, part, ml, gr, grp, chunks, lists, out, so_b, so_h);
   return hipGetLastError();
 }
 
