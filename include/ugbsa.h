@@ -317,7 +317,8 @@ int ugbsa_decode(const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_
  * Slots past a sequence's length may hold anything, NaN included. */
 typedef struct {
   void* k_pages; /* [num_pages, Hk, 64, D] of dtype or e4m3, head_dim stride 1, */
-  void* v_pages; /* 16-byte aligned rows; the other strides in elements, a slot's at most 2^24 */
+  void* v_pages; /* 16-byte aligned rows; the other strides in elements, at most 2^24 a
+                    slot, below 2^35 a page or head */
   int64_t sk_p, sk_h, sk_n;
   int64_t sv_p, sv_h, sv_n;
   uint8_t* k_scale; /* [num_pages, Hk, 64] contiguous, e4m3 only: a value is */
@@ -385,7 +386,7 @@ int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int unit
  * all k_slots).  Entries outside the sequence's pages are skipped; a page must
  * not be listed twice.  q [B, H, 1, D], out [B, H, D] of dtype with
  * even strides (4-byte aligned rows); B, H <= 65535, B * H * max_pages (or k_slots)
- * below 2^31 - 2^16.  A row without a key, or whose every weight is 0, gives
+ * at most 2^30.  A row without a key, or whose every weight is 0, gives
  * zeros.  workspace (16-byte aligned) holds the pieces of rows that several
  * workgroups share; its contents on entry do not matter. */
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,

@@ -89,6 +89,8 @@ int check_pages(const ugbsa_paged_cache* c) {
   // lane offsets within a page are 32-bit
   if (c->sk_n < 0 || c->sv_n < 0 || c->sk_n > 1 << 24 || c->sv_n > 1 << 24)
     return fail(UGBSA_ELAYOUT, "the pages' slot strides must lie in [0, 2^24]");
+  for (const int64_t s : {c->sk_p, c->sk_h, c->sv_p, c->sv_h})
+    if (s < 0 || s >= int64_t{1} << 35) return fail(UGBSA_ELAYOUT, "the pages' strides must lie in [0, 2^35)");
   if (e4m3 && (c->k_scale == nullptr || c->v_scale == nullptr))
     return fail(UGBSA_EARG, "an e4m3 cache needs k_scale and v_scale");
   if (e4m3 && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 7)
@@ -701,9 +703,9 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
   if (!(scale - scale == 0.f)) return fail(UGBSA_EARG, "scale must be finite");
   if (kv_idx != nullptr && (k_slots < 1 || k_slots > 1 << 24))
     return fail(UGBSA_EARG, "k_slots must lie in [1, 2^24] (%d)", k_slots);
-  // the rows' pages are numbered end to end in 32 bits
-  if (static_cast<int64_t>(B) * H * (kv_idx != nullptr ? k_slots : max_pages) > INT32_MAX - 65536)
-    return fail(UGBSA_EARG, "B * H * pages a row must be below 2^31 - 2^16");
+  // the rows' pages, and a few units more a row, are numbered end to end in 32 bits
+  if (static_cast<int64_t>(B) * H * (kv_idx != nullptr ? k_slots : max_pages) > 1 << 30)
+    return fail(UGBSA_EARG, "B * H * pages a row must be at most 2^30");
   if (kv_idx == nullptr && counts != nullptr) return fail(UGBSA_EARG, "counts without kv_idx");
   if (out == nullptr || so_d != 1) return fail(UGBSA_ELAYOUT, "out must be non-null with unit head_dim stride");
   if ((reinterpret_cast<uintptr_t>(out) & 3) || so_b % 2 || so_h % 2)

@@ -12,6 +12,16 @@ namespace ugbsa {
 
 constexpr int kPdWaves = 4;       // wavefronts per workgroup
 constexpr int kPdStep = 32;       // keys per wavefront step: half a page
+// Four dims of a head, over their weights' sum; a row without a key, or whose every
+// weight is 0, gives zeros.
+template <typename E>
+__device__ __forceinline__ void store4(uint16_t* to, f32x4 x, float sum) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = sum == 0.f ? 0.f : x[j] / sum;
+  reinterpret_cast<uint32_t*>(to)[0] = E::pack2(x[0], x[1]);
+  reinterpret_cast<uint32_t*>(to)[1] = E::pack2(x[2], x[3]);
+}
+
 // Query heads per workgroup: the 16 MFMA columns; 8 at head_dim 256, where the
 // wavefronts' O of 16 heads would take 66 KiB of LDS.
 __host__ __device__ constexpr int pd_heads(int D) { return D > 128 ? 8 : 16; }
@@ -29,12 +39,14 @@ struct PagedRows {
 
 // The work of a call is its rows' pages (or list entries), laid end to end: a group
 // is a sequence, or with lists a (sequence, KV head), its members the (KV head,)
-// head chunks that visit its n pages, one row each.  Workgroup w takes units
-// [w per, (w + 1) per) of the line, however the batch's lengths are spread, so
-// rows begin and end inside workgroups.  A row that one workgroup holds is written
-// by it; the pieces of the others meet in paged_combine_kernel: piece 2 w of
-// workgroup w continues a row, piece 2 w + 1 begins one.
+// head chunks that visit its n pages, one row each.  A row takes n + kPdRowCost
+// units of the line, the first kPdRowCost for its start and end.  Workgroup w takes
+// units [w per, (w + 1) per), however the batch's lengths are spread, so rows begin
+// and end inside workgroups.  A row whose pages one workgroup holds is written by it;
+// the pieces of the others meet in paged_combine_kernel: piece 2 w of workgroup w
+// continues a row, piece 2 w + 1 begins one.
 constexpr int kPdUnits = 2;       // fewest units of a workgroup: a half page a wavefront
+constexpr int kPdRowCost = 3;
 
 struct PagedGroups {
   int groups, members, Hk;
@@ -47,6 +59,14 @@ __device__ __forceinline__ int group_units(const PagedRows& r, int Hk, int i) {
   const int n = r.counts == nullptr ? r.k_slots : r.counts[i];
   return len == 0 ? 0 : min(max(n, 0), r.k_slots);
 }
+// Units of a row of n pages on the line.
+__device__ __forceinline__ int row_units(int n) { return n > 0 ? n + kPdRowCost : 0; }
+
+template <bool NT, typename T>
+__device__ __forceinline__ auto stream_load(T* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
 
 // Wavefronts per SIMD that the registers allow, which is also the workgroups per CU
 // that a call launches: a line cut into more than are resident leaves a second round
@@ -57,7 +77,7 @@ __host__ __device__ constexpr int pd_occupancy(int D, bool F8) {
   return D == 64 ? 4 : (D == 128 ? (F8 ? 3 : 2) : (F8 ? 2 : 1));
 }
 
-template <typename E, int D, bool F8>
+template <typename E, int D, bool F8, bool NT>
 __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_decode_kernel(
     PagedCache c, PagedRows rows, PagedGroups gr, const uint16_t* __restrict__ q, int64_t sq_b,
     int64_t sq_h, int grp, int chunks, float scale_log2, uint16_t* __restrict__ out, int64_t so_b,
@@ -78,7 +98,7 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
   const bool few = gr.groups <= 64;
   const int each = few ? 1 : (gr.groups + 255) / 256, i0 = (few ? lane : threadIdx.x) * each;
   int mine = 0;
-  for (int i = i0; i < min(i0 + each, gr.groups); ++i) mine += group_units(rows, gr.Hk, i);
+  for (int i = i0; i < min(i0 + each, gr.groups); ++i) mine += row_units(group_units(rows, gr.Hk, i));
   mine *= gr.members;
   int incl = mine;
 #pragma unroll
@@ -102,14 +122,14 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     int s = incl - mine;
     for (int i = i0; i < min(i0 + each, gr.groups); ++i) {
       starts[i] = s;
-      s += group_units(rows, gr.Hk, i) * gr.members;
+      s += row_units(group_units(rows, gr.Hk, i)) * gr.members;
     }
     if (threadIdx.x == 0) starts[gr.groups] = total, starts[gr.groups + 1] = per;
   }
   if (static_cast<int64_t>(blockIdx.x) * per >= total) return;
   int u = blockIdx.x * per;
   const int u_end = min(u + per, total);
-  int group, n, off0;                              // off0: units of the group before u
+  int group, n, off0;                              // n: units of a row; off0: the group's before u
   if (few) {
     group = __builtin_popcountll(__ballot(incl <= u));
     const int units = __builtin_amdgcn_readlane(mine, group);
@@ -119,7 +139,7 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     if (incl - mine <= u && u < incl) {            // one thread
       int s = incl - mine;
       for (int i = i0;; ++i) {
-        const int k = group_units(rows, gr.Hk, i) * gr.members;
+        const int k = row_units(group_units(rows, gr.Hk, i)) * gr.members;
         if (u < s + k) {
           s_start[0] = i;
           s_start[1] = u - s;
@@ -131,10 +151,10 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     __syncthreads();
     group = __builtin_amdgcn_readfirstlane(s_start[0]);
     off0 = __builtin_amdgcn_readfirstlane(s_start[1]);
-    n = __builtin_amdgcn_readfirstlane(group_units(rows, gr.Hk, group));
+    n = __builtin_amdgcn_readfirstlane(row_units(group_units(rows, gr.Hk, group)));
   }
   int member = static_cast<int>(static_cast<uint32_t>(off0) / static_cast<uint32_t>(n));
-  int p0 = off0 - member * n;
+  int x0 = off0 - member * n;                      // the row's units before u
 
   // MFMA row R of S^T tile mt is key 8 (R >> 2) + 4 mt + (R & 3) of the step:
   // the lane then holds keys 8 g4 + 4 mt + i
@@ -145,8 +165,9 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
   const uint32_t k_row = static_cast<uint32_t>(c.sk_n * SZ), v_row = static_cast<uint32_t>(c.sv_n * SZ);
 
   for (;;) {
-    // this workgroup's piece [p0, p1) of row (b, g, ck)
-    const int p1 = min(n, p0 + u_end - u);
+    // this workgroup's units [x0, x1), and so pages [p0, p1), of row (b, g, ck)
+    const int x1 = min(n, x0 + u_end - u);
+    const int p0 = max(x0 - kPdRowCost, 0), p1 = max(x1 - kPdRowCost, 0), pages = n - kPdRowCost;
     const int b = rows.kv_idx == nullptr ? group : group / gr.Hk;
     const int g = rows.kv_idx == nullptr ? member / chunks : group % gr.Hk;
     const int ck = rows.kv_idx == nullptr ? member % chunks : member;
@@ -196,7 +217,7 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
         gchar* row = half + 4u * mt * k_row;
 #pragma unroll
         for (int j = 0; j < (F8 ? KS / 2 : KS); ++j)
-          kf[mt][j] = *reinterpret_cast<gu32x4*>(row + (k_lane + 64u * j));
+          kf[mt][j] = stream_load<NT>(reinterpret_cast<gu32x4*>(row + (k_lane + 64u * j)));
         if constexpr (F8)
           ksc[mt] = e8m0(c.k_scale[(s.page * gr.Hk + g) * kBlock + s.base + krow + 4 * mt]);
       }
@@ -217,14 +238,14 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
         for (int l = 0; l < VL; ++l) {
           gchar* at = row + (v_lane + 256u * l);
           if constexpr (LB == 16) {
-            const u32x4 x = *reinterpret_cast<gu32x4*>(at);
+            const u32x4 x = stream_load<NT>(reinterpret_cast<gu32x4*>(at));
 #pragma unroll
             for (int j = 0; j < 4; ++j) vr[i][4 * l + j] = x[j];
           } else if constexpr (LB == 8) {
-            const u32x2 x = *reinterpret_cast<gu32x2*>(at);
+            const u32x2 x = stream_load<NT>(reinterpret_cast<gu32x2*>(at));
             vr[i][0] = x[0], vr[i][1] = x[1];
           } else {
-            vr[i][0] = *reinterpret_cast<gu32*>(at);
+            vr[i][0] = stream_load<NT>(reinterpret_cast<gu32*>(at));
           }
         }
       }
@@ -334,27 +355,26 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     }
     __syncthreads();
 
-    const bool whole = p0 == 0 && p1 == n;
+    const bool whole = p0 == 0 && p1 == pages;
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (p0 == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < heads * D; i += 64 * kPdWaves) {
-      const int hh = i / D, d = i % D;
+    for (int i = threadIdx.x; p0 < p1 && i < heads * (D / 4); i += 64 * kPdWaves) {
+      const int hh = i / (D / 4), d = 4 * (i % (D / 4));
       float mm = s_ml[0][hh][0];
 #pragma unroll
       for (int w = 1; w < kPdWaves; ++w) mm = fmaxf(mm, s_ml[w][hh][0]);
       const float off = mm == -INFINITY ? 0.f : mm;
-      float acc = 0.f, ll = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      float ll = 0.f;
 #pragma unroll
       for (int w = 0; w < kPdWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(s_ml[w][hh][0] - off);
-        acc += s_o[w][hh][d] * f;
+        acc += *reinterpret_cast<const f32x4*>(&s_o[w][hh][d]) * f;
         ll += s_ml[w][hh][1] * f;
       }
       if (whole) {
-        // no key at all: zeros
-        out[b * so_b + (h0 + hh) * so_h + d] =
-            static_cast<uint16_t>(E::pack2(ll == 0.f ? 0.f : acc / ll, 0.f) & 0xFFFFu);
+        store4<E>(out + b * so_b + (h0 + hh) * so_h + d, acc, ll);
       } else {
-        part[(piece * NH + hh) * D + d] = acc;
+        *reinterpret_cast<f32x4*>(part + (piece * NH + hh) * D + d) = acc;
         if (d == 0) {
           ml[(piece * NH + hh) * 2] = mm;
           ml[(piece * NH + hh) * 2 + 1] = ll;
@@ -362,14 +382,14 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
       }
     }
 
-    u += p1 - p0;
+    u += x1 - x0;
     if (u >= u_end) return;
     // the next row with pages
-    p0 = 0;
+    x0 = 0;
     if (++member == gr.members) {
       member = 0;
       for (++group;; group += 64) {
-        const int k = group + lane < gr.groups ? group_units(rows, gr.Hk, group + lane) : 0;
+        const int k = group + lane < gr.groups ? row_units(group_units(rows, gr.Hk, group + lane)) : 0;
         const uint64_t some = __ballot(k > 0);
         if (some == 0) continue;                   // u < total: a later group has pages
         const int f = __builtin_ctzll(some);
@@ -406,7 +426,7 @@ __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
     if (tid < D) o[tid] = 0;
     return;
   }
-  const int wa = static_cast<int>(first / per);
+  const int wa = static_cast<int>((first + kPdRowCost) / per);
   const int pieces = static_cast<int>((first + n - 1) / per) - wa + 1;
   if (pieces == 1) return;
   auto at = [&](int i) { return (2 * (wa + i) + (i == 0 ? 1 : 0)) * NH + hh; };
@@ -451,11 +471,7 @@ __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
   if (tid < D / 4) {
 #pragma unroll
     for (int r = 1; r < RUNS; ++r) acc += s_acc[r][tid];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = total == 0.f ? 0.f : acc[j] / total;
-    uint32_t* w = reinterpret_cast<uint32_t*>(o) + 2 * tid;
-    w[0] = E::pack2(acc[0], acc[1]);
-    w[1] = E::pack2(acc[2], acc[3]);
+    store4<E>(o + 4 * tid, acc, total);
   }
 }
 
@@ -463,7 +479,7 @@ __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
 // cannot have kPdUnits for each.
 static int paged_decode_workgroups(int B, int H, int Hk, int D, bool e4m3, int units) {
   const int64_t rows = static_cast<int64_t>(B) * Hk * ((H / Hk + pd_heads(D) - 1) / pd_heads(D));
-  const int64_t most = (rows * units + kPdUnits - 1) / kPdUnits;
+  const int64_t most = (rows * (units + kPdRowCost) + kPdUnits - 1) / kPdUnits;
   const int64_t resident = 256 * pd_occupancy(D, e4m3);
   return static_cast<int>(most < resident ? most : resident);
 }
@@ -487,8 +503,16 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
   float* part = ws;
   float* ml = part + pieces * D;
   int* starts = reinterpret_cast<int*>(ml + 2 * pieces);
-  paged_decode_kernel<E, D, F8><<<dim3(wgs), 64 * kPdWaves, 0, stream>>>(
-      c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out, so_b, so_h, starts, part, ml);
+  // Pages are read past the 256 MB memory-side cache where the call can hold three
+  // times as much and they would only displace each other there (32 x 16K tokens,
+  // 40/8 heads, bf16 362 -> 336 us; 32 x 64K in e4m3 725 -> 698; 24 of up to 16K 77 ->
+  // 72); smaller calls may find theirs in it (4 of up to 64K, head_dim 256, 41.1 and
+  // 42.2).  The table's width bounds the lengths, which are on the device.
+  const int64_t most = static_cast<int64_t>(B) * c.Hk * (lists ? rows.k_slots : rows.max_pages) *
+                       (2 * kBlock * D * (F8 ? 1 : 2));
+  const auto kernel = most > 768ll << 20 ? paged_decode_kernel<E, D, F8, true> : paged_decode_kernel<E, D, F8, false>;
+  kernel<<<dim3(wgs), 64 * kPdWaves, 0, stream>>>(c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out,
+                                                  so_b, so_h, starts, part, ml);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   paged_combine_kernel<E, D><<<dim3(B * H), kPdCombineThreads, 0, stream>>>(
