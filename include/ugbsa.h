@@ -376,9 +376,9 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
                        float* sigma, uint8_t* uncertain, float* workspace,
                        int64_t workspace_elems, void* stream);
 
-/* fp32 elements of a ugbsa_paged_decode workspace (0 for sizes no call takes).
- * units: max_pages, or k_slots of a call with lists. */
-int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units);
+/* fp32 elements of a ugbsa_paged_decode workspace (0: none is needed, or sizes no
+ * call takes).  units: max_pages, or k_slots of a call with lists. */
+int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units, int cache_dtype);
 
 /* Decode over pages — attention of one query row per head over the tokens below
  * lens[b]: of every page (kv_idx NULL), or of the pages that kv_idx [B, Hk,

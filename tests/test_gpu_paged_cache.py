@@ -475,6 +475,28 @@ def test_decode_listed(hip_lib, H, Hk, D, dtype, e4m3):
     assert torch.equal(a, pc.paged_decode(q, cache, table, i32(lens), 0.1, kv_idx=kv))
 
 
+# More sequences than a wavefront's lanes and a workgroup's threads, most of them without a key, in
+# tables from one page to many; lists of as many rows.
+@pytest.mark.parametrize("B,width", [(65, 40), (300, 70), (300, 2), (700, 20)])
+def test_decode_many_sequences(hip_lib, B, width):
+    g = gen(B)
+    lens = [0] * B
+    for i in list(range(0, B, 97)) + [B - 1, B // 2, B // 2 + 1]:
+        lens[i] = min(64 * width, 1 + (i * 37) % 2500)
+    lens[B // 3] = 64 * width
+    table, P = tables(lens, g, width=width)
+    cache = filled(g, P, 2, 64, BF, B % 2 == 0)
+    q = torch.randn(B, 6, 1, 64, generator=g, device=DEV).to(BF)
+    out = check_decode(q, cache, table, lens, 0.125)
+    assert (out[torch.tensor(lens, device=DEV) == 0] == 0).all()
+    nb = torch.tensor([(n + 63) // 64 for n in lens], device=DEV)
+    kv = torch.arange(width, device=DEV, dtype=torch.int32).view(1, 1, -1).repeat(B, 2, 1)
+    counts = torch.stack([nb, (nb + 1) // 2], 1).to(torch.int32)
+    check_decode(q, cache, table, lens, 0.125, kv_idx=kv, counts=counts)
+    assert torch.equal(pc.paged_decode(q, cache, table, i32(lens), 0.125, kv_idx=kv)[:, :, :3],
+                       pc.paged_decode(q, cache, table, i32(lens), 0.125, kv_idx=kv, counts=counts)[:, :, :3])
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_decode_absent_pages_and_lengths(hip_lib, e4m3):
     cache = filled(gen(8), 6, 2, 128, BF, e4m3)

@@ -61,7 +61,7 @@ def test_decode_refusals(lib):
     refused(lib, decode(lib, struct(), kv=16, slots=0), -1, "k_slots")
     refused(lib, decode(lib, struct(), counts=16), -1, "counts")
     refused(lib, decode(lib, struct(), out=None), -2, "out")
-    need = lib.ugbsa_paged_decode_workspace_elems(1, 4, 2, 128, 64)
+    need = lib.ugbsa_paged_decode_workspace_elems(1, 4, 2, 128, 64, _capi.CACHE_MODEL)
     assert need > 0
     refused(lib, decode(lib, struct(), pages=64, n=need - 1), -1, "workspace")
     refused(lib, decode(lib, struct(), pages=64, ws=None), -1, "workspace")
@@ -104,7 +104,7 @@ def test_write_and_read_refusals(lib):
 def test_workspace_queries_of_sizes_no_call_takes(lib):
     for B, H, Hk, D, units in ((0, 4, 2, 128, 8), (1, 0, 2, 128, 8), (1, 5, 2, 128, 8), (1, 4, 2, 96, 8),
                                (1, 4, 2, 128, 0), (1, 4, 2, 128, -1)):
-        assert lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, units) == 0
+        assert lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, units, _capi.CACHE_E4M3) == 0
     assert lib.ugbsa_paged_select_workspace_elems(0, 2, 8) == lib.ugbsa_paged_select_workspace_elems(1, 2, 0) == 0
 
 

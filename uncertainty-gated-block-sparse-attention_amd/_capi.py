@@ -87,7 +87,7 @@ SIGNATURES = {
     "ugbsa_paged_select_workspace_elems": (_i64, [_i, _i, _i]),
     "ugbsa_paged_select": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _i,
                                 _i, _f, _p, _p, _p, _p, _p, _i64, _p]),
-    "ugbsa_paged_decode_workspace_elems": (_i64, [_i, _i, _i, _i, _i]),
+    "ugbsa_paged_decode_workspace_elems": (_i64, [_i, _i, _i, _i, _i, _i]),
     "ugbsa_paged_decode": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _p,
                                 _p, _i, _p, _i64, _i64, _i64, _p, _i64, _p]),
 }

@@ -626,7 +626,7 @@ int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_
   if ((rc = check_bf16_operand("k", k, 0, sk_h, sk_t, sk_d))) return rc;
   if ((rc = check_bf16_operand("v", v, 0, sv_h, sv_t, sv_d))) return rc;
   if (ugbsa::paged_write_units(B, T, cu_new != nullptr) >= 1 << 24)
-    return fail(UGBSA_EARG, "more than 2^24 pages in one write (T=%d, B=%d)", T, B);
+    return fail(UGBSA_EARG, "2^24 pages or more in one write (T=%d, B=%d)", T, B);
   return hip_result(ugbsa::launch_paged_write(paged_cache(cache), static_cast<const uint16_t*>(k), sk_t,
                                               sk_h, static_cast<const uint16_t*>(v), sv_t, sv_h, cu_new,
                                               lens, table, st_b, B, T, max_pages,
@@ -685,10 +685,9 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
                     "paged_select");
 }
 
-int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units) {
+int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units, int cache_dtype) {
   if (check_dims(B, H, Hk, D, UGBSA_DTYPE_BF16) || units < 1) return 0;
-  // one size for both cache types: e4m3 keeps more workgroups resident
-  return ugbsa::paged_decode_ws_elems(B, H, Hk, D, true, units);
+  return ugbsa::paged_decode_ws_elems(B, H, Hk, D, cache_dtype == UGBSA_CACHE_E4M3, units);
 }
 
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
@@ -712,8 +711,9 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
     return fail(UGBSA_ELAYOUT, "out must have 4-byte aligned rows");
   if (static_cast<int64_t>(B) * H >= 1 << 24) return fail(UGBSA_EARG, "B * H must be below 2^24");
   const int64_t need = ugbsa_paged_decode_workspace_elems(B, H, cache->Hk, cache->D,
-                                                          kv_idx != nullptr ? k_slots : max_pages);
-  if (workspace == nullptr || workspace_elems < need)
+                                                          kv_idx != nullptr ? k_slots : max_pages,
+                                                          cache->cache_dtype);
+  if (need > 0 && (workspace == nullptr || workspace_elems < need))
     return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_decode_workspace_elems (%lld)",
                 (long long)workspace_elems, (long long)need);
   if (!aligned16(workspace)) return fail(UGBSA_ELAYOUT, "workspace must be 16-byte aligned");

@@ -28,6 +28,13 @@ typedef const __attribute__((address_space(1))) u32x4 gu32x4;
 typedef const __attribute__((address_space(1))) u32x2 gu32x2;
 typedef const __attribute__((address_space(1))) uint32_t gu32;
 
+// A load, NT: of data read once, which need not displace other data from the caches.
+template <bool NT, typename T>
+__device__ __forceinline__ auto stream_load(T* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // Eight e4m3 codes (lo: dims 0-3, hi: 4-7) times 2^(byte - 127) in E's format (exact).
 template <typename E>
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t codes, float scale, bool hi) {

@@ -62,12 +62,6 @@ __device__ __forceinline__ int group_units(const PagedRows& r, int Hk, int i) {
 // Units of a row of n pages on the line.
 __device__ __forceinline__ int row_units(int n) { return n > 0 ? n + kPdRowCost : 0; }
 
-template <bool NT, typename T>
-__device__ __forceinline__ auto stream_load(T* p) {
-  if constexpr (NT) return __builtin_nontemporal_load(p);
-  else return *p;
-}
-
 // Wavefronts per SIMD that the registers allow, which is also the workgroups per CU
 // that a call launches: a line cut into more than are resident leaves a second round
 // of them (us, 256 / 512 / 768 / 1024 workgroups: 24 sequences of up to 16K tokens,
@@ -77,8 +71,11 @@ __host__ __device__ constexpr int pd_occupancy(int D, bool F8) {
   return D == 64 ? 4 : (D == 128 ? (F8 ? 3 : 2) : (F8 ? 2 : 1));
 }
 
-template <typename E, int D, bool F8, bool NT>
-__global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_decode_kernel(
+// Wavefronts of a workgroup: four, or eight where it has a row to itself.
+__host__ __device__ constexpr int pd_waves(bool one) { return one ? 8 : kPdWaves; }
+
+template <typename E, int D, bool F8, bool NT, bool ONE>
+__global__ __launch_bounds__(64 * pd_waves(ONE), ONE ? 2 : pd_occupancy(D, F8)) void paged_decode_kernel(
     PagedCache c, PagedRows rows, PagedGroups gr, const uint16_t* __restrict__ q, int64_t sq_b,
     int64_t sq_h, int grp, int chunks, float scale_log2, uint16_t* __restrict__ out, int64_t so_b,
     int64_t so_h, int* __restrict__ starts, float* __restrict__ part, float* __restrict__ ml) {
@@ -86,75 +83,82 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
   constexpr int DPL = D / 16;                    // dims a lane loads per key of V
   // 16-bit rows are read 8 dims a load, or 4 at head_dim 64 (VW = dims a load)
   constexpr int VW = F8 ? DPL : (D == 64 ? 4 : 8), VL = DPL / VW;
-  constexpr int SZ = F8 ? 1 : 2;
-  __shared__ float s_o[kPdWaves][NH][D + 4];
-  __shared__ float s_ml[kPdWaves][NH][2];
-  __shared__ int s_sum[kPdWaves], s_start[2];
+  constexpr int SZ = F8 ? 1 : 2, WAVES = pd_waves(ONE);
+  __shared__ float s_o[WAVES][NH][D + 4];
+  __shared__ float s_ml[WAVES][NH][2];
+  __shared__ int s_sum[WAVES], s_start[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g4 = lane >> 4, r16 = lane & 15;
 
-  // The line's length, and the row where this workgroup's units begin: up to 64
-  // groups lie in a wavefront's lanes, more in the workgroup's threads, some each.
-  const bool few = gr.groups <= 64;
-  const int each = few ? 1 : (gr.groups + 255) / 256, i0 = (few ? lane : threadIdx.x) * each;
-  int mine = 0;
-  for (int i = i0; i < min(i0 + each, gr.groups); ++i) mine += row_units(group_units(rows, gr.Hk, i));
-  mine *= gr.members;
-  int incl = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += y;
-  }
-  int total = __builtin_amdgcn_readlane(incl, 63);
-  if (!few) {
-    if (lane == 63) s_sum[wave] = incl;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kPdWaves; ++w) {
-      if (w < wave) incl += s_sum[w];
-      total += s_sum[w];
-    }
-  }
-  const int per = max(kPdUnits, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
-  if (blockIdx.x == 0 && (!few || wave == 0)) {    // for the joining kernel
-    int s = incl - mine;
-    for (int i = i0; i < min(i0 + each, gr.groups); ++i) {
-      starts[i] = s;
-      s += row_units(group_units(rows, gr.Hk, i)) * gr.members;
-    }
-    if (threadIdx.x == 0) starts[gr.groups] = total, starts[gr.groups + 1] = per;
-  }
-  if (static_cast<int64_t>(blockIdx.x) * per >= total) return;
-  int u = blockIdx.x * per;
-  const int u_end = min(u + per, total);
-  int group, n, off0;                              // n: units of a row; off0: the group's before u
-  if (few) {
-    group = __builtin_popcountll(__ballot(incl <= u));
-    const int units = __builtin_amdgcn_readlane(mine, group);
-    off0 = u - (__builtin_amdgcn_readlane(incl, group) - units);
-    n = static_cast<int>(static_cast<uint32_t>(units) / static_cast<uint32_t>(gr.members));
+  int group, member, n, x0, u, u_end;              // n: units of the row, x0 of them before u
+  if constexpr (ONE) {
+    group = blockIdx.x / gr.members, member = blockIdx.x % gr.members;
+    n = row_units(__builtin_amdgcn_readfirstlane(group_units(rows, gr.Hk, group)));
+    x0 = u = 0, u_end = n;
   } else {
-    if (incl - mine <= u && u < incl) {            // one thread
-      int s = incl - mine;
-      for (int i = i0;; ++i) {
-        const int k = row_units(group_units(rows, gr.Hk, i)) * gr.members;
-        if (u < s + k) {
-          s_start[0] = i;
-          s_start[1] = u - s;
-          break;
-        }
-        s += k;
+    // The line's length, and the row where this workgroup's units begin: up to 64
+    // groups lie in a wavefront's lanes, more in the workgroup's threads, some each.
+    const bool few = gr.groups <= 64;
+    const int each = few ? 1 : (gr.groups + 255) / 256, i0 = (few ? lane : threadIdx.x) * each;
+    int mine = 0;
+    for (int i = i0; i < min(i0 + each, gr.groups); ++i) mine += row_units(group_units(rows, gr.Hk, i));
+    mine *= gr.members;
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += y;
+    }
+    int total = __builtin_amdgcn_readlane(incl, 63);
+    if (!few) {
+      if (lane == 63) s_sum[wave] = incl;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) incl += s_sum[w];
+        total += s_sum[w];
       }
     }
-    __syncthreads();
-    group = __builtin_amdgcn_readfirstlane(s_start[0]);
-    off0 = __builtin_amdgcn_readfirstlane(s_start[1]);
-    n = __builtin_amdgcn_readfirstlane(row_units(group_units(rows, gr.Hk, group)));
+    const int per = max(kPdUnits, static_cast<int>((static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x));
+    if (blockIdx.x == 0 && (!few || wave == 0)) {    // for the joining kernel
+      int s = incl - mine;
+      for (int i = i0; i < min(i0 + each, gr.groups); ++i) {
+        starts[i] = s;
+        s += row_units(group_units(rows, gr.Hk, i)) * gr.members;
+      }
+      if (threadIdx.x == 0) starts[gr.groups] = total, starts[gr.groups + 1] = per;
+    }
+    if (static_cast<int64_t>(blockIdx.x) * per >= total) return;
+    u = blockIdx.x * per;
+    u_end = min(u + per, total);
+    int off0;                                        // units of the group before u
+    if (few) {
+      group = __builtin_popcountll(__ballot(incl <= u));
+      const int units = __builtin_amdgcn_readlane(mine, group);
+      off0 = u - (__builtin_amdgcn_readlane(incl, group) - units);
+      n = static_cast<int>(static_cast<uint32_t>(units) / static_cast<uint32_t>(gr.members));
+    } else {
+      if (incl - mine <= u && u < incl) {            // one thread
+        int s = incl - mine;
+        for (int i = i0;; ++i) {
+          const int k = row_units(group_units(rows, gr.Hk, i)) * gr.members;
+          if (u < s + k) {
+            s_start[0] = i;
+            s_start[1] = u - s;
+            break;
+          }
+          s += k;
+        }
+      }
+      __syncthreads();
+      group = __builtin_amdgcn_readfirstlane(s_start[0]);
+      off0 = __builtin_amdgcn_readfirstlane(s_start[1]);
+      n = __builtin_amdgcn_readfirstlane(row_units(group_units(rows, gr.Hk, group)));
+    }
+    member = static_cast<int>(static_cast<uint32_t>(off0) / static_cast<uint32_t>(n));
+    x0 = off0 - member * n;
   }
-  int member = static_cast<int>(static_cast<uint32_t>(off0) / static_cast<uint32_t>(n));
-  int x0 = off0 - member * n;                      // the row's units before u
 
   // MFMA row R of S^T tile mt is key 8 (R >> 2) + 4 mt + (R & 3) of the step:
   // the lane then holds keys 8 g4 + 4 mt + i
@@ -173,6 +177,11 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     const int ck = rows.kv_idx == nullptr ? member % chunks : member;
     const int heads = min(NH, grp - ck * NH);    // live columns
     const int h0 = g * grp + ck * NH;
+    if (ONE && n == 0) {
+      for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * WAVES)
+        store4<E>(out + b * so_b + (h0 + i / (D / 4)) * so_h + 4 * (i % (D / 4)), f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
+      return;
+    }
     const int len = cached_len(rows.lens, b, rows.max_pages);
     const int32_t* table = rows.table + b * rows.st_b;
     const int32_t* list = rows.kv_idx == nullptr
@@ -263,12 +272,12 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
       cur = step_at(st);
       load_k(cur);
       load_v(cur);
-      if (st + kPdWaves < st1) nxt = step_at(st + kPdWaves);
+      if (st + WAVES < st1) nxt = step_at(st + WAVES);
     }
-    for (; st < st1; st += kPdWaves) {
-      const bool more = st + kPdWaves < st1;
+    for (; st < st1; st += WAVES) {
+      const bool more = st + WAVES < st1;
       // the page after the next one's: its number is on the way during this step
-      if (st + 2 * kPdWaves < st1) far = step_at(st + 2 * kPdWaves);
+      if (st + 2 * WAVES < st1) far = step_at(st + 2 * WAVES);
       f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
@@ -355,18 +364,18 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     }
     __syncthreads();
 
-    const bool whole = p0 == 0 && p1 == pages;
+    const bool whole = ONE || (p0 == 0 && p1 == pages);
     const int64_t piece = 2 * static_cast<int64_t>(blockIdx.x) + (p0 == 0 ? 1 : 0);
-    for (int i = threadIdx.x; p0 < p1 && i < heads * (D / 4); i += 64 * kPdWaves) {
+    for (int i = threadIdx.x; p0 < p1 && i < heads * (D / 4); i += 64 * WAVES) {
       const int hh = i / (D / 4), d = 4 * (i % (D / 4));
       float mm = s_ml[0][hh][0];
 #pragma unroll
-      for (int w = 1; w < kPdWaves; ++w) mm = fmaxf(mm, s_ml[w][hh][0]);
+      for (int w = 1; w < WAVES; ++w) mm = fmaxf(mm, s_ml[w][hh][0]);
       const float off = mm == -INFINITY ? 0.f : mm;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       float ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPdWaves; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float f = __builtin_amdgcn_exp2f(s_ml[w][hh][0] - off);
         acc += *reinterpret_cast<const f32x4*>(&s_o[w][hh][d]) * f;
         ll += s_ml[w][hh][1] * f;
@@ -383,7 +392,7 @@ __global__ __launch_bounds__(64 * kPdWaves, pd_occupancy(D, F8)) void paged_deco
     }
 
     u += x1 - x0;
-    if (u >= u_end) return;
+    if (ONE || u >= u_end) return;
     // the next row with pages
     x0 = 0;
     if (++member == gr.members) {
@@ -475,6 +484,15 @@ __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
   }
 }
 
+// Whether each row gets a workgroup to itself, with no line to find and nothing to
+// join: where a row's K and V are at most 256 KB, which one CU streams (about 25 bytes a
+// clock) in what the joining launch costs.  us, this form / the line: 512 tokens, 28/4
+// heads, head_dim 128, bf16, 1 sequence 9.1 / 10.5, 128 sequences 15.9 / 22.3; 1024
+// tokens (512 KB) 13.3 / 10.8 and 23.6 / 26.8, in e4m3 10.8 / 11.0 and 19.1 / 23.3.
+static bool paged_decode_one(int D, bool e4m3, int units) {
+  return static_cast<int64_t>(units) * (2 * kBlock * D * (e4m3 ? 1 : 2)) <= 256 << 10;
+}
+
 // Workgroups of a call: as many as the card holds at once, unless the call's rows
 // cannot have kPdUnits for each.
 static int paged_decode_workgroups(int B, int H, int Hk, int D, bool e4m3, int units) {
@@ -486,6 +504,7 @@ static int paged_decode_workgroups(int B, int H, int Hk, int D, bool e4m3, int u
 
 // The pieces, their (m, l), then starts [groups + 2] int32.
 int64_t paged_decode_ws_elems(int B, int H, int Hk, int D, bool e4m3, int units) {
+  if (paged_decode_one(D, e4m3, units)) return 0;
   const int64_t pieces = 2 * static_cast<int64_t>(paged_decode_workgroups(B, H, Hk, D, e4m3, units)) * pd_heads(D);
   return pieces * (D + 2) + static_cast<int64_t>(B) * Hk + 2;
 }
@@ -497,8 +516,13 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
                                         hipStream_t stream) {
   const int grp = H / c.Hk, chunks = (grp + pd_heads(D) - 1) / pd_heads(D);
   const bool lists = rows.kv_idx != nullptr;
-  const int wgs = paged_decode_workgroups(B, H, c.Hk, D, F8, lists ? rows.k_slots : rows.max_pages);
   const PagedGroups gr{lists ? B * c.Hk : B, lists ? chunks : c.Hk * chunks, c.Hk};
+  if (paged_decode_one(D, F8, lists ? rows.k_slots : rows.max_pages)) {
+    paged_decode_kernel<E, D, F8, false, true><<<dim3(B * c.Hk * chunks), 64 * pd_waves(true), 0, stream>>>(
+        c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out, so_b, so_h, nullptr, nullptr, nullptr);
+    return hipGetLastError();
+  }
+  const int wgs = paged_decode_workgroups(B, H, c.Hk, D, F8, lists ? rows.k_slots : rows.max_pages);
   const int64_t pieces = 2 * static_cast<int64_t>(wgs) * pd_heads(D);
   float* part = ws;
   float* ml = part + pieces * D;
@@ -510,7 +534,8 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
   // 42.2).  The table's width bounds the lengths, which are on the device.
   const int64_t most = static_cast<int64_t>(B) * c.Hk * (lists ? rows.k_slots : rows.max_pages) *
                        (2 * kBlock * D * (F8 ? 1 : 2));
-  const auto kernel = most > 768ll << 20 ? paged_decode_kernel<E, D, F8, true> : paged_decode_kernel<E, D, F8, false>;
+  const auto kernel = most > 768ll << 20 ? paged_decode_kernel<E, D, F8, true, false>
+                                         : paged_decode_kernel<E, D, F8, false, false>;
   kernel<<<dim3(wgs), 64 * kPdWaves, 0, stream>>>(c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out,
                                                   so_b, so_h, starts, part, ml);
   const hipError_t e = hipGetLastError();

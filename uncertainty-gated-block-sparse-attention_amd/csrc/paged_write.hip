@@ -23,11 +23,12 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
   constexpr int CH = D / 8, RG = 256 / CH;
   __shared__ float red[2][RG][D + 1];
   __shared__ int s_sum[4], s_unit[4];
-  const int tid = threadIdx.x, ch = tid % CH, rg = tid / CH, h = blockIdx.y;
+  const int tid = threadIdx.x, ch = tid % CH, rg = tid / CH;
+  const uint32_t h = blockIdx.y, unit = blockIdx.x;
   const int64_t most = static_cast<int64_t>(max_pages) * kBlock;
 
   // the sequence, its first new token and the page this workgroup is for
-  int b = blockIdx.x, page_at = 0, t0 = blockIdx.x, t1 = blockIdx.x + 1;
+  int b = unit, page_at = 0, t0 = unit, t1 = unit + 1;
   if (cu_new != nullptr) {
     int64_t before = 0;                     // touched pages of the sequences already passed
     if (tid == 0) s_unit[0] = -1;
@@ -52,15 +53,15 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
       __syncthreads();
       int64_t start = before + incl - n;
       for (int w = 0; w < (tid >> 6); ++w) start += s_sum[w];
-      if (blockIdx.x >= start && blockIdx.x < start + n) {
+      if (unit >= start && unit < start + n) {
         s_unit[0] = i;
-        s_unit[1] = static_cast<int>(blockIdx.x - start);
+        s_unit[1] = static_cast<int>(unit - start);
         s_unit[2] = a0;
         s_unit[3] = a1;
       }
       before += s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
       __syncthreads();
-      if (before > blockIdx.x) break;
+      if (before > unit) break;
     }
     if (s_unit[0] < 0) return;
     b = s_unit[0], page_at = s_unit[1], t0 = s_unit[2], t1 = s_unit[3];
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       const uint16_t* src = (kv ? v + tok * sv_t + h * sv_h : k + tok * sk_t + h * sk_h) + 8 * ch;
-      const u32x4 raw = *reinterpret_cast<const u32x4*>(src);
+      const u32x4 raw = stream_load<true>(reinterpret_cast<const u32x4*>(src));
       const int64_t at = page * (kv ? c.sv_p : c.sk_p) + h * (kv ? c.sv_h : c.sk_h) +
                          s * (kv ? c.sv_n : c.sk_n) + 8 * ch;
       float x[8];
@@ -128,6 +129,29 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
     }
   }
   if (c.planes == nullptr) return;
+  if (s1 - s0 == 1) {             // a decode step's token: its threads hold all there is
+    if (rg != 0) return;
+    uint16_t* out = c.planes + head * 2 * D + 8 * ch;
+    u32x4 hi = {0u, 0u, 0u, 0u}, lo = hi;
+    if (s0 > 0) {
+      hi = *reinterpret_cast<const u32x4*>(out);
+      lo = *reinterpret_cast<const u32x4*>(out + D);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (s0 > 0) {
+        mx[2 * j] = fmaxf(mx[2 * j], E::to_f32(hi[j] & 0xFFFFu));
+        mx[2 * j + 1] = fmaxf(mx[2 * j + 1], E::to_f32(hi[j] >> 16));
+        mn[2 * j] = fminf(mn[2 * j], E::to_f32(lo[j] & 0xFFFFu));
+        mn[2 * j + 1] = fminf(mn[2 * j + 1], E::to_f32(lo[j] >> 16));
+      }
+      hi[j] = E::from_f32(mx[2 * j]) | static_cast<uint32_t>(E::from_f32(mx[2 * j + 1])) << 16;
+      lo[j] = E::from_f32(mn[2 * j]) | static_cast<uint32_t>(E::from_f32(mn[2 * j + 1])) << 16;
+    }
+    *reinterpret_cast<u32x4*>(out) = hi;
+    *reinterpret_cast<u32x4*>(out + D) = lo;
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     red[0][rg][8 * ch + j] = mx[j];
@@ -147,8 +171,10 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
   }
 }
 
-// One workgroup per (64 output rows, KV head, sequence): rows past the length are zeros.
-template <typename E, int D, bool F8>
+// One workgroup per (64 output rows, KV head, sequence): rows past the length are
+// zeros.  NT: an output that the 256 MB memory-side cache does not hold goes past it,
+// as do the pages it comes from.
+template <typename E, int D, bool F8, bool NT>
 __global__ __launch_bounds__(256) void paged_read_kernel(
     PagedCache c, const int32_t* __restrict__ lens, const int32_t* __restrict__ table, int64_t st_b,
     int max_pages, int N, uint16_t* __restrict__ ko, int64_t sok_b, int64_t sok_h, int64_t sok_n,
@@ -170,15 +196,16 @@ __global__ __launch_bounds__(256) void paged_read_kernel(
         const int64_t at = page * (kv ? c.sv_p : c.sk_p) + h * (kv ? c.sv_h : c.sk_h) +
                            s * (kv ? c.sv_n : c.sk_n) + 8 * ch;
         if constexpr (!F8) {
-          x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(kv ? c.v : c.k) + at);
+          x = stream_load<NT>(reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(kv ? c.v : c.k) + at));
         } else {
-          const u32x2 code = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(kv ? c.v : c.k) + at);
+          const u32x2 code = stream_load<NT>(reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(kv ? c.v : c.k) + at));
           const float scale = e8m0((kv ? c.v_scale : c.k_scale)[head * kBlock + s]);
           x = __builtin_bit_cast(u32x4, e4m3_x8<E>(code[0], code[1], scale));
         }
       }
       uint16_t* dst = (kv ? vo + b * sov_b + h * sov_h + n * sov_n : ko + b * sok_b + h * sok_h + n * sok_n) + 8 * ch;
-      *reinterpret_cast<u32x4*>(dst) = x;
+      if constexpr (NT) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(dst));
+      else *reinterpret_cast<u32x4*>(dst) = x;
     }
   }
 }
@@ -223,9 +250,12 @@ hipError_t launch_paged_read(const PagedCache& c, const int32_t* lens, const int
                              int64_t sok_h, int64_t sok_n, uint16_t* vo, int64_t sov_b, int64_t sov_h,
                              int64_t sov_n, hipStream_t stream) {
   const dim3 grid((N + kBlock - 1) / kBlock, c.Hk, B);
-#define UGBSA_CALL(E_, D_, F8_)                                                                 \
-  paged_read_kernel<E_, D_, F8_><<<grid, 256, 0, stream>>>(c, lens, table, st_b, max_pages, N, ko, \
-                                                           sok_b, sok_h, sok_n, vo, sov_b, sov_h, sov_n)
+  // 64K tokens of 8 heads from e4m3 (268 MB): 86 -> 81.6 us
+  const bool past_cache = 4 * static_cast<int64_t>(B) * c.Hk * N * c.D >= 256 << 20;
+#define UGBSA_CALL(E_, D_, F8_)                                                                     \
+  (past_cache ? paged_read_kernel<E_, D_, F8_, true> : paged_read_kernel<E_, D_, F8_, false>)       \
+      <<<grid, 256, 0, stream>>>(c, lens, table, st_b, max_pages, N, ko, sok_b, sok_h, sok_n, vo, sov_b, \
+                                 sov_h, sov_n)
   UGBSA_PAGED_INSTANCES(UGBSA_CALL);
 #undef UGBSA_CALL
 }

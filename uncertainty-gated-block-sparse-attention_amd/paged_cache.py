@@ -259,10 +259,11 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
         out = torch.empty(B, 1, H, s.D, dtype=cache.dtype, device=cache.device)
     assert tuple(out.shape) == (B, 1, H, s.D) and out.dtype == cache.dtype and out.device == cache.device
     lib = _capi.lib()
-    n = lib.ugbsa_paged_decode_workspace_elems(B, H, s.Hk, s.D, slots or block_table.shape[1])
-    ws = torch.empty(n, dtype=torch.float32, device=cache.device)
+    n = lib.ugbsa_paged_decode_workspace_elems(B, H, s.Hk, s.D, slots or block_table.shape[1],
+                                               s.cache_dtype)
+    ws = torch.empty(n, dtype=torch.float32, device=cache.device) if n else None
     _call(cache, "paged_decode", lib.ugbsa_paged_decode, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
           block_table.data_ptr(), block_table.stride(0), B, block_table.shape[1], float(scale),
           _capi.ptr(kv_idx), _capi.ptr(counts), slots, out.data_ptr(), out.stride(0), out.stride(2),
-          out.stride(3), ws.data_ptr(), n)
+          out.stride(3), _capi.ptr(ws), n)
     return out
