@@ -53,7 +53,9 @@ class PagedCache:
     v_scale: torch.Tensor | None = None
     planes: torch.Tensor | None = None
     dtype: torch.dtype | None = None
+    device: torch.device = field(init=False, default=None)
     _struct: _capi.PagedCacheStruct = field(init=False, repr=False, compare=False, default=None)
+    _call: tuple = field(init=False, repr=False, compare=False, default=None)   # address, device, Hk, D
 
     def __post_init__(self):
         k, v, planes = self.k_pages, self.v_pages, self.planes
@@ -97,6 +99,8 @@ class PagedCache:
         tensors = [t for t in (k, v, self.k_scale, self.v_scale, planes) if t is not None]
         assert all(t.is_cuda and t.device == tensors[0].device for t in tensors), "HIP tensors of one device required"
         object.__setattr__(self, "_struct", s)
+        object.__setattr__(self, "device", tensors[0].device)
+        object.__setattr__(self, "_call", (ctypes.addressof(s), tensors[0].get_device(), s.Hk, s.D))
 
     @classmethod
     def empty(cls, num_pages, Hk, D, dtype, device, e4m3=False, summaries=True):
@@ -108,10 +112,6 @@ class PagedCache:
         planes = torch.empty(num_pages, Hk, 2, D, dtype=dtype, device=device) if summaries else None
         return cls(k, v, ks, vs, planes, dtype)
 
-    @property
-    def device(self):
-        return (self.planes if self.k_pages is None else self.k_pages).device
-
 
 @dataclass
 class PagedSelection:
@@ -121,8 +121,13 @@ class PagedSelection:
     uncertain: torch.Tensor    # uint8 [B, Hk]
 
 
-def _check_operand(name, t, cache, shape):
+def _operand(name, t, cache, shape):
     """A 16-bit tensor of the cache's dtype and device that the kernels read in place."""
+    st = t.stride()
+    if (t.dtype is cache.dtype and t.get_device() == cache._call[1] and t.shape == shape and st[-1] == 1
+            and not (t.requires_grad or t.data_ptr() & 15 or t.is_neg())
+            and not any(s & 7 for s in st[:-1])):
+        return t
     assert t.dtype == cache.dtype, f"{name}: {cache.dtype} required, got {t.dtype}"
     assert t.device == cache.device, f"{name} must be on the cache's device"
     assert tuple(t.shape) == shape, f"{name} {list(shape)} expected, got {list(t.shape)}"
@@ -134,32 +139,34 @@ def _check_operand(name, t, cache, shape):
     return t
 
 
-def _check_table(cache, block_table, seq_lens):
-    """B of a call's table and lengths."""
-    assert block_table.dim() == 2 and block_table.dtype == torch.int32 and (
-        block_table.stride(1) == 1 or block_table.shape[1] == 1), "block_table [B, max_pages] int32 expected"
-    B = block_table.shape[0]
-    assert B >= 1 and block_table.shape[1] >= 1, "block_table is empty"
-    _check_ints("seq_lens", seq_lens, cache, (B,))
-    assert block_table.device == cache.device, "block_table must be on the cache's device"
-    return B
-
-
 def _check_ints(name, t, cache, shape):
-    assert t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(), \
-        f"{name} {list(shape)} int32 contiguous expected"
-    assert t.device == cache.device, f"{name} must be on the cache's device"
+    assert t.dtype is torch.int32 and t.shape == shape and t.is_contiguous() \
+        and t.get_device() == cache._call[1], \
+        f"{name} {list(shape)} int32 contiguous on the cache's device expected"
 
 
-def _call(cache, what, fn, *args):
+def _table(cache, block_table, seq_lens):
+    """(B, max_pages, row stride) of a call's table, whose lengths are checked too."""
+    assert block_table.dim() == 2 and block_table.dtype is torch.int32 \
+        and block_table.get_device() == cache._call[1], "block_table [B, max_pages] int32 on the cache's device expected"
+    B, max_pages = block_table.shape
+    st_b, st_p = block_table.stride()
+    assert B >= 1 and max_pages >= 1, "block_table is empty"
+    assert st_p == 1 or max_pages == 1, "block_table: a row's entries must be contiguous"
+    _check_ints("seq_lens", seq_lens, cache, (B,))
+    return B, max_pages, st_b
+
+
+def _launch(cache, what, fn, *args):
     """fn(cache, *args, stream) on the cache's device."""
-    device = cache.device
-    if torch._C._cuda_getDevice() == device.index:
-        rc = fn(ctypes.addressof(cache._struct), *args, _capi.stream_ptr(device))
+    address, index, _, _ = cache._call
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(address, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(ctypes.addressof(cache._struct), *args, _capi.stream_ptr(device))
-    _capi.check(rc, what)
+        with torch.cuda.device(index):
+            rc = fn(address, *args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _capi.check(rc, what)
 
 
 def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
@@ -174,32 +181,33 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
     pages, but not ones that both write to.
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
-    B = _check_table(cache, block_table, seq_lens)
-    T, s = k.shape[0], cache._struct
-    k = _check_operand("k", k, cache, (T, s.Hk, s.D))
-    v = _check_operand("v", v, cache, (T, s.Hk, s.D))
+    B, max_pages, st_b = _table(cache, block_table, seq_lens)
+    shape = (k.shape[0], *cache._call[2:])
+    k = _operand("k", k, cache, shape)
+    v = _operand("v", v, cache, shape)
     if cu_new is not None:
         _check_ints("cu_new", cu_new, cache, (B + 1,))
-    _call(cache, "paged_write", _capi.lib().ugbsa_paged_write, k.data_ptr(), *k.stride(),
-          v.data_ptr(), *v.stride(), _capi.ptr(cu_new), seq_lens.data_ptr(), block_table.data_ptr(),
-          block_table.stride(0), B, T, block_table.shape[1])
+    _launch(cache, "paged_write", _capi.lib().ugbsa_paged_write, k.data_ptr(), *k.stride(),
+            v.data_ptr(), *v.stride(), None if cu_new is None else cu_new.data_ptr(), seq_lens.data_ptr(),
+            block_table.data_ptr(), st_b, B, shape[0], max_pages)
 
 
 def paged_read(cache, block_table, seq_lens, n, out=None):
     """(k, v) [B, Hk, n, D] in ``cache.dtype``: the first n cached tokens of every sequence, zeros
     past its length (``out``: a pair of such tensors to fill)."""
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
-    B, s = _check_table(cache, block_table, seq_lens), cache._struct
-    shape = (B, s.Hk, n, s.D)
+    B, max_pages, st_b = _table(cache, block_table, seq_lens)
+    _, index, Hk, D = cache._call
+    shape = (B, Hk, n, D)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
-    k, v = out
-    for t in out:
-        assert tuple(t.shape) == shape and t.dtype == cache.dtype and t.device == cache.device, \
-            f"out: a pair of {list(shape)} in {cache.dtype} expected"
-    _call(cache, "paged_read", _capi.lib().ugbsa_paged_read, seq_lens.data_ptr(), block_table.data_ptr(),
-          block_table.stride(0), B, block_table.shape[1], n, k.data_ptr(), *k.stride(),
-          v.data_ptr(), *v.stride())
+        k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
+    else:
+        k, v = out
+        for t in out:
+            assert t.shape == shape and t.dtype is cache.dtype and t.get_device() == index, \
+                f"out: a pair of {list(shape)} in {cache.dtype} expected"
+    _launch(cache, "paged_read", _capi.lib().ugbsa_paged_read, seq_lens.data_ptr(), block_table.data_ptr(),
+            st_b, B, max_pages, n, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride())
     return k, v
 
 
@@ -216,22 +224,22 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
     other sequence of the batch.  Returns a ``PagedSelection`` for ``paged_decode``.
     """
     assert cache.planes is not None, "the cache keeps no page summaries"
-    B, s = _check_table(cache, block_table, seq_lens), cache._struct
+    B, max_pages, st_b = _table(cache, block_table, seq_lens)
+    _, _, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
-    q = _check_operand("q", q, cache, (B, H, 1, s.D))
-    device, max_pages = cache.device, block_table.shape[1]
-    r = PagedSelection(torch.empty(B, s.Hk, k_slots, dtype=torch.int32, device=device),
-                       torch.empty(B, s.Hk, dtype=torch.int32, device=device),
-                       torch.empty(B, s.Hk, dtype=torch.float32, device=device),
-                       torch.empty(B, s.Hk, dtype=torch.uint8, device=device))
+    q = _operand("q", q, cache, (B, H, 1, D))
+    device = cache.device
+    kv_idx = torch.empty((B, Hk, max(k_slots, 0)), dtype=torch.int32, device=device)
+    counts = torch.empty((B, Hk), dtype=torch.int32, device=device)
+    sigma = torch.empty((B, Hk), dtype=torch.float32, device=device)
+    uncertain = torch.empty((B, Hk), dtype=torch.uint8, device=device)
     lib = _capi.lib()
-    n = lib.ugbsa_paged_select_workspace_elems(B, s.Hk, max_pages)
+    n = lib.ugbsa_paged_select_workspace_elems(B, Hk, max_pages)
     ws = torch.empty(n, dtype=torch.float32, device=device)
-    _call(cache, "paged_select", lib.ugbsa_paged_select, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
-          block_table.data_ptr(), block_table.stride(0), B, max_pages, float(scaling), k_base, k_slots,
-          float(tau), r.kv_idx.data_ptr(), r.counts.data_ptr(), r.sigma.data_ptr(), r.uncertain.data_ptr(),
-          ws.data_ptr(), n)
-    return r
+    _launch(cache, "paged_select", lib.ugbsa_paged_select, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
+            block_table.data_ptr(), st_b, B, max_pages, scaling, k_base, k_slots, tau, kv_idx.data_ptr(),
+            counts.data_ptr(), sigma.data_ptr(), uncertain.data_ptr(), ws.data_ptr(), n)
+    return PagedSelection(kv_idx, counts, sigma, uncertain)
 
 
 def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=None, out=None):
@@ -243,27 +251,30 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     that the KV head's query heads attend to; counts [B, Hk] int32: how many entries count (None:
     all).  Entries that are no page of the sequence are skipped.
     Returns [B, 1, H, D] contiguous, the dispatcher's layout (``out`` if given).  A sequence without
-    a key gives zeros.
+    a key gives zeros.  The launch is shaped by the table's (or list's) width: pass a table cut to
+    the longest sequence where the batch is short.
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
-    B, s = _check_table(cache, block_table, seq_lens), cache._struct
+    B, max_pages, st_b = _table(cache, block_table, seq_lens)
+    _, index, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
-    q = _check_operand("q", q, cache, (B, H, 1, s.D))
+    q = _operand("q", q, cache, (B, H, 1, D))
     slots = 0
     if kv_idx is not None:
         slots = kv_idx.shape[-1]
-        _check_ints("kv_idx", kv_idx, cache, (B, s.Hk, slots))
+        _check_ints("kv_idx", kv_idx, cache, (B, Hk, slots))
     if counts is not None:
-        _check_ints("counts", counts, cache, (B, s.Hk))
+        _check_ints("counts", counts, cache, (B, Hk))
     if out is None:
-        out = torch.empty(B, 1, H, s.D, dtype=cache.dtype, device=cache.device)
-    assert tuple(out.shape) == (B, 1, H, s.D) and out.dtype == cache.dtype and out.device == cache.device
+        out = torch.empty((B, 1, H, D), dtype=cache.dtype, device=cache.device)
+    else:
+        assert out.shape == (B, 1, H, D) and out.dtype is cache.dtype and out.get_device() == index, \
+            f"out: {[B, 1, H, D]} in {cache.dtype} expected"
+    so_b, _, so_h, so_d = out.stride()
     lib = _capi.lib()
-    n = lib.ugbsa_paged_decode_workspace_elems(B, H, s.Hk, s.D, slots or block_table.shape[1],
-                                               s.cache_dtype)
+    n = lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
     ws = torch.empty(n, dtype=torch.float32, device=cache.device) if n else None
-    _call(cache, "paged_decode", lib.ugbsa_paged_decode, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
-          block_table.data_ptr(), block_table.stride(0), B, block_table.shape[1], float(scale),
-          _capi.ptr(kv_idx), _capi.ptr(counts), slots, out.data_ptr(), out.stride(0), out.stride(2),
-          out.stride(3), _capi.ptr(ws), n)
+    _launch(cache, "paged_decode", lib.ugbsa_paged_decode, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
+            block_table.data_ptr(), st_b, B, max_pages, scale, _capi.ptr(kv_idx), _capi.ptr(counts), slots,
+            out.data_ptr(), so_b, so_h, so_d, _capi.ptr(ws), n)
     return out
