@@ -348,7 +348,7 @@ int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_
 
 /* Cached tokens back: k_out, v_out [B, Hk, N, D] of dtype (the prefill entry
  * points' layout), row n of sequence b its token n, zeros from lens[b] on.
- * Exact: e4m3 values are values of dtype. */
+ * Exact: e4m3 values are values of dtype.  N <= 2^29. */
 int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const int32_t* table,
                      int64_t st_b, int B, int max_pages, int N, void* k_out, int64_t sk_b,
                      int64_t sk_h, int64_t sk_n, int64_t sk_d, void* v_out, int64_t sv_b,
@@ -367,8 +367,9 @@ int64_t ugbsa_paged_select_workspace_elems(int B, int Hk, int max_pages);
  * k_base - 2; 2 where no page is cut.  Out: kv_idx [B, Hk, k_slots] int32, page
  * numbers within the sequence, ascending, then max_pages; counts [B, Hk] int32;
  * sigma [B, Hk] fp32 and uncertain [B, Hk] uint8 (either may be NULL).
- * 3 <= k_base <= k_slots; scaling positive and finite; workspace 8-byte
- * aligned. */
+ * A NaN score ranks first and makes sigma NaN, which is not below tau.  3 <=
+ * k_base <= k_slots; scaling positive and finite; B * Hk < 2^23, B * Hk *
+ * max_pages <= 2^29; workspace 8-byte aligned. */
 int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
                        int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
                        const int32_t* table, int64_t st_b, int B, int max_pages, float scaling,

@@ -642,7 +642,7 @@ int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const 
   if (rc || (rc = check_pages(cache))) return rc;
   if ((rc = check_bf16_operand("k_out", k_out, sk_b, sk_h, sk_n, sk_d))) return rc;
   if ((rc = check_bf16_operand("v_out", v_out, sv_b, sv_h, sv_n, sv_d))) return rc;
-  if (N < 1 || N > 1 << 30) return fail(UGBSA_EARG, "N must lie in [1, 2^30] (%d)", N);
+  if (N < 1 || N > 1 << 29) return fail(UGBSA_EARG, "N must lie in [1, 2^29] (%d)", N);
   return hip_result(ugbsa::launch_paged_read(paged_cache(cache), lens, table, st_b, B, max_pages, N,
                                              static_cast<uint16_t*>(k_out), sk_b, sk_h, sk_n,
                                              static_cast<uint16_t*>(v_out), sv_b, sv_h, sv_n,
@@ -676,7 +676,8 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
     return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_select_workspace_elems (%lld)",
                 (long long)workspace_elems, (long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 7) return fail(UGBSA_ELAYOUT, "workspace must be 8-byte aligned");
-  if (static_cast<int64_t>(B) * cache->Hk >= 1 << 24) return fail(UGBSA_EARG, "B * Hk must be below 2^24");
+  if (static_cast<int64_t>(B) * cache->Hk >= 1 << 23 || static_cast<int64_t>(B) * cache->Hk * max_pages > 1 << 29)
+    return fail(UGBSA_EARG, "B * Hk must be below 2^23 and B * Hk * max_pages at most 2^29");
   return hip_result(ugbsa::launch_paged_select(paged_cache(cache), static_cast<const uint16_t*>(q), sq_b,
                                                sq_h, B, H, lens, table, st_b, max_pages, scaling, k_base,
                                                k_slots, tau, kv_idx, counts, sigma, uncertain,

@@ -92,7 +92,9 @@ __global__ __launch_bounds__(64 * pd_waves(ONE), ONE ? 2 : pd_occupancy(D, F8)) 
 
   int group, member, n, x0, u, u_end;              // n: units of the row, x0 of them before u
   if constexpr (ONE) {
-    group = blockIdx.x / gr.members, member = blockIdx.x % gr.members;
+    const bool lists = rows.kv_idx != nullptr;
+    group = lists ? blockIdx.y * gr.Hk + blockIdx.x / chunks : blockIdx.y;
+    member = lists ? blockIdx.x % chunks : blockIdx.x;
     n = row_units(__builtin_amdgcn_readfirstlane(group_units(rows, gr.Hk, group)));
     x0 = u = 0, u_end = n;
   } else {
@@ -518,7 +520,7 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
   const bool lists = rows.kv_idx != nullptr;
   const PagedGroups gr{lists ? B * c.Hk : B, lists ? chunks : c.Hk * chunks, c.Hk};
   if (paged_decode_one(D, F8, lists ? rows.k_slots : rows.max_pages)) {
-    paged_decode_kernel<E, D, F8, false, true><<<dim3(B * c.Hk * chunks), 64 * pd_waves(true), 0, stream>>>(
+    paged_decode_kernel<E, D, F8, false, true><<<dim3(c.Hk * chunks, B), 64 * pd_waves(true), 0, stream>>>(
         c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out, so_b, so_h, nullptr, nullptr, nullptr);
     return hipGetLastError();
   }

