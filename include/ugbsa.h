@@ -354,7 +354,8 @@ int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const 
                      int64_t sk_h, int64_t sk_n, int64_t sk_d, void* v_out, int64_t sv_b,
                      int64_t sv_h, int64_t sv_n, int64_t sv_d, void* stream);
 
-/* fp32 elements of a ugbsa_paged_select workspace (0 for sizes no call takes). */
+/* fp32 elements of a ugbsa_paged_select workspace (0 for sizes no call takes); none
+ * is needed where max_pages <= k_base. */
 int64_t ugbsa_paged_select_workspace_elems(int B, int Hk, int max_pages);
 
 /* Pages for one new token of each sequence: q [B, H, 1, D] of dtype, lens with

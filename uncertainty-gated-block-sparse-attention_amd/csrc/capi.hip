@@ -671,8 +671,8 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
   if (!(scaling > 0.f && scaling <= 3.4e38f)) return fail(UGBSA_EARG, "scaling must be positive and finite");
   if (tau != tau) return fail(UGBSA_EARG, "tau is NaN");
   if (kv_idx == nullptr || counts == nullptr) return fail(UGBSA_EARG, "kv_idx or counts is null");
-  const int64_t need = ugbsa_paged_select_workspace_elems(B, cache->Hk, max_pages);
-  if (workspace == nullptr || workspace_elems < need)
+  const int64_t need = max_pages <= k_base ? 0 : ugbsa_paged_select_workspace_elems(B, cache->Hk, max_pages);
+  if (need > 0 && (workspace == nullptr || workspace_elems < need))
     return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_select_workspace_elems (%lld)",
                 (long long)workspace_elems, (long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 7) return fail(UGBSA_ELAYOUT, "workspace must be 8-byte aligned");

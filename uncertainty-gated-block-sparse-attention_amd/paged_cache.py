@@ -236,11 +236,11 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
     sigma = torch.empty((B, Hk), dtype=torch.float32, device=device)
     uncertain = torch.empty((B, Hk), dtype=torch.uint8, device=device)
     lib = _capi.lib()
-    n = lib.ugbsa_paged_select_workspace_elems(B, Hk, max_pages)
-    ws = torch.empty(n, dtype=torch.float32, device=device)
+    n = lib.ugbsa_paged_select_workspace_elems(B, Hk, max_pages) if max_pages > k_base else 0
+    ws = torch.empty(n, dtype=torch.float32, device=device) if n else None
     _launch(cache, "paged_select", lib.ugbsa_paged_select, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
             block_table.data_ptr(), st_b, B, max_pages, scaling, k_base, k_slots, tau, kv_idx.data_ptr(),
-            counts.data_ptr(), sigma.data_ptr(), uncertain.data_ptr(), ws.data_ptr(), n)
+            counts.data_ptr(), sigma.data_ptr(), uncertain.data_ptr(), _capi.ptr(ws), n)
     return PagedSelection(kv_idx, counts, sigma, uncertain)
 
 
