@@ -423,7 +423,8 @@ SHAPES = [(8, 8, 64, BF, False), (8, 2, 64, FH, True), (28, 4, 128, BF, False), 
 
 # Lengths around the step, the page and the splits, with slots without a sequence; slots past a
 # length and pages of no sequence hold NaN.
-@pytest.mark.parametrize("lens", [[1], [0, 31, 32, 33, 63, 64, 65], [511, 0, 1000, 2], [4097], [300] * 40])
+@pytest.mark.parametrize("lens", [[1], [0, 31, 32, 33, 63, 64, 65], [511, 0, 1000, 2], [4097], [300] * 40,
+                                  [130, 0, 256, 1] * 33])
 @pytest.mark.parametrize("H,Hk,D,dtype,e4m3", SHAPES)
 def test_decode(hip_lib, lens, H, Hk, D, dtype, e4m3):
     print(f"[case] paged decode {lens[:7]} H={H}/{Hk} D={D} {dtype} {e4m3}", flush=True)

@@ -71,11 +71,9 @@ __host__ __device__ constexpr int pd_occupancy(int D, bool F8) {
   return D == 64 ? 4 : (D == 128 ? (F8 ? 3 : 2) : (F8 ? 2 : 1));
 }
 
-// Wavefronts of a workgroup: four, or eight where it has a row to itself.
-__host__ __device__ constexpr int pd_waves(bool one) { return one ? 8 : kPdWaves; }
-
-template <typename E, int D, bool F8, bool NT, bool ONE>
-__global__ __launch_bounds__(64 * pd_waves(ONE), ONE ? 2 : pd_occupancy(D, F8)) void paged_decode_kernel(
+// ONE: the wavefronts of a workgroup that has a row to itself, 0: workgroups on the line.
+template <typename E, int D, bool F8, bool NT, int ONE>
+__global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy(D, F8)) void paged_decode_kernel(
     PagedCache c, PagedRows rows, PagedGroups gr, const uint16_t* __restrict__ q, int64_t sq_b,
     int64_t sq_h, int grp, int chunks, float scale_log2, uint16_t* __restrict__ out, int64_t so_b,
     int64_t so_h, int* __restrict__ starts, float* __restrict__ part, float* __restrict__ ml) {
@@ -83,7 +81,7 @@ __global__ __launch_bounds__(64 * pd_waves(ONE), ONE ? 2 : pd_occupancy(D, F8)) 
   constexpr int DPL = D / 16;                    // dims a lane loads per key of V
   // 16-bit rows are read 8 dims a load, or 4 at head_dim 64 (VW = dims a load)
   constexpr int VW = F8 ? DPL : (D == 64 ? 4 : 8), VL = DPL / VW;
-  constexpr int SZ = F8 ? 1 : 2, WAVES = pd_waves(ONE);
+  constexpr int SZ = F8 ? 1 : 2, WAVES = ONE ? ONE : kPdWaves;
   __shared__ float s_o[WAVES][NH][D + 4];
   __shared__ float s_ml[WAVES][NH][2];
   __shared__ int s_sum[WAVES], s_start[2];
@@ -91,7 +89,7 @@ __global__ __launch_bounds__(64 * pd_waves(ONE), ONE ? 2 : pd_occupancy(D, F8)) 
   const int g4 = lane >> 4, r16 = lane & 15;
 
   int group, member, n, x0, u, u_end;              // n: units of the row, x0 of them before u
-  if constexpr (ONE) {
+  if constexpr (ONE != 0) {
     const bool lists = rows.kv_idx != nullptr;
     group = lists ? blockIdx.y * gr.Hk + blockIdx.x / chunks : blockIdx.y;
     member = lists ? blockIdx.x % chunks : blockIdx.x;
@@ -520,8 +518,15 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
   const bool lists = rows.kv_idx != nullptr;
   const PagedGroups gr{lists ? B * c.Hk : B, lists ? chunks : c.Hk * chunks, c.Hk};
   if (paged_decode_one(D, F8, lists ? rows.k_slots : rows.max_pages)) {
-    paged_decode_kernel<E, D, F8, false, true><<<dim3(c.Hk * chunks, B), 64 * pd_waves(true), 0, stream>>>(
-        c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out, so_b, so_h, nullptr, nullptr, nullptr);
+    // Eight wavefronts a row; four where there are more rows than CUs and a CU's
+    // registers hold one workgroup of eight but two or three of four (1024 sequences of
+    // up to 1K tokens, e4m3, head_dim 128 106 / 80.5 us, 64 x 8 heads 23.4 / 22.2, but 32 x
+    // 4 heads 11.4 / 13.5; head_dim 64 25.4 / 26.3).
+    const bool four = D >= 128 && static_cast<int64_t>(B) * c.Hk * chunks > 256;
+    const auto kernel = four ? paged_decode_kernel<E, D, F8, false, 4> : paged_decode_kernel<E, D, F8, false, 8>;
+    kernel<<<dim3(c.Hk * chunks, B), 64 * (four ? 4 : 8), 0, stream>>>(c, rows, gr, q, sq_b, sq_h, grp, chunks,
+                                                                       scale * kLog2e, out, so_b, so_h, nullptr,
+                                                                       nullptr, nullptr);
     return hipGetLastError();
   }
   const int wgs = paged_decode_workgroups(B, H, c.Hk, D, F8, lists ? rows.k_slots : rows.max_pages);
@@ -536,8 +541,8 @@ static hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& ro
   // 42.2).  The table's width bounds the lengths, which are on the device.
   const int64_t most = static_cast<int64_t>(B) * c.Hk * (lists ? rows.k_slots : rows.max_pages) *
                        (2 * kBlock * D * (F8 ? 1 : 2));
-  const auto kernel = most > 768ll << 20 ? paged_decode_kernel<E, D, F8, true, false>
-                                         : paged_decode_kernel<E, D, F8, false, false>;
+  const auto kernel = most > 768ll << 20 ? paged_decode_kernel<E, D, F8, true, 0>
+                                         : paged_decode_kernel<E, D, F8, false, 0>;
   kernel<<<dim3(wgs), 64 * kPdWaves, 0, stream>>>(c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out,
                                                   so_b, so_h, starts, part, ml);
   const hipError_t e = hipGetLastError();
