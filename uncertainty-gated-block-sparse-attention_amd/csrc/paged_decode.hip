@@ -6,12 +6,17 @@
 // head's query heads as the columns, K and V straight from the pages into operand
 // registers.  e4m3 pages are widened there, times their tokens' scales, which is
 // exact in either 16-bit format.
+//
+// Bound by memory: 32 sequences of 64K tokens, 40/8 heads, e4m3 (4.3 GB) 698 us, 6.2
+// TB/s; 24 of up to 16K, bf16 (375 MB) 69.5 us, 5.4 TB/s with the joining launch; one of
+// 1000 tokens 11 us, two launches of about 4 us.
 #include "paged.h"
 
 namespace ugbsa {
 
 constexpr int kPdWaves = 4;       // wavefronts per workgroup
 constexpr int kPdStep = 32;       // keys per wavefront step: half a page
+
 // Four dims of a head, over their weights' sum; a row without a key, or whose every
 // weight is 0, gives zeros.
 template <typename E>
