@@ -727,3 +727,115 @@ def test_refusals(hip_lib):
     # read as their values: strided and negated views
     for x in (q.transpose(2, 3).contiguous().transpose(2, 3), torch._neg_view(-q)):
         assert torch.equal(pc.paged_decode(x, cache, table, seq, 0.1), pc.paged_decode(q, cache, table, seq, 0.1))
+
+
+# ---- selection at the ends of the score range ---------------------------------------------------
+
+def cut_ref(score, scale, k_base, k_slots, tau, NB):
+    """(list, count, sigma, flag) of one row from its pages' fp64 scores; NaN ranks first."""
+    nb = len(score)
+    order = sorted(range(1, nb - 1), key=lambda j: (0, 0, j) if math.isnan(score[j]) else (1, -score[j], j))
+    keep, k, sigma = min(k_base, nb), k_base - 2, 2.0
+    if nb > k_base:
+        first, last, below = (score[order[i]] * scale for i in (0, k - 1, k))
+        gap, reach = last - below, first - below
+        sigma = NAN if math.isnan(gap) or math.isnan(reach) or math.isinf(gap) else \
+            min(max(gap / max(reach, 1e-9), 0.0), 2.0)
+        if sigma < tau:
+            keep = min(k_slots, nb)
+    kept = list(range(nb)) if nb <= keep else sorted([0, nb - 1] + order[:keep - 2])
+    return kept + [NB] * (k_slots - len(kept)), keep, sigma, int(sigma < tau)
+
+
+def page_scores(q, planes, table):
+    """fp64 scores [Hk, pages] of one sequence by the definition; absent pages are -inf."""
+    Hk, P = planes.shape[1], planes.shape[0]
+    there = (table >= 0) & (table < P)
+    pl = planes[table.clamp(0, P - 1).long()].double().transpose(0, 1)            # [Hk, pages, 2, D]
+    x = q.view(Hk, -1, q.shape[-1]).double()                                      # [Hk, G, D]
+    s = torch.stack([torch.where(x[:, i:i + 1] >= 0, x[:, i:i + 1] * pl[:, :, 0],
+                                 x[:, i:i + 1] * pl[:, :, 1]).sum(-1) for i in range(x.shape[1])]).amax(0)
+    return torch.where(there, s, -INF)
+
+
+def select_guarded(q, cache, table, lens, scale, k_base, k_slots, tau):
+    """(kv_idx, counts, sigma, uncertain) through the C ABI, the lists between guard values."""
+    B, H, _, D = q.shape
+    Hk, NB, lib = cache.planes.shape[1], table.shape[1], _capi.lib()
+    n = B * Hk * k_slots
+    wide = torch.full((n + 8192,), -77, dtype=torch.int32, device=DEV)
+    lists = wide[4096:4096 + n]
+    counts = torch.empty(B, Hk, dtype=torch.int32, device=DEV)
+    sigma = torch.empty(B, Hk, device=DEV)
+    flags = torch.empty(B, Hk, dtype=torch.uint8, device=DEV)
+    ws = torch.empty(lib.ugbsa_paged_select_workspace_elems(B, Hk, NB), device=DEV)
+    _capi.check(lib.ugbsa_paged_select(
+        cache._call[0], q.data_ptr(), *q.stride(), H, lens.data_ptr(), table.data_ptr(), table.stride(0), B,
+        NB, scale, k_base, k_slots, tau, lists.data_ptr(), counts.data_ptr(), sigma.data_ptr(),
+        flags.data_ptr(), ws.data_ptr(), ws.numel(), _capi.stream_ptr(DEV)), "paged_select")
+    assert (wide[:4096] == -77).all() and (wide[4096 + n:] == -77).all()
+    return lists.view(B, Hk, k_slots), counts, sigma, flags
+
+
+def check_cut(q, cache, table, lens, scale, k_base, k_slots, tau):
+    got = select_guarded(q, cache, table, i32(lens), scale, k_base, k_slots, tau)
+    for b, n in enumerate(lens):
+        nb = (n + 63) // 64
+        score = page_scores(q[b, :, 0], cache.planes, table[b, :nb]).tolist()
+        for h, row in enumerate(score):
+            kept, keep, sigma, flag = cut_ref(row, scale, k_base, k_slots, tau, table.shape[1])
+            assert got[0][b, h].tolist() == kept, (b, h)
+            assert (int(got[1][b, h]), int(got[3][b, h])) == (keep, flag), (b, h)
+            s = float(got[2][b, h])
+            assert not abs(s - sigma) > 2.0 ** -24 * sigma + 1e-12, (b, h)
+
+
+# Rows of every form of the pick (128, 256 and 512 threads with their keys in registers, and longer).
+@pytest.mark.parametrize("nb", [60, 1500, 3000, 5000])
+@pytest.mark.parametrize("value", [INF, NAN])
+def test_select_cut_among_infinite_and_nan_pages(hip_lib, nb, value):
+    """Fewer, as many and more such pages than the list has places, with and without absent pages."""
+    print(f"[case] select among {value} pages nb={nb}", flush=True)
+    g = gen(nb)
+    k_base, k_slots = 8, 20
+    for n in (1, 5, 6, 7, 18, 19, 40):
+        for absent in (0, 3):
+            cache = filled(g, 2 * nb + 1, 2, 64, BF, False)
+            table = torch.randperm(2 * nb, generator=g, device=DEV).view(2, nb).int()
+            q = torch.randn(2, 6, 1, 64, generator=g, device=DEV).to(BF)
+            q[..., 0] = 1.0
+            for h in range(2):
+                at = table[:, 1:nb - 1].gather(1, torch.rand(2, nb - 2, generator=g, device=DEV).argsort(1)[:, :n])
+                cache.planes[at[0].long(), h, 0, 0] = value
+                cache.planes[at[1, :n - h].long(), h, 0, 0] = value
+            table[:, 2:2 + absent] = -1
+            check_cut(q, cache, table, [64 * nb, 64 * nb - 63], 0.125, k_base, k_slots, 0.05)
+
+
+def test_select_of_a_nan_query(hip_lib):
+    """Every page's score is NaN but an absent one's; the other sequence's list is its own."""
+    g = gen(20)
+    for nb in (70, 1100):
+        cache = filled(g, 2 * nb, 1, 64, FH, False)
+        table = torch.arange(2 * nb, device=DEV, dtype=torch.int32).view(2, nb)
+        table[0, 9] = -1
+        q = torch.randn(2, 4, 1, 64, generator=g, device=DEV).to(FH)
+        q[0, :, :, 3] = NAN
+        check_cut(q, cache, table, [64 * nb, 64 * nb], 0.125, 64, 66, 0.05)
+
+
+# A cut whose first bin holds more keys than a workgroup has threads is looked for in it again.
+@pytest.mark.parametrize("nb", [600, 1500, 3000, 5000])
+def test_select_cut_among_near_equal_scores(hip_lib, nb):
+    cache = filled(gen(21), nb, 1, 64, BF, False)
+    i = torch.randperm(nb, generator=gen(22), device=DEV)
+    cache.planes[:] = 0.0
+    cache.planes[:, :, :, 0] = 1.0
+    cache.planes[:, 0, :, 1] = ((i % 256) * 2.0 ** -30).to(BF).unsqueeze(-1)      # all exact in fp64
+    cache.planes[:, 0, :, 2] = ((i // 256) * 2.0 ** -22).to(BF).unsqueeze(-1)
+    q = torch.ones(1, 2, 1, 64, device=DEV, dtype=BF)
+    for far in (2.0 ** 100, -2.0 ** 100):
+        cache.planes[nb // 2, :, :, 3] = far
+        table = torch.arange(nb, device=DEV, dtype=torch.int32).view(1, nb)
+        for k_base, k_slots, tau in ((5, 9, 0.0), (400, 500, 1.5), (580, 590, 0.0)):
+            check_cut(q, cache, table, [64 * nb], 0.125, k_base, k_slots, tau)

@@ -286,7 +286,9 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(
       }
       __syncthreads();
       lo += static_cast<uint64_t>(s_bin) << shift;
-      hi = lo + ((1ull << shift) - 1);
+      // the topmost bin may reach past hi, and past 2^64 where hi is NaN's or +inf's key
+      const uint64_t span = (1ull << shift) - 1;
+      hi = hi - lo < span ? hi : lo + span;
       left = s_left;
       if (shift == 0) return lo;
       if (s_in <= NT) break;
@@ -366,7 +368,9 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(
     each([&](int i, uint64_t x) {
       if (j0 + i >= nb) return;
       const bool tie = !forced(i) && x == cut;
-      if (forced(i) || x > cut || (tie && e < room)) list[o + min(e, room)] = j0 + i;
+      const int at = o + min(e, room);
+      if ((forced(i) || x > cut || (tie && e < room)) && static_cast<uint32_t>(at) < static_cast<uint32_t>(keep))
+        list[at] = j0 + i;
       o += forced(i) || x > cut;
       e += tie;
     });
