@@ -787,7 +787,7 @@ def check_cut(q, cache, table, lens, scale, k_base, k_slots, tau):
             assert got[0][b, h].tolist() == kept, (b, h)
             assert (int(got[1][b, h]), int(got[3][b, h])) == (keep, flag), (b, h)
             s = float(got[2][b, h])
-            assert not abs(s - sigma) > 2.0 ** -24 * sigma + 1e-12, (b, h)
+            assert math.isnan(s) == math.isnan(sigma) and not abs(s - sigma) > 2.0 ** -24 * sigma + 1e-12, (b, h)
 
 
 # Rows of every form of the pick (128, 256 and 512 threads with their keys in registers, and longer).
@@ -810,6 +810,18 @@ def test_select_cut_among_infinite_and_nan_pages(hip_lib, nb, value):
                 cache.planes[at[1, :n - h].long(), h, 0, 0] = value
             table[:, 2:2 + absent] = -1
             check_cut(q, cache, table, [64 * nb, 64 * nb - 63], 0.125, k_base, k_slots, 0.05)
+
+
+def test_select_sigma_of_one_nan_page(hip_lib):
+    """The page ranks first and the cut lies among finite scores: sigma is NaN, below no tau."""
+    g = gen(23)
+    cache = filled(g, 40, 1, 64, BF, False)
+    cache.planes[17, 0, :, 5] = NAN
+    q = torch.randn(1, 4, 1, 64, generator=g, device=DEV).to(BF)
+    r = pc.paged_select(q, cache, torch.arange(40, device=DEV, dtype=torch.int32).view(1, 40), i32([40 * 64]),
+                        0.125, 8, 16, tau=3.0)
+    assert r.sigma.isnan().all() and r.uncertain.tolist() == [[0]] and r.counts.tolist() == [[8]]
+    assert 17 in r.kv_idx[0, 0].tolist()
 
 
 def test_select_of_a_nan_query(hip_lib):

@@ -327,7 +327,8 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(
     uint64_t below;
     reduce(mx, ~0ull, n, below, unused, all);
     const double sc = scaling, c = key_double(all > k ? a : below) * sc;
-    const double reach = key_double(top) * sc - c, ratio = (key_double(a) * sc - c) / (reach > 1e-9 ? reach : 1e-9);
+    const double reach = key_double(top) * sc - c;         // NaN stays NaN
+    const double ratio = (key_double(a) * sc - c) / (reach < 1e-9 ? 1e-9 : reach);
     const double clamped = ratio < 0.0 ? 0.0 : (ratio > 2.0 ? 2.0 : ratio);
     sg = static_cast<float>(clamped);
     unsure = clamped < static_cast<double>(tau);
