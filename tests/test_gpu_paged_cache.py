@@ -851,3 +851,22 @@ def test_select_cut_among_near_equal_scores(hip_lib, nb):
         table = torch.arange(nb, device=DEV, dtype=torch.int32).view(1, nb)
         for k_base, k_slots, tau in ((5, 9, 0.0), (400, 500, 1.5), (580, 590, 0.0)):
             check_cut(q, cache, table, [64 * nb], 0.125, k_base, k_slots, tau)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("heads", [1, 5, 9])
+def test_select_bounds_of_different_magnitude(hip_lib, D, heads):
+    """The bound that a dim does not take is 2^60 times the one it takes: no part of the score.  The
+    scores are whole numbers, so their sums are exact in any order."""
+    g = gen(D + heads)
+    nb = 40
+    cache = filled(g, nb, 2, D, BF, False)
+    small = torch.randint(-8, 9, (nb, D), generator=g, device=DEV).to(BF)
+    huge = (2.0 ** 60 * torch.randint(1, 9, (nb, D), generator=g, device=DEV)).to(BF)
+    cache.planes[:, 0, 0], cache.planes[:, 0, 1] = small, -huge        # taken by q >= 0
+    cache.planes[:, 1, 0], cache.planes[:, 1, 1] = huge, small         # taken by q < 0
+    q = torch.randint(1, 9, (1, 2 * heads, 1, D), generator=g, device=DEV).to(BF)
+    q[:, heads:] *= -1
+    table = torch.arange(nb, device=DEV, dtype=torch.int32).view(1, nb)
+    for k_base, k_slots, tau in ((6, 12, 0.02), (20, 30, 0.0)):
+        check_cut(q, cache, table, [64 * nb], 0.125, k_base, k_slots, tau)

@@ -10,11 +10,12 @@
 //           scaling, s(i) the i-th best, k' = k_base - 2; 2 where nothing is cut.
 //
 // The list decides whole pages, so near ties matter: scores are summed in fp64,
-// where the 16-bit products are exact and sums of them round far below any
-// spacing of theirs.
+// where the 16-bit products are exact and a sum rounds at 2^-53 of the terms that the
+// score consists of; the bound that a dim does not take has no part in it, however
+// large it is.
 //
-// 64 sequences of up to 128K tokens, 40/8 heads (119 MB of planes): scoring 48 us,
-// picking 10.7; one of 32K, 28/4 heads, 3.8 and 6.9.
+// 64 sequences of up to 128K tokens, 40/8 heads (119 MB of planes): scoring 49 us,
+// picking 11; one of 32K, 28/4 heads, 4.3 and 6.9.
 #include "paged.h"
 
 namespace ugbsa {
@@ -58,16 +59,10 @@ __device__ __forceinline__ double group_sum(double x) {
   return x;
 }
 
-// The score of one page by its definition, read from memory: for planes that hold
-// infinities or NaN, where the sums below are not the definition's.
-template <typename E, int D>
-__device__ double plain_score(const uint16_t* pl, const uint16_t* q) {
-  double s = 0.0;
-  for (int d = 0; d < D; ++d) {
-    const float x = E::to_f32(q[d]);
-    s += static_cast<double>(x) * E::to_f32(x >= 0.f ? pl[d] : pl[D + d]);
-  }
-  return s;
+// fp64 of a 16-bit value: its lower word is 0, so the upper one stands for it.
+template <typename E>
+__device__ __forceinline__ uint32_t double_top(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_bit_cast(uint64_t, static_cast<double>(E::to_f32(x))) >> 32);
 }
 
 constexpr int kScoreAhead = 2;          // steps of a wavefront whose loads are in flight
@@ -75,12 +70,9 @@ constexpr int kScoreAhead = 2;          // steps of a wavefront whose loads are 
 // keys [B, Hk, max_pages] of the pages between the first and the last of each row.
 //
 // D / 8 lanes take a page, 8 dims each, so a wavefront reads 64 / (D / 8) pages' whole
-// planes per step, two 16-byte loads a lane.  Twice the score is
-//   sum_d q_d (kmax_d + kmin_d) + |q_d| (kmax_d - kmin_d),
-// two fp64 FMAs a dim and head (|q| is a source modifier) and no select by the sign
-// of q; the sums and differences are shared by the GC heads of a pass, whose q stay
-// in registers as fp64.  fp64 FMAs run at the fp32 rate here, and the pass is
-// bound by them and the 4 D bytes a page about equally at five heads.
+// planes per step, two 16-byte loads a lane, and converts them to fp64 once for the GC
+// heads of a pass, whose q stay in registers as fp64: per dim and head a select by the
+// sign of q and an fp64 FMA, which runs at the fp32 rate here.
 template <typename E, int D, int GC>
 __global__ __launch_bounds__(256) void paged_score_kernel(
     PagedCache c, const uint16_t* __restrict__ q, int64_t sq_b, int64_t sq_h, int grp,
@@ -129,42 +121,28 @@ __global__ __launch_bounds__(256) void paged_score_kernel(
         if (j >= j1) return;
         const u32x4 hi = his[s], lo = los[s];
         const int at = pages[s];
-        double sum[8], dif[8];
+        uint32_t top[8], low[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const double a = E::to_f32(hi[i] & 0xFFFFu), z = E::to_f32(lo[i] & 0xFFFFu);
-          const double a1 = E::to_f32(hi[i] >> 16), z1 = E::to_f32(lo[i] >> 16);
-          sum[2 * i] = a + z, dif[2 * i] = a - z;
-          sum[2 * i + 1] = a1 + z1, dif[2 * i + 1] = a1 - z1;
+          top[2 * i] = double_top<E>(hi[i] & 0xFFFFu), low[2 * i] = double_top<E>(lo[i] & 0xFFFFu);
+          top[2 * i + 1] = double_top<E>(hi[i] >> 16), low[2 * i + 1] = double_top<E>(lo[i] >> 16);
         }
         const int ahead = j + kScoreAhead * NP;
         if (ahead < j1) load(ahead, his[s], los[s], pages[s]);
         double best = -INFINITY;
-        bool odd = false;
 #pragma unroll
         for (int h = 0; h < GC; ++h) {
           double acc = 0.0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            acc = __builtin_fma(qd[h][i], sum[i], acc);
-            acc = __builtin_fma(__builtin_fabs(qd[h][i]), dif[i], acc);
+            const uint32_t w = qd[h][i] >= 0.0 ? top[i] : low[i];
+            acc = __builtin_fma(qd[h][i], __builtin_bit_cast(double, static_cast<uint64_t>(w) << 32), acc);
           }
           acc = group_sum<LP>(acc);
-          odd |= acc != acc;
-          best = acc > best ? acc : best;
+          best = acc > best || acc != acc ? acc : best;        // NaN stays
         }
-        best *= 0.5;
         if (lane % LP != 0 || j + sub >= j1) return;
-        if (at < 0) {
-          best = -INFINITY;
-        } else if (odd || best == INFINITY || best == -INFINITY) {
-          best = -INFINITY;
-          const uint16_t* pl = c.planes + (static_cast<int64_t>(at) * c.Hk + g) * 2 * D;
-          for (int h = 0; h < min(GC, grp - h0); ++h) {
-            const double x = plain_score<E, D>(pl, qh + h * sq_h);
-            best = (x > best || x != x) ? x : best;
-          }
-        }
+        if (at < 0) best = -INFINITY;
         uint64_t key = double_key(best);
         if (h0 > 0) {                                // the earlier heads' best, by this lane
           const uint64_t before = kr[j + sub];
@@ -397,12 +375,11 @@ static hipError_t launch_paged_select_t(const PagedCache& c, const uint16_t* q, 
   // heads a pass: an even share of the group, at most the 8 whose q fit the registers
   const int grp = H / c.Hk, passes = (grp + 7) / 8, gc = (grp + passes - 1) / passes;
   // pages a wavefront: as many as leave the card 4096 wavefronts, from one step to
-  // 16 (64 sequences of up to 128K tokens, both launches: 8 / 16 / 32 / 64 pages 62.7 /
-  // 56.4 / 62.1 / 79 us; with four steps' loads in flight instead of two, which cost a
-  // wavefront per SIMD, 78.8 / 67.1 / 75 / 88)
+  // 24 (64 sequences of up to 128K tokens, 40/8 heads, this launch: 16 / 24 / 32 pages
+  // 56.2 / 49.4 / 59.9 us at two wavefronts per SIMD)
   constexpr int NP = 512 / D;
   const int64_t pages = static_cast<int64_t>(B) * c.Hk * max_pages;
-  int per = static_cast<int>(pages / 4096 < 16 ? pages / 4096 : 16) / NP * NP;
+  int per = static_cast<int>(pages / 4096 < 24 ? pages / 4096 : 24) / NP * NP;
   if (per < NP) per = NP;
   const dim3 grid((max_pages + 4 * per - 1) / (4 * per) * c.Hk, B);
 #define UGBSA_SCORE(GC_)                                                                          \
