@@ -1,6 +1,7 @@
 """The paged cache's argument checks and size queries, which need no GPU."""
 
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -118,3 +119,30 @@ def test_caches_of_host_tensors_are_refused():
                  lambda: pc.PagedCache.empty(2, 1, 64, torch.bfloat16, "cpu", e4m3=True)):
         with pytest.raises(AssertionError):
             make()
+
+
+# ---- argument checks of the Python calls, on host tensors ----------------------------------------
+
+def host_cache(dtype=torch.bfloat16, Hk=2, D=64, P=3):
+    """What the calls look at of a cache; pages that no call gets as far as reading."""
+    pages = torch.zeros(P, Hk, 64, D, dtype=dtype)
+    return SimpleNamespace(dtype=dtype, device=torch.device("cpu"), k_pages=pages, v_pages=pages.clone(),
+                           planes=torch.zeros(P, Hk, 2, D, dtype=dtype), _call=(None, -1, Hk, D),
+                           _struct=SimpleNamespace(cache_dtype=_capi.CACHE_MODEL))
+
+
+def test_decode_refuses_an_empty_list(monkeypatch):
+    """A list of no entries is no call for every page, which is what a null list asks the C side for."""
+    def launched(*a):
+        raise RuntimeError("launched")
+    monkeypatch.setattr(pc, "_launch", launched)
+    cache, q = host_cache(), torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for shape in ((1, 2, 0), (2,), ()):
+        with pytest.raises(AssertionError, match="at least one slot"):
+            pc.paged_decode(q, cache, table, lens, 0.1, kv_idx=torch.zeros(shape, dtype=torch.int32))
+    lists = torch.zeros(1, 2, 5, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="at least one slot"):
+        pc.paged_decode(q, cache, table, lens, 0.1, kv_idx=lists[..., :0])
+    with pytest.raises(RuntimeError, match="launched"):
+        pc.paged_decode(q, cache, table, lens, 0.1, kv_idx=lists[..., :1].contiguous())

@@ -249,7 +249,7 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     listed ones.
 
     q : [B, H, 1, D]; seq_lens counts the new token, which ``paged_write`` has put in the cache
-    kv_idx : [B, Hk, k_slots] int32, the pages (numbered within the sequence, each at most once)
+    kv_idx : [B, Hk, k_slots >= 1] int32, the pages (numbered within the sequence, each at most once)
     that the KV head's query heads attend to; counts [B, Hk] int32: how many entries count (None:
     all).  Entries that are no page of the sequence are skipped.
     Returns [B, 1, H, D] contiguous, the dispatcher's layout (``out`` if given).  A sequence without
@@ -263,7 +263,8 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     q = _operand("q", q, cache, (B, H, 1, D))
     slots = 0
     if kv_idx is not None:
-        slots = kv_idx.shape[-1]
+        slots = kv_idx.shape[-1] if kv_idx.dim() == 3 else 0
+        assert slots >= 1, "kv_idx [B, Hk, k_slots] with at least one slot expected (counts of 0 list no page)"
         _check_ints("kv_idx", kv_idx, cache, (B, Hk, slots))
     if counts is not None:
         _check_ints("counts", counts, cache, (B, Hk))
