@@ -146,3 +146,41 @@ def test_decode_refuses_an_empty_list(monkeypatch):
         pc.paged_decode(q, cache, table, lens, 0.1, kv_idx=lists[..., :0])
     with pytest.raises(RuntimeError, match="launched"):
         pc.paged_decode(q, cache, table, lens, 0.1, kv_idx=lists[..., :1].contiguous())
+
+
+def calls(cache, q, k, v, out=None, pair=None):
+    """Each operator once on the tensors given."""
+    table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    return {"decode": lambda: pc.paged_decode(q, cache, table, lens, 0.1, out=out),
+            "select": lambda: pc.paged_select(q, cache, table, lens, 0.1, 3, 4),
+            "write": lambda: pc.paged_write(cache, k, v, table, lens),
+            "read": lambda: pc.paged_read(cache, table, lens, 5, out=pair)}
+
+
+def no_launch(monkeypatch):
+    monkeypatch.setattr(pc, "_launch", lambda *a: None)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_tangents_and_traces_are_refused(monkeypatch):
+    """A dual tensor requires no gradient and points at its primal: its tangent would be dropped."""
+    no_launch(monkeypatch)
+    fw = torch.autograd.forward_ad
+    q, k = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16), torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    out, pair = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16), [torch.zeros(1, 2, 5, 64, dtype=torch.bfloat16) for _ in "kv"]
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+        for name, args in (("decode", (dual(q), k, k)), ("select", (dual(q), k, k)), ("write", (q, dual(k), k)),
+                           ("write", (q, k, dual(k))), ("decode", (q, k, k, dual(out))),
+                           ("read", (q, k, k, None, (pair[0], dual(pair[1]))))):
+            with pytest.raises(AssertionError, match="forward-mode"):
+                calls(host_cache(), *args)[name]()
+        for call in calls(host_cache(), q, k, k, out, pair).values():        # no tangent in reach
+            call()
+    for name in ("decode", "select", "write", "read"):
+        def traced(x, name=name):
+            calls(host_cache(), q + x, k + x, k + x)[name]()
+            return x
+        with pytest.raises(AssertionError, match="traced"):
+            torch.jit.trace(traced, torch.zeros(1, dtype=torch.bfloat16), check_trace=False)

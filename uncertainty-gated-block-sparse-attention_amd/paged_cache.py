@@ -19,8 +19,8 @@ them on the host, and every call is asynchronous on the current stream and can b
 graph.  Lengths outside [0, 64 * max_pages] are taken as the nearer end; table entries outside the
 cache name absent pages, which are never written, read as zeros and take no part in attention.
 
-The operators have no backward pass: tensors that require gradients are refused where gradients
-are recorded.
+The operators have no derivatives: tensors that require gradients are refused where gradients are
+recorded, and so are tensors with a forward-mode tangent and calls that are being traced.
 """
 
 from __future__ import annotations
@@ -29,6 +29,7 @@ import ctypes
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd import forward_ad
 
 import _capi
 
@@ -100,6 +101,7 @@ class PagedCache:
         tensors = [t for t in (k, v, self.k_scale, self.v_scale, planes) if t is not None]
         assert all(t.is_cuda and t.device == tensors[0].device for t in tensors), "HIP tensors of one device required"
         assert not any(t.requires_grad or t.is_neg() for t in tensors), "plain tensors without gradients required"
+        _check_unwatched(*tensors)
         object.__setattr__(self, "_struct", s)
         object.__setattr__(self, "device", tensors[0].device)
         object.__setattr__(self, "_call", (ctypes.addressof(s), tensors[0].get_device(), s.Hk, s.D))
@@ -121,6 +123,15 @@ class PagedSelection:
     counts: torch.Tensor       # int32 [B, Hk] pages listed
     sigma: torch.Tensor        # fp32 [B, Hk] margin at the cut
     uncertain: torch.Tensor    # uint8 [B, Hk]
+
+
+def _check_unwatched(*tensors):
+    """Refuses what would lose or freeze values without an error: a tangent beside a tensor's data, a
+    trace that records the calls around a launch.  (Functional transforms have no data to point at.)"""
+    assert torch._C._get_tracing_state() is None, "the paged operators cannot be traced"
+    if forward_ad._current_level >= 0:
+        assert all(forward_ad.unpack_dual(t).tangent is None for t in tensors if t.is_floating_point()), \
+            "the paged operators have no forward-mode derivative"
 
 
 def _operand(name, t, cache, shape):
@@ -187,6 +198,7 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
     shape = (k.shape[0], *cache._call[2:])
     k = _operand("k", k, cache, shape)
     v = _operand("v", v, cache, shape)
+    _check_unwatched(k, v)
     if cu_new is not None:
         _check_ints("cu_new", cu_new, cache, (B + 1,))
     _launch(cache, "paged_write", _capi.lib().ugbsa_paged_write, k.data_ptr(), *k.stride(),
@@ -201,6 +213,7 @@ def paged_read(cache, block_table, seq_lens, n, out=None):
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
     _, index, Hk, D = cache._call
     shape = (B, Hk, n, D)
+    _check_unwatched(*out or ())
     if out is None:
         k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
     else:
@@ -230,6 +243,7 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
     _, _, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
     q = _operand("q", q, cache, (B, H, 1, D))
+    _check_unwatched(q)
     device = cache.device
     kv_idx = torch.empty((B, Hk, max(k_slots, 0)), dtype=torch.int32, device=device)
     counts = torch.empty((B, Hk), dtype=torch.int32, device=device)
@@ -261,6 +275,7 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     _, index, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
     q = _operand("q", q, cache, (B, H, 1, D))
+    _check_unwatched(q) if out is None else _check_unwatched(q, out)
     slots = 0
     if kv_idx is not None:
         slots = kv_idx.shape[-1] if kv_idx.dim() == 3 else 0
