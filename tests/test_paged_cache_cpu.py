@@ -161,7 +161,7 @@ def no_launch(monkeypatch):
     monkeypatch.setattr(pc, "_launch", lambda *a: None)
 
 
-@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.filterwarnings("ignore")
 def test_tangents_and_traces_are_refused(monkeypatch):
     """A dual tensor requires no gradient and points at its primal: its tangent would be dropped."""
     no_launch(monkeypatch)
@@ -184,3 +184,24 @@ def test_tangents_and_traces_are_refused(monkeypatch):
             return x
         with pytest.raises(AssertionError, match="traced"):
             torch.jit.trace(traced, torch.zeros(1, dtype=torch.bfloat16), check_trace=False)
+
+
+def test_outputs_that_do_not_hold_what_is_stored_are_refused(monkeypatch):
+    """Negated views, tensors that record gradients, elements that share memory, K and V in one place."""
+    no_launch(monkeypatch)
+    bf = torch.bfloat16
+    q, k = torch.zeros(1, 4, 1, 64, dtype=bf), torch.zeros(1, 2, 64, dtype=bf)
+    for bad in (torch._neg_view(torch.zeros(1, 1, 4, 64, dtype=bf)), torch.zeros(1, 1, 4, 64, dtype=bf, requires_grad=True),
+                torch.zeros(1, 1, 1, 64, dtype=bf).expand(1, 1, 4, 64), torch.zeros(1, 1, 4, 128, dtype=bf)):
+        with pytest.raises(AssertionError, match="out"):
+            calls(host_cache(), q, k, k, out=bad)["decode"]()
+    good = torch.zeros(1, 2, 5, 64, dtype=bf)
+    for bad in (torch._neg_view(good.clone()), good.clone().requires_grad_(),
+                torch.zeros(1, 1, 5, 64, dtype=bf).expand(1, 2, 5, 64), good):
+        for pair in ((good, bad), (bad, good)):
+            with pytest.raises(AssertionError, match="out"):
+                calls(host_cache(), q, k, k, pair=pair)["read"]()
+    with torch.no_grad():                                  # as for any in-place write
+        calls(host_cache(), q, k, k, out=torch.zeros(1, 1, 4, 64, dtype=bf, requires_grad=True))["decode"]()
+    calls(host_cache(), q, k, k, out=torch.zeros(4, 1, 1, 64, dtype=bf).transpose(0, 2))["decode"]()
+    calls(host_cache(), q, k, k, pair=(good, torch.zeros(2, 1, 5, 64, dtype=bf).transpose(0, 1)))["read"]()

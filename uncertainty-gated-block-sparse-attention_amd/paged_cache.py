@@ -152,6 +152,16 @@ def _operand(name, t, cache, shape):
     return t
 
 
+def _check_out(t, cache, shape):
+    """A result tensor that the kernels fill in place: what is stored is what the tensor holds, and each
+    element has a place of its own."""
+    assert t.shape == shape and t.dtype is cache.dtype and t.get_device() == cache._call[1], \
+        f"out: {list(shape)} in {cache.dtype} on the cache's device expected"
+    assert not t.is_neg() and not (t.requires_grad and torch.is_grad_enabled()), \
+        "out: a plain tensor without gradients required"
+    assert not any(s == 0 and n > 1 for s, n in zip(t.stride(), shape)), "out: elements share memory"
+
+
 def _check_ints(name, t, cache, shape):
     assert t.dtype is torch.int32 and t.shape == shape and t.is_contiguous() \
         and t.get_device() == cache._call[1], \
@@ -211,16 +221,16 @@ def paged_read(cache, block_table, seq_lens, n, out=None):
     past its length (``out``: a pair of such tensors to fill)."""
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
-    _, index, Hk, D = cache._call
+    _, _, Hk, D = cache._call
     shape = (B, Hk, n, D)
     _check_unwatched(*out or ())
     if out is None:
         k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
     else:
         k, v = out
-        for t in out:
-            assert t.shape == shape and t.dtype is cache.dtype and t.get_device() == index, \
-                f"out: a pair of {list(shape)} in {cache.dtype} expected"
+        _check_out(k, cache, shape)
+        _check_out(v, cache, shape)
+        assert k.data_ptr() != v.data_ptr(), "out: k and v are the same memory"
     _launch(cache, "paged_read", _capi.lib().ugbsa_paged_read, seq_lens.data_ptr(), block_table.data_ptr(),
             st_b, B, max_pages, n, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride())
     return k, v
@@ -272,7 +282,7 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
-    _, index, Hk, D = cache._call
+    _, _, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
     q = _operand("q", q, cache, (B, H, 1, D))
     _check_unwatched(q) if out is None else _check_unwatched(q, out)
@@ -286,8 +296,7 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     if out is None:
         out = torch.empty((B, 1, H, D), dtype=cache.dtype, device=cache.device)
     else:
-        assert out.shape == (B, 1, H, D) and out.dtype is cache.dtype and out.get_device() == index, \
-            f"out: {[B, 1, H, D]} in {cache.dtype} expected"
+        _check_out(out, cache, (B, 1, H, D))
     so_b, _, so_h, so_d = out.stride()
     lib = _capi.lib()
     n = lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
