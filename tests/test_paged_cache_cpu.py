@@ -205,3 +205,23 @@ def test_outputs_that_do_not_hold_what_is_stored_are_refused(monkeypatch):
         calls(host_cache(), q, k, k, out=torch.zeros(1, 1, 4, 64, dtype=bf, requires_grad=True))["decode"]()
     calls(host_cache(), q, k, k, out=torch.zeros(4, 1, 1, 64, dtype=bf).transpose(0, 2))["decode"]()
     calls(host_cache(), q, k, k, pair=(good, torch.zeros(2, 1, 5, 64, dtype=bf).transpose(0, 1)))["read"]()
+
+
+def test_operands_that_cannot_be_read_in_place_are_copied():
+    """Also those that count as contiguous: at an odd address, or with an odd stride of a dimension of
+    one element (the query or the one new token of a batch of one, cut out of a wider projection)."""
+    bf, cache = torch.bfloat16, host_cache()
+    flat = torch.arange(4096, dtype=torch.float32).to(bf)
+    views = [flat[4:4 + 256].view(1, 4, 1, 64),                               # 8 bytes past a boundary
+             flat[:258 * 2].view(2, 258)[:1, :256].view(1, 1, 4, 64).transpose(1, 2)[:1],
+             flat[:257].view(1, 257)[:, :256].view(1, 4, 1, 64),              # batch stride 257
+             flat[:4 * 65].view(1, 4, 1, 65)[..., :64], flat[:256].view(1, 64, 1, 4).transpose(1, 3)]
+    for v in views:
+        t = pc._operand("q", v, cache, (1, 4, 1, 64))
+        assert torch.equal(t, v) and t.data_ptr() % 16 == 0 and t.stride(-1) == 1
+        assert not any(s % 8 for s in t.stride()[:-1]), v.stride()
+    k = flat[:131].view(1, 131)[:, :128].view(1, 2, 64)
+    t = pc._operand("k", k, cache, (1, 2, 64))
+    assert torch.equal(t, k) and not any(s % 8 for s in t.stride()[:-1])
+    same = flat[:256].view(1, 4, 1, 64)
+    assert pc._operand("q", same, cache, (1, 4, 1, 64)) is same

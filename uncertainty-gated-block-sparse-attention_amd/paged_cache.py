@@ -148,7 +148,9 @@ def _operand(name, t, cache, shape):
     if t.is_neg():
         t = t.resolve_neg()
     if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
-        t = t.contiguous()
+        # not contiguous(): that is the tensor itself where only the address or the stride of a
+        # dimension of one element is in the way
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
