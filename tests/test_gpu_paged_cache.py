@@ -870,3 +870,19 @@ def test_select_bounds_of_different_magnitude(hip_lib, D, heads):
     table = torch.arange(nb, device=DEV, dtype=torch.int32).view(1, nb)
     for k_base, k_slots, tau in ((6, 12, 0.02), (20, 30, 0.0)):
         check_cut(q, cache, table, [64 * nb], 0.125, k_base, k_slots, tau)
+
+
+def test_pages_that_share_memory_are_read_only(hip_lib):
+    """Expanded pages, or one tensor for K and V: attended to and read back, not written."""
+    g = gen(24)
+    full = filled(g, 3, 2, 64, BF, False)
+    table, seq = i32([[2, 0]]), i32([100])
+    q, k1 = torch.randn(1, 4, 1, 64, generator=g, device=DEV).to(BF), torch.zeros(1, 2, 64, device=DEV, dtype=BF)
+    for k, v in ((full.k_pages[:, :1].expand(3, 2, 64, 64), full.v_pages), (full.k_pages, full.k_pages)):
+        shared, own = pc.PagedCache(k, v), pc.PagedCache(k.contiguous(), v.clone())
+        assert torch.equal(pc.paged_decode(q, shared, table, seq, 0.1), pc.paged_decode(q, own, table, seq, 0.1))
+        for a, b in zip(pc.paged_read(shared, table, seq, 100), pc.paged_read(own, table, seq, 100)):
+            assert torch.equal(a, b)
+        with pytest.raises(AssertionError, match="share memory"):
+            pc.paged_write(shared, k1, k1, table, seq)
+        pc.paged_write(own, k1, k1, table, seq)

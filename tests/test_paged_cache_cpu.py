@@ -127,7 +127,7 @@ def host_cache(dtype=torch.bfloat16, Hk=2, D=64, P=3):
     """What the calls look at of a cache; pages that no call gets as far as reading."""
     pages = torch.zeros(P, Hk, 64, D, dtype=dtype)
     return SimpleNamespace(dtype=dtype, device=torch.device("cpu"), k_pages=pages, v_pages=pages.clone(),
-                           planes=torch.zeros(P, Hk, 2, D, dtype=dtype), _call=(None, -1, Hk, D),
+                           planes=torch.zeros(P, Hk, 2, D, dtype=dtype), _call=(None, -1, Hk, D), _writable=True,
                            _struct=SimpleNamespace(cache_dtype=_capi.CACHE_MODEL))
 
 

@@ -42,7 +42,8 @@ class PagedCache:
     they are written in place, never resized or pointed elsewhere.
 
     k_pages, v_pages : [P, Hk, 64, D] in ``dtype`` or ``torch.float8_e4m3fn`` (unit stride on
-    head_dim, 16-byte aligned rows, any other strides)
+    head_dim, 16-byte aligned rows, any other strides; expanded pages, or one tensor for both, can
+    be read but not written)
     k_scale, v_scale : [P, Hk, 64] uint8 contiguous, for e4m3 pages: a value is code * 2^(byte - 127)
     planes : [P, Hk, 2, D] in ``dtype``, contiguous: K-max and K-min of each page.  Optional where
     nothing is selected; a cache of planes alone (no pages) serves ``paged_select`` only.
@@ -58,6 +59,7 @@ class PagedCache:
     device: torch.device = field(init=False, default=None)
     _struct: _capi.PagedCacheStruct = field(init=False, repr=False, compare=False, default=None)
     _call: tuple = field(init=False, repr=False, compare=False, default=None)   # address, device, Hk, D
+    _writable: bool = field(init=False, repr=False, compare=False, default=False)
 
     def __post_init__(self):
         k, v, planes = self.k_pages, self.v_pages, self.planes
@@ -102,6 +104,8 @@ class PagedCache:
         assert all(t.is_cuda and t.device == tensors[0].device for t in tensors), "HIP tensors of one device required"
         assert not any(t.requires_grad or t.is_neg() for t in tensors), "plain tensors without gradients required"
         _check_unwatched(*tensors)
+        object.__setattr__(self, "_writable", k is not None and k.data_ptr() != v.data_ptr() and not any(
+            st == 0 and n > 1 for t in (k, v) for st, n in zip(t.stride(), t.shape)))
         object.__setattr__(self, "_struct", s)
         object.__setattr__(self, "device", tensors[0].device)
         object.__setattr__(self, "_call", (ctypes.addressof(s), tensors[0].get_device(), s.Hk, s.D))
@@ -206,6 +210,7 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
     pages, but not ones that both write to.
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
+    assert cache._writable, "pages whose elements share memory cannot be written"
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
     shape = (k.shape[0], *cache._call[2:])
     k = _operand("k", k, cache, shape)
