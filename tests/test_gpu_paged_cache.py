@@ -886,3 +886,102 @@ def test_pages_that_share_memory_are_read_only(hip_lib):
         with pytest.raises(AssertionError, match="share memory"):
             pc.paged_write(shared, k1, k1, table, seq)
         pc.paged_write(own, k1, k1, table, seq)
+
+
+# ---- branches that take large calls ---------------------------------------------------------------
+
+# The pages that a table's width admits are more than 768 MB: they are read past the cache.
+@pytest.mark.parametrize("H,Hk,D,dtype,e4m3", [(6, 2, 64, BF, False), (6, 2, 64, FH, True), (28, 4, 128, BF, False),
+                                               (8, 2, 128, FH, True), (8, 2, 128, FH, False), (16, 2, 256, BF, True),
+                                               (8, 2, 128, BF, True), (16, 2, 256, FH, False), (6, 2, 64, FH, False),
+                                               (6, 2, 64, BF, True), (16, 2, 256, BF, False), (16, 2, 256, FH, True)])
+def test_decode_of_tables_wide_enough_to_stream(hip_lib, H, Hk, D, dtype, e4m3):
+    print(f"[case] streamed decode H={H}/{Hk} D={D} {dtype} {e4m3}", flush=True)
+    g = gen(D + H)
+    lens = [1500, 0, 700]
+    width = (768 << 20) // (len(lens) * Hk * 2 * 64 * D * (1 if e4m3 else 2)) + 1
+    table, P = tables(lens, g, width=width)
+    cache = filled(g, P, Hk, D, dtype, e4m3)
+    q = torch.randn(len(lens), H, 1, D, generator=g, device=DEV).to(dtype)
+    check_decode(q, cache, table, lens, D ** -0.5)
+
+
+# An output of 256 MiB or more is written past the cache, and its pages read past it.
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_read_of_lengths_long_enough_to_stream(hip_lib, D, dtype, e4m3):
+    g = gen(D)
+    lens, Hk = [1000, 64, 0, 333], 4
+    table, P = tables(lens, g)
+    cache = filled(g, P, Hk, D, dtype, e4m3)
+    n = (256 << 20) // (4 * len(lens) * Hk * D) + 3
+    near = pc.paged_read(cache, table, i32(lens), 1000)
+    for a, b in zip(pc.paged_read(cache, table, i32(lens), n), near):
+        assert torch.equal(a[:, :, :1000], b) and not a[:, :, 1000:].any()
+
+
+@pytest.mark.parametrize("nb", [1024, 1025, 1500, 2048, 2049, 3000, 4096, 4097])
+def test_select_at_the_sizes_of_the_pick(hip_lib, nb):
+    """Rows of 128, 256 and 512 threads with keys in registers, and of more."""
+    g = gen(nb)
+    cache = filled(g, nb, 2, 64, BF, False)
+    table = torch.stack([torch.randperm(nb, generator=g, device=DEV) for _ in range(2)]).int()
+    q = torch.randn(2, 8, 1, 64, generator=g, device=DEV).to(BF)
+    for k_base, k_slots, tau in ((64, 128, 0.005), (256, 300, 0.0), (3, 9, 9.0), (nb - 1, nb, 1e-4)):
+        check_cut(q, cache, table, [64 * nb - 7, 64 * (nb // 2)], 0.125, k_base, k_slots, tau)
+
+
+# ---- lengths that go back -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_planes_after_a_shorter_length(hip_lib, e4m3):
+    """Tokens taken back and others written in their place: the planes bound the keys that were given
+    for every token that is left, and a page that starts again at slot 0 forgets the old ones."""
+    g = gen(25)
+    cache = filled(g, 5, 2, 128, BF, e4m3)
+    table = i32([[3, 0, 4]])
+    keys = 4 * torch.randn(190, 2, 128, generator=g, device=DEV).to(BF)
+    pc.paged_write(cache, keys, keys, table, i32([0]), cu_new=i32([0, 190]))
+    for back, n in ((100, 20), (64, 1), (63, 90)):
+        new = torch.randn(n, 2, 128, generator=g, device=DEV).to(BF)
+        keys = torch.cat([keys[:back], new])
+        pc.paged_write(cache, new, new, table, i32([back]), cu_new=i32([0, n]))
+        for j in range((len(keys) + 63) // 64):
+            page, held = int(table[0, j]), keys[64 * j:64 * j + 64]
+            assert (cache.planes[page, :, 0] >= held.amax(0)).all() and (cache.planes[page, :, 1] <= held.amin(0)).all()
+            if 64 * j >= back:
+                assert torch.equal(cache.planes[page, :, 0], held.amax(0))
+                assert torch.equal(cache.planes[page, :, 1], held.amin(0))
+
+
+def test_contiguous_decode_over_what_is_read_back(hip_lib):
+    """The cache read back is the dispatcher's layout: its decode attends to it as the paged one does."""
+    g = gen(26)
+    table, P = tables([777], g)
+    for e4m3 in (False, True):
+        cache = filled(g, P, 2, 128, BF, e4m3)
+        q = torch.randn(1, 8, 1, 128, generator=g, device=DEV).to(BF)
+        k, v = pc.paged_read(cache, table, i32([777]), 777)
+        ref, mass = decode_ref(q, cache, table, [777], 0.09)
+        out, _ = sa.block_sparse_attention(None, q, k, v, None, 0.09)
+        check_close(out, ref, mass, BF)
+        check_close(pc.paged_decode(q, cache, table, i32([777]), 0.09), ref, mass, BF)
+
+
+def test_calls_repeat_themselves(hip_lib):
+    """The same call gives the same bits: no result depends on the order in which workgroups end."""
+    g = gen(27)
+    lens = [3000, 1, 0, 9000, 640, 70] * 9
+    table, P = tables(lens, g)
+    for dtype, e4m3 in ((BF, False), (FH, True)):
+        cache = filled(g, P, 2, 128, dtype, e4m3)
+        q = torch.randn(len(lens), 8, 1, 128, generator=g, device=DEV).to(dtype)
+        first = pc.paged_decode(q, cache, table, i32(lens), 0.09)
+        sel = pc.paged_select(q, cache, table, i32(lens), 0.09, 8, 16, tau=0.1)
+        part = pc.paged_decode(q, cache, table, i32(lens), 0.09, sel.kv_idx, sel.counts)
+        for _ in range(5):
+            assert torch.equal(first, pc.paged_decode(q, cache, table, i32(lens), 0.09))
+            again = pc.paged_select(q, cache, table, i32(lens), 0.09, 8, 16, tau=0.1)
+            assert torch.equal(sel.kv_idx, again.kv_idx) and torch.equal(sel.sigma, again.sigma)
+            assert torch.equal(part, pc.paged_decode(q, cache, table, i32(lens), 0.09, sel.kv_idx, sel.counts))
