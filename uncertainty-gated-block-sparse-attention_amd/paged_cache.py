@@ -35,6 +35,8 @@ import _capi
 
 PAGE = 64    # tokens per page: the selection block
 
+_tracing_state = torch._C._get_tracing_state
+
 
 @dataclass(frozen=True, eq=False)
 class PagedCache:
@@ -132,10 +134,16 @@ class PagedSelection:
 def _check_unwatched(*tensors):
     """Refuses what would lose or freeze values without an error: a tangent beside a tensor's data, a
     trace that records the calls around a launch.  (Functional transforms have no data to point at.)"""
-    assert torch._C._get_tracing_state() is None, "the paged operators cannot be traced"
+    assert _tracing_state() is None, "the paged operators cannot be traced"
     if forward_ad._current_level >= 0:
-        assert all(forward_ad.unpack_dual(t).tangent is None for t in tensors if t.is_floating_point()), \
+        assert all(forward_ad.unpack_dual(t).tangent is None for t in tensors
+                   if t is not None and t.is_floating_point()), \
             "the paged operators have no forward-mode derivative"
+
+
+def _watched():
+    """Whether a call has to look closer: next to nothing of its time otherwise."""
+    return forward_ad._current_level >= 0 or _tracing_state() is not None
 
 
 def _operand(name, t, cache, shape):
@@ -215,7 +223,8 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
     shape = (k.shape[0], *cache._call[2:])
     k = _operand("k", k, cache, shape)
     v = _operand("v", v, cache, shape)
-    _check_unwatched(k, v)
+    if _watched():
+        _check_unwatched(k, v)
     if cu_new is not None:
         _check_ints("cu_new", cu_new, cache, (B + 1,))
     _launch(cache, "paged_write", _capi.lib().ugbsa_paged_write, k.data_ptr(), *k.stride(),
@@ -230,7 +239,8 @@ def paged_read(cache, block_table, seq_lens, n, out=None):
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
     _, _, Hk, D = cache._call
     shape = (B, Hk, n, D)
-    _check_unwatched(*out or ())
+    if _watched():
+        _check_unwatched(*out or ())
     if out is None:
         k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
     else:
@@ -260,7 +270,8 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
     _, _, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
     q = _operand("q", q, cache, (B, H, 1, D))
-    _check_unwatched(q)
+    if _watched():
+        _check_unwatched(q)
     device = cache.device
     kv_idx = torch.empty((B, Hk, max(k_slots, 0)), dtype=torch.int32, device=device)
     counts = torch.empty((B, Hk), dtype=torch.int32, device=device)
@@ -292,7 +303,8 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     _, _, Hk, D = cache._call
     H = q.shape[1] if q.dim() == 4 else 0
     q = _operand("q", q, cache, (B, H, 1, D))
-    _check_unwatched(q) if out is None else _check_unwatched(q, out)
+    if _watched():
+        _check_unwatched(q, out)
     slots = 0
     if kv_idx is not None:
         slots = kv_idx.shape[-1] if kv_idx.dim() == 3 else 0
