@@ -339,8 +339,9 @@ typedef struct {
  * values that would read back infinite are held at the largest that does not,
  * NaN stays NaN.  planes: K-max and K-min of a page start over with its slot 0
  * and otherwise take the new keys in (from k as given, before any rounding; NaN
- * is passed over).  A page must not be named by two of the sequences that write
- * to it. */
+ * is passed over; what an e4m3 page holds may lie past them by half a step, 1/16
+ * of its magnitude or 2^-10 of the scale).  No page that the call writes to may be named twice by the table
+ * entries it writes through, and its elements may not share memory. */
 int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
                       int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
                       const int32_t* cu_new, const int32_t* lens, const int32_t* table,
@@ -348,7 +349,8 @@ int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_
 
 /* Cached tokens back: k_out, v_out [B, Hk, N, D] of dtype (the prefill entry
  * points' layout), row n of sequence b its token n, zeros from lens[b] on.
- * Exact: e4m3 values are values of dtype.  N <= 2^29. */
+ * Exact for what ugbsa_paged_write stored: its e4m3 values are values of dtype.
+ * N <= 2^29. */
 int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const int32_t* table,
                      int64_t st_b, int B, int max_pages, int N, void* k_out, int64_t sk_b,
                      int64_t sk_h, int64_t sk_n, int64_t sk_d, void* v_out, int64_t sv_b,
@@ -368,7 +370,8 @@ int64_t ugbsa_paged_select_workspace_elems(int B, int Hk, int max_pages);
  * k_base - 2; 2 where no page is cut.  Out: kv_idx [B, Hk, k_slots] int32, page
  * numbers within the sequence, ascending, then max_pages; counts [B, Hk] int32;
  * sigma [B, Hk] fp32 and uncertain [B, Hk] uint8 (either may be NULL).
- * A NaN score ranks first and makes sigma NaN, which is not below tau.  3 <=
+ * A NaN score ranks first; sigma is NaN, which is not below tau, where one of its
+ * scores is NaN or infinities leave it undefined.  3 <=
  * k_base <= k_slots; scaling positive and finite; B * Hk < 2^23, B * Hk *
  * max_pages <= 2^29; workspace 8-byte aligned. */
 int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
@@ -389,7 +392,8 @@ int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int unit
  * not be listed twice.  q [B, H, 1, D], out [B, H, D] of dtype with
  * even strides (4-byte aligned rows); B, H <= 65535, B * H * max_pages (or k_slots)
  * at most 2^30.  A row without a key, or whose every weight is 0, gives
- * zeros.  workspace (16-byte aligned) holds the pieces of rows that several
+ * zeros.  Statistics and sums are fp32; weights are rounded to dtype before the
+ * product with V.  workspace (16-byte aligned) holds the pieces of rows that several
  * workgroups share; its contents on entry do not matter. */
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
                        int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,

@@ -4,13 +4,15 @@
 //
 //   K, V    [P, Hk, 64, D] in the call's 16-bit format, or e4m3 bytes with a
 //           scale byte per token and head ([P, Hk, 64]): value = code * 2^(byte - 127)
-//   planes  [P, Hk, 2, D] in the 16-bit format: K-max and K-min of a page's keys,
-//           the Quest summary of kernel 1, one block a page
+//   planes  [P, Hk, 2, D] in the 16-bit format: K-max and K-min of a page's keys as
+//           they were given, the Quest summary of kernel 1, one block a page.  What an
+//           e4m3 page holds of them is rounded, and may lie past the planes by half a
+//           step: 1/16 of its magnitude, or 2^-10 of the token's scale if that is more
 //
 // Power-of-two scales keep every step exact but one: x 2^-e is exact, the
-// rounding to e4m3's four significant bits is the only one, and the value read
-// back is exact in bf16 and fp16 alike (four bits at an exponent the unquantised
-// value had).  A float format loses next to nothing by it: the scale only has to
+// rounding to e4m3's four significant bits is the only one, and what the write
+// stored reads back exactly in its format, bf16 or fp16 (four bits at an exponent the
+// unquantised value had).  A float format loses next to nothing by it: the scale only has to
 // place the token's largest magnitude in the top binade.
 //
 // Lengths and table entries are device data that the host cannot check.  A

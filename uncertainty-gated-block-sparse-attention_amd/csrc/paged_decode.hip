@@ -493,7 +493,16 @@ __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
 // join: where a row's K and V are at most 256 KB, which one CU streams (about 25 bytes a
 // clock) in what the joining launch costs.  us, this form / the line: 512 tokens, 28/4
 // heads, head_dim 128, bf16, 1 sequence 9.1 / 10.5, 128 sequences 15.9 / 22.3; 1024
-// tokens (512 KB) 13.3 / 10.8 and 23.6 / 26.8, in e4m3 10.8 / 11.0 and 19.1 / 23.3.
+// tokens in e4m3 (256 KB) 10.8 / 11.0 and 19.1 / 23.3, in bf16 (512 KB) 13.3 / 10.8 and
+// 23.6 / 26.8: past 256 KB one row is slower this way and many rows are faster.  The rule
+// goes by a row's bytes alone and takes the line there.
+//
+// The bytes are those that the table's width admits; the lengths are on the device.  24
+// sequences of 500 tokens, 40/8 heads, in a table of 8 / 256 / 2048 pages: bf16 12.5 / 21.3
+// / 21.2 us, e4m3 8.5 / 16.2 / 16.9.
+//
+// At head_dim 256 in 16 bits this form's instances spill 44 bytes a lane at the two
+// wavefronts per SIMD that they are bound to.
 static bool paged_decode_one(int D, bool e4m3, int units) {
   return static_cast<int64_t>(units) * (2 * kBlock * D * (e4m3 ? 1 : 2)) <= 256 << 10;
 }

@@ -15,7 +15,7 @@
 // large it is.
 //
 // 64 sequences of up to 128K tokens, 40/8 heads (119 MB of planes): scoring 49 us,
-// picking 11; one of 32K, 28/4 heads, 4.3 and 6.9.
+// picking 11.3; one of 32K, 28/4 heads, 4.3 and 7.0.
 #include "paged.h"
 
 namespace ugbsa {

@@ -3,7 +3,8 @@
 The dispatcher's decode attends to a contiguous ``[B, Hk, N, D]`` cache; a server keeps keys and
 values in pages of 64 tokens, the selection block, that a block table names.  Pages hold the
 model's dtype or e4m3 codes with a power-of-two scale per token and head, and beside them stands
-each page's Quest summary (K-max, K-min), kept up to date as tokens are written:
+each page's Quest summary (K-max, K-min of the keys as given, before e4m3 rounds them), kept up to
+date as tokens are written:
 
     cache = PagedCache.empty(num_pages, Hk, D, torch.bfloat16, "cuda", e4m3=True)
     paged_write(cache, k, v, block_table, seq_lens, cu_new=cu)     # prompts [T, Hk, D], packed
@@ -12,7 +13,7 @@ each page's Quest summary (K-max, K-min), kept up to date as tokens are written:
     seq_lens += 1
     sel = paged_select(q, cache, block_table, seq_lens, scale, k_base=64, k_slots=128, tau=0.01)
     out = paged_decode(q, cache, block_table, seq_lens, scale, sel.kv_idx, sel.counts)
-    k, v = paged_read(cache, block_table, seq_lens, N)             # [B, Hk, N, D] for a prefill
+    k, v = paged_read(cache, block_table, seq_lens, N)             # [B, Hk, N, D], contiguous
 
 ``block_table`` [B, max_pages] int32 and ``seq_lens`` [B] int32 live on the device: no call reads
 them on the host, and every call is asynchronous on the current stream and can be captured in a
@@ -210,12 +211,12 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
     """New tokens into the cache, quantised if it holds e4m3, and its page summaries.
 
     k, v : [T, Hk, D], the new tokens of all sequences, packed
-    cu_new : [B + 1] int32, sequence b's are rows cu_new[b] .. cu_new[b + 1] - 1; None: one token
-    each, row b
+    cu_new : [B + 1] int32, ascending: sequence b's are rows cu_new[b] .. cu_new[b + 1] - 1; None:
+    one token each, row b
     seq_lens : tokens cached before this call; the new ones follow them (the caller adds them up)
 
     Rows behind the last sequence and tokens past the table are left out.  Two sequences may share
-    pages, but not ones that both write to.
+    pages, but no page that a call writes to may be named twice by the entries it writes through.
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
     assert cache._writable, "pages whose elements share memory cannot be written"
@@ -233,14 +234,16 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
 
 
 def paged_read(cache, block_table, seq_lens, n, out=None):
-    """(k, v) [B, Hk, n, D] in ``cache.dtype``: the first n cached tokens of every sequence, zeros
-    past its length (``out``: a pair of such tensors to fill)."""
+    """(k, v) [B, Hk, n, D] in ``cache.dtype``: the first n >= 1 cached tokens of every sequence, zeros
+    past its length (``out``: a pair of such tensors to fill).  The layout of a contiguous cache, which
+    the dispatcher's decode attends to; its sparse prefills take as many queries as keys and so no
+    cached prefix."""
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
     _, _, Hk, D = cache._call
     shape = (B, Hk, n, D)
     if _watched():
-        _check_unwatched(*out or ())
+        _check_unwatched(*(() if out is None else out))
     if out is None:
         k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
     else:
@@ -259,7 +262,7 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
 
     q : [B, H, 1, D]; seq_lens counts the new token.  A page's score is the Quest bound of its
     summary, maximised over the KV head's query heads and summed in fp64.  The first and the last
-    page are kept, and the best others by (score desc, page asc) up to ``k_base`` pages, or
+    page are kept, and the best others by (score desc, page asc) up to ``k_base`` >= 3 pages, or
     ``k_slots`` where the margin at the cut, sigma = clamp((s(k) - s(k + 1)) / max(s(1) - s(k + 1),
     1e-9), 0, 2) over the scaled scores of the others, k = k_base - 2, is below ``tau``
     (``Selector.router_tau``'s role; 0 keeps k_base throughout).  A sequence's list depends on no
@@ -295,8 +298,9 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     that the KV head's query heads attend to; counts [B, Hk] int32: how many entries count (None:
     all).  Entries that are no page of the sequence are skipped.
     Returns [B, 1, H, D] contiguous, the dispatcher's layout (``out`` if given).  A sequence without
-    a key gives zeros.  The launch is shaped by the table's (or list's) width: pass a table cut to
-    the longest sequence where the batch is short.
+    a key gives zeros.  Weights are rounded to ``dtype`` before the product with V.  The launch is
+    shaped by the table's (or list's) width: pass a table cut to the longest sequence where the batch
+    is short.
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
