@@ -985,3 +985,18 @@ def test_calls_repeat_themselves(hip_lib):
             again = pc.paged_select(q, cache, table, i32(lens), 0.09, 8, 16, tau=0.1)
             assert torch.equal(sel.kv_idx, again.kv_idx) and torch.equal(sel.sigma, again.sigma)
             assert torch.equal(part, pc.paged_decode(q, cache, table, i32(lens), 0.09, sel.kv_idx, sel.counts))
+
+
+@pytest.mark.parametrize("heads", [1, 4, 5, 7, 8])
+def test_select_zeros_of_either_sign_take_the_upper_bound(hip_lib, heads):
+    """q = -0 is >= 0: its bound is K-max, which shows where one of the bounds is infinite."""
+    g = gen(heads)
+    nb = 30
+    cache = filled(g, nb, 2, 64, BF, False)
+    q = torch.randn(1, 2 * heads, 1, 64, generator=g, device=DEV).to(BF)
+    q[..., 7], q[..., 8] = -0.0, 0.0
+    cache.planes[3, 0, 0, 7] = cache.planes[4, 0, 0, 8] = INF                 # NaN scores
+    cache.planes[5, :, 1, 7] = cache.planes[6, :, 1, 8] = -INF                # not looked at
+    table = torch.arange(nb, device=DEV, dtype=torch.int32).view(1, nb)
+    check_cut(q, cache, table, [64 * nb], 0.125, 4, 8, 0.1)
+    check_cut(q, cache, table, [64 * nb], 0.125, 9, 12, 0.1)

@@ -15,7 +15,7 @@
 // large it is.
 //
 // 64 sequences of up to 128K tokens, 40/8 heads (119 MB of planes): scoring 49 us,
-// picking 11.3; one of 32K, 28/4 heads, 4.3 and 7.0.
+// picking 11.3; one of 32K, 28/4 heads, 4.0 and 6.5.
 #include "paged.h"
 
 namespace ugbsa {
@@ -129,13 +129,18 @@ __global__ __launch_bounds__(256) void paged_score_kernel(
         }
         const int ahead = j + kScoreAhead * NP;
         if (ahead < j1) load(ahead, his[s], los[s], pages[s]);
+        // Past five heads the selects' masks do not fit the SGPRs (and their spills cost 8
+        // sequences of up to 64K tokens 3 to 7 % of both launches): a 0 that the compiler does
+        // not know keeps the compares with the selects.
+        double zero = 0.0;
+        if constexpr (GC > 5) asm volatile("s_mov_b64 %0, 0" : "=s"(zero));
         double best = -INFINITY;
 #pragma unroll
         for (int h = 0; h < GC; ++h) {
           double acc = 0.0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const uint32_t w = qd[h][i] >= 0.0 ? top[i] : low[i];
+            const uint32_t w = qd[h][i] >= zero ? top[i] : low[i];
             acc = __builtin_fma(qd[h][i], __builtin_bit_cast(double, static_cast<uint64_t>(w) << 32), acc);
           }
           acc = group_sum<LP>(acc);
