@@ -302,6 +302,31 @@ int ugbsa_decode(const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_
                  int64_t so_h, int64_t so_d, float* workspace, int64_t workspace_elems,
                  void* stream);
 
+/* ---- rotary positions ------------------------------------------------------ */
+
+/* Pair j < rotary_dim / 2 of a head's dims turns by turns[j] times the position, in
+ * turns (the frequency over 2 pi, 64 bits, device data), and is multiplied by
+ * attention; pairs are (j, j + rotary_dim / 2) or, interleaved, (2 j, 2 j + 1).
+ * rotary_dim is even and at most head_dim; the other dims pass unchanged. */
+typedef struct {
+  const double* turns;
+  int rotary_dim, interleaved;
+  float attention;
+} ugbsa_rotary_table;
+
+/* q [B, H, M, D] and, unless Hk is 0, k [B, Hk, M, D] of dtype turned by positions
+ * [B, M] int32 (row stride sp_b, 0 where all rows share them; entries contiguous; any
+ * value) into q_out and k_out, computed in fp32 and rounded once.  inverse: by the
+ * opposite angle, which is the gradient's map.  An output may be its own input (same
+ * address and strides) and must not otherwise overlap an input.  B * M * (H + Hk)
+ * < 2^28; M = 0 does nothing. */
+int ugbsa_rotary(const ugbsa_rotary_table* table, const int32_t* positions, int64_t sp_b,
+                 const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_t sq_d, void* q_out,
+                 int64_t so_b, int64_t so_h, int64_t so_m, int64_t so_d, int H, const void* k,
+                 int64_t sk_b, int64_t sk_h, int64_t sk_m, int64_t sk_d, void* k_out, int64_t sl_b,
+                 int64_t sl_h, int64_t sl_m, int64_t sl_d, int Hk, int B, int M, int D, int dtype,
+                 int inverse, void* stream);
+
 /* ---- paged key-value cache ----------------------------------------------- */
 
 #define UGBSA_CACHE_MODEL 0 /* pages hold dtype */

@@ -90,8 +90,16 @@ SIGNATURES = {
     "ugbsa_paged_decode_workspace_elems": (_i64, [_i, _i, _i, _i, _i, _i]),
     "ugbsa_paged_decode": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _p,
                                 _p, _i, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "ugbsa_rotary": (_i, [_p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i,
+                          _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i,
+                          _i, _i, _p]),
 }
 ABI_VERSION = 4
+
+
+class RotaryStruct(ctypes.Structure):
+    """``ugbsa_rotary_table`` of the header."""
+    _fields_ = [("turns", _p), ("rotary_dim", _i), ("interleaved", _i), ("attention", _f)]
 
 
 class PagedCacheStruct(ctypes.Structure):

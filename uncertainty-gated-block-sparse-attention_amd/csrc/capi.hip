@@ -62,6 +62,17 @@ int64_t kv_copy_elems(int B, int Hk, int N, int D) {
   return 2 * static_cast<int64_t>(B) * Hk * nb * ugbsa::kBlock * D;
 }
 
+int rotary_table(const ugbsa_rotary_table* t, int D, ugbsa::RotaryTable* to) {
+  if (t == nullptr || t->turns == nullptr) return fail(UGBSA_EARG, "rotary table is null");
+  if (reinterpret_cast<uintptr_t>(t->turns) & 7) return fail(UGBSA_ELAYOUT, "turns must be 8-byte aligned");
+  if (t->rotary_dim < 2 || t->rotary_dim > D || t->rotary_dim % 2)
+    return fail(UGBSA_EARG, "rotary_dim must be even and lie in [2, head_dim] (%d, head_dim %d)", t->rotary_dim, D);
+  if (!(t->attention - t->attention == 0.f)) return fail(UGBSA_EARG, "attention factor must be finite");
+  to->turns = t->turns, to->pairs = t->rotary_dim / 2;
+  to->interleaved = t->interleaved != 0, to->attention = t->attention;
+  return UGBSA_OK;
+}
+
 // A paged cache whose pages the kernels can read, and the table that names them.
 int check_paged(const ugbsa_paged_cache* c, int H, const int32_t* lens, const int32_t* table,
                 int64_t st_b, int B, int max_pages) {
@@ -723,6 +734,35 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
                                                k_slots, scale, static_cast<uint16_t*>(out), so_b, so_h,
                                                workspace, static_cast<hipStream_t>(stream)),
                     "paged_decode");
+}
+
+int ugbsa_rotary(const ugbsa_rotary_table* table, const int32_t* positions, int64_t sp_b, const void* q,
+                 int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_t sq_d, void* q_out, int64_t so_b, int64_t so_h,
+                 int64_t so_m, int64_t so_d, int H, const void* k, int64_t sk_b, int64_t sk_h, int64_t sk_m,
+                 int64_t sk_d, void* k_out, int64_t sl_b, int64_t sl_h, int64_t sl_m, int64_t sl_d, int Hk, int B,
+                 int M, int D, int dtype, int inverse, void* stream) {
+  int rc = check_dims(B, H, 1, D, dtype);
+  ugbsa::RotaryTable t;
+  if (rc || (rc = rotary_table(table, D, &t))) return rc;
+  if (Hk < 0 || H > 65535 || Hk > 65535) return fail(UGBSA_EARG, "heads must be at most 65535 (H=%d, Hk=%d)", H, Hk);
+  if (M < 0 || static_cast<int64_t>(B) * M >= 1 << 28 || static_cast<int64_t>(B) * M * (H + Hk) >= 1 << 28)
+    return fail(UGBSA_EARG, "B * M * (H + Hk) must be below 2^28 (B=%d, M=%d)", B, M);
+  if (M == 0) return hip_result(hipSuccess, "rotary");
+  if (positions == nullptr || (reinterpret_cast<uintptr_t>(positions) & 3))
+    return fail(UGBSA_EARG, "positions is null or not 4-byte aligned");
+  if ((rc = check_bf16_operand("q", q, sq_b, sq_h, sq_m, sq_d))) return rc;
+  if ((rc = check_bf16_operand("q_out", q_out, so_b, so_h, so_m, so_d))) return rc;
+  if (Hk > 0 && (rc = check_bf16_operand("k", k, sk_b, sk_h, sk_m, sk_d))) return rc;
+  if (Hk > 0 && (rc = check_bf16_operand("k_out", k_out, sl_b, sl_h, sl_m, sl_d))) return rc;
+  const ugbsa::RotaryHeads hq{static_cast<const uint16_t*>(q), sq_b, sq_h, sq_m, static_cast<uint16_t*>(q_out),
+                              so_b, so_h, so_m, H};
+  ugbsa::RotaryHeads hk;
+  if (Hk > 0)
+    hk = ugbsa::RotaryHeads{static_cast<const uint16_t*>(k), sk_b, sk_h, sk_m, static_cast<uint16_t*>(k_out),
+                            sl_b, sl_h, sl_m, Hk};
+  return hip_result(ugbsa::launch_rotary(t, positions, sp_b, hq, hk, B, M, D, dtype, inverse != 0,
+                                         static_cast<hipStream_t>(stream)),
+                    "rotary");
 }
 
 }  // extern "C"

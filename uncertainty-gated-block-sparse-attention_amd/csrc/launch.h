@@ -158,6 +158,23 @@ hipError_t launch_decode(const uint16_t* q, int64_t sq_b, int64_t sq_h, const ui
                          float scale, uint16_t* out, int64_t so_b, int64_t so_h, float* ws,
                          hipStream_t stream);
 
+// Rotary positions (rotary.h).  turns: f_j / 2 pi of each pair; attention: what the
+// turned values are multiplied by; heads: 0 where there is no such tensor.
+struct RotaryTable {
+  const double* turns = nullptr;
+  int pairs = 0, interleaved = 0;
+  float attention = 1.f;
+};
+struct RotaryHeads {
+  const uint16_t* x = nullptr;
+  int64_t sx_b = 0, sx_h = 0, sx_m = 0;
+  uint16_t* y = nullptr;
+  int64_t sy_b = 0, sy_h = 0, sy_m = 0;
+  int heads = 0;
+};
+hipError_t launch_rotary(const RotaryTable& t, const int32_t* positions, int64_t sp_b, const RotaryHeads& q,
+                         const RotaryHeads& k, int B, int M, int D, int elem, bool inverse, hipStream_t stream);
+
 // The paged cache of a call (paged.h): element strides of K and V, the scales
 // and planes contiguous; elem as above, e4m3: K and V hold e4m3 bytes.
 struct PagedCache {
