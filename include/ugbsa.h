@@ -331,6 +331,7 @@ int ugbsa_rotary(const ugbsa_rotary_table* table, const int32_t* positions, int6
 
 #define UGBSA_CACHE_MODEL 0 /* pages hold dtype */
 #define UGBSA_CACHE_E4M3 1  /* pages hold e4m3 codes, scales a byte per token and head */
+#define UGBSA_CACHE_E2M1 2  /* pages hold e2m1 codes, scales a byte per 32 dims of a token's head */
 
 /* A cache of num_pages pages of 64 tokens (the key block), Hk heads of D.  A
  * block table [B, max_pages] int32 (row stride st_b, entries contiguous) names
@@ -341,13 +342,14 @@ int ugbsa_rotary(const ugbsa_rotary_table* table, const int32_t* positions, int6
  *    written to it, it reads as zeros, and its keys take no part.
  * Slots past a sequence's length may hold anything, NaN included. */
 typedef struct {
-  void* k_pages; /* [num_pages, Hk, 64, D] of dtype or e4m3, head_dim stride 1, */
-  void* v_pages; /* 16-byte aligned rows; the other strides in elements, at most 2^24 a
-                    slot, below 2^35 a page or head */
+  void* k_pages; /* [num_pages, Hk, 64, D] of dtype or e4m3, or [num_pages, Hk, 64, D / 2] */
+  void* v_pages; /* bytes of two e2m1 codes, the even dim in the low four bits; last stride
+                    1, 16-byte aligned rows; the other strides in elements (bytes of codes),
+                    at most 2^24 a slot, below 2^35 a page or head */
   int64_t sk_p, sk_h, sk_n;
   int64_t sv_p, sv_h, sv_n;
-  uint8_t* k_scale; /* [num_pages, Hk, 64] contiguous, e4m3 only: a value is */
-  uint8_t* v_scale; /* code * 2^(byte - 127) */
+  uint8_t* k_scale; /* e4m3 [num_pages, Hk, 64], e2m1 [num_pages, Hk, D / 32, 64], */
+  uint8_t* v_scale; /* contiguous: a value is code * 2^(byte - 127); e2m1: NaN for 255 */
   void* planes;     /* [num_pages, Hk, 2, D] of dtype, contiguous: K-max and K-min
                        of each page (16-byte aligned), or NULL */
   int num_pages, Hk, D;
@@ -362,19 +364,31 @@ typedef struct {
  * token's head is divided by the smallest power of two that brings its largest
  * finite magnitude to 448 or less and rounded to nearest even; infinities and
  * values that would read back infinite are held at the largest that does not,
- * NaN stays NaN.  planes: K-max and K-min of a page start over with its slot 0
+ * NaN stays NaN.  e2m1: the same for each 32 dims, with 6 (the format's largest) for
+ * 448; the 32 become NaN where one of them is.  planes: K-max and K-min of a page start over with its slot 0
  * and otherwise take the new keys in (from k as given, before any rounding; NaN
  * is passed over; what an e4m3 page holds may lie past them by half a step, 1/16
- * of its magnitude or 2^-10 of the scale).  No page that the call writes to may be named twice by the table
+ * of its magnitude or 2^-10 of the scale; e2m1 a quarter of its magnitude or of the
+ * scale).  No page that the call writes to may be named twice by the table
  * entries it writes through, and its elements may not share memory. */
 int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
                       int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
                       const int32_t* cu_new, const int32_t* lens, const int32_t* table,
                       int64_t st_b, int B, int T, int max_pages, void* stream);
 
+/* ugbsa_paged_write of keys that are turned by their positions first, as ugbsa_rotary
+ * turns them (bit for bit): positions [T] int32, or NULL: a token's place in its
+ * sequence, lens[b] on. */
+int ugbsa_paged_write_rotary(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t,
+                             int64_t sk_h, int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h,
+                             int64_t sv_d, const int32_t* cu_new, const int32_t* lens,
+                             const int32_t* table, int64_t st_b, int B, int T, int max_pages,
+                             const ugbsa_rotary_table* rotary, const int32_t* positions,
+                             void* stream);
+
 /* Cached tokens back: k_out, v_out [B, Hk, N, D] of dtype (the prefill entry
  * points' layout), row n of sequence b its token n, zeros from lens[b] on.
- * Exact for what ugbsa_paged_write stored: its e4m3 values are values of dtype.
+ * Exact for what ugbsa_paged_write stored: the values of its codes are values of dtype.
  * N <= 2^29. */
 int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const int32_t* table,
                      int64_t st_b, int B, int max_pages, int N, void* k_out, int64_t sk_b,
@@ -418,7 +432,7 @@ int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int unit
  * even strides (4-byte aligned rows); B, H <= 65535, B * H * max_pages (or k_slots)
  * at most 2^30.  A row without a key, or whose every weight is 0, gives
  * zeros.  Statistics and sums are fp32; weights are rounded to dtype before the
- * product with V.  workspace (16-byte aligned) holds the pieces of rows that several
+ * product with V.  Codes count as the values that ugbsa_paged_read gives.  workspace (16-byte aligned) holds the pieces of rows that several
  * workgroups share; its contents on entry do not matter. */
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
                        int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,

@@ -27,7 +27,7 @@ GRAIN_CELL, GRAIN_ROW = 0, 1
 ROUTER_ABS, ROUTER_QUANTILE = 0, 1
 V1_TOPK, V1_BELIEF = 0, 1
 DECODE_ONE_SPLIT = 512
-CACHE_MODEL, CACHE_E4M3 = 0, 1
+CACHE_MODEL, CACHE_E4M3, CACHE_E2M1 = 0, 1, 2
 
 # Every symbol include/ugbsa.h declares, with its ctypes signature.
 _i, _i64, _f, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -90,6 +90,8 @@ SIGNATURES = {
     "ugbsa_paged_decode_workspace_elems": (_i64, [_i, _i, _i, _i, _i, _i]),
     "ugbsa_paged_decode": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _p,
                                 _p, _i, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "ugbsa_paged_write_rotary": (_i, [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64,
+                                      _i, _i, _i, _p, _p, _p]),
     "ugbsa_rotary": (_i, [_p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i,
                           _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i,
                           _i, _i, _p]),

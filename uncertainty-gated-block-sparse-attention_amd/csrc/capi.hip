@@ -79,7 +79,8 @@ int check_paged(const ugbsa_paged_cache* c, int H, const int32_t* lens, const in
   if (c == nullptr) return fail(UGBSA_EARG, "cache is null");
   int rc = check_dims(B, H, c->Hk, c->D, c->dtype);
   if (rc) return rc;
-  if (c->cache_dtype != UGBSA_CACHE_MODEL && c->cache_dtype != UGBSA_CACHE_E4M3)
+  if (c->cache_dtype != UGBSA_CACHE_MODEL && c->cache_dtype != UGBSA_CACHE_E4M3 &&
+      c->cache_dtype != UGBSA_CACHE_E2M1)
     return fail(UGBSA_EDTYPE, "unknown cache dtype %d", c->cache_dtype);
   if (B > 65535 || H > 65535) return fail(UGBSA_EARG, "B and H must be at most 65535 (B=%d, H=%d)", B, H);
   if (c->num_pages < 1) return fail(UGBSA_EARG, "num_pages must be positive");
@@ -91,8 +92,8 @@ int check_paged(const ugbsa_paged_cache* c, int H, const int32_t* lens, const in
 }
 
 int check_pages(const ugbsa_paged_cache* c) {
-  const bool e4m3 = c->cache_dtype == UGBSA_CACHE_E4M3;
-  const int64_t unit = e4m3 ? 16 : 8;      // elements of a 16-byte load
+  const bool codes = c->cache_dtype != UGBSA_CACHE_MODEL;
+  const int64_t unit = codes ? 16 : 8;      // elements (bytes of codes) of a 16-byte load
   if (c->k_pages == nullptr || c->v_pages == nullptr) return fail(UGBSA_EARG, "k_pages or v_pages is null");
   if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || c->sk_p % unit || c->sk_h % unit ||
       c->sk_n % unit || c->sv_p % unit || c->sv_h % unit || c->sv_n % unit)
@@ -102,9 +103,9 @@ int check_pages(const ugbsa_paged_cache* c) {
     return fail(UGBSA_ELAYOUT, "the pages' slot strides must lie in [0, 2^24]");
   for (const int64_t s : {c->sk_p, c->sk_h, c->sv_p, c->sv_h})
     if (s < 0 || s >= int64_t{1} << 35) return fail(UGBSA_ELAYOUT, "the pages' strides must lie in [0, 2^35)");
-  if (e4m3 && (c->k_scale == nullptr || c->v_scale == nullptr))
-    return fail(UGBSA_EARG, "an e4m3 cache needs k_scale and v_scale");
-  if (e4m3 && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 7)
+  if (codes && (c->k_scale == nullptr || c->v_scale == nullptr))
+    return fail(UGBSA_EARG, "a quantised cache needs k_scale and v_scale");
+  if (codes && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 7)
     return fail(UGBSA_ELAYOUT, "scales must be 8-byte aligned");
   if (!aligned16(c->planes)) return fail(UGBSA_ELAYOUT, "planes must be 16-byte aligned");
   return UGBSA_OK;
@@ -118,7 +119,7 @@ ugbsa::PagedCache paged_cache(const ugbsa_paged_cache* c) {
   p.k_scale = c->k_scale, p.v_scale = c->v_scale;
   p.planes = static_cast<uint16_t*>(c->planes);
   p.num_pages = c->num_pages, p.Hk = c->Hk, p.D = c->D, p.elem = c->dtype;
-  p.e4m3 = c->cache_dtype == UGBSA_CACHE_E4M3;
+  p.kind = c->cache_dtype;
   return p;
 }
 
@@ -625,10 +626,11 @@ int ugbsa_decode(const void* q, int64_t sq_b, int64_t sq_h, int64_t sq_m, int64_
                     "decode");
 }
 
-int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
-                      int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
-                      const int32_t* cu_new, const int32_t* lens, const int32_t* table,
-                      int64_t st_b, int B, int T, int max_pages, void* stream) {
+static int paged_write_impl(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
+                            int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
+                            const int32_t* cu_new, const int32_t* lens, const int32_t* table,
+                            int64_t st_b, int B, int T, int max_pages, const ugbsa::RotaryTable* rot,
+                            const int32_t* positions, void* stream) {
   int rc = check_paged(cache, cache ? cache->Hk : 1, lens, table, st_b, B, max_pages);
   if (rc || (rc = check_pages(cache))) return rc;
   if (T < 0 || (cu_new == nullptr && T < B))
@@ -641,8 +643,30 @@ int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_
   return hip_result(ugbsa::launch_paged_write(paged_cache(cache), static_cast<const uint16_t*>(k), sk_t,
                                               sk_h, static_cast<const uint16_t*>(v), sv_t, sv_h, cu_new,
                                               lens, table, st_b, B, T, max_pages,
-                                              static_cast<hipStream_t>(stream)),
+                                              static_cast<hipStream_t>(stream), rot, positions),
                     "paged_write");
+}
+
+int ugbsa_paged_write(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
+                      int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
+                      const int32_t* cu_new, const int32_t* lens, const int32_t* table,
+                      int64_t st_b, int B, int T, int max_pages, void* stream) {
+  return paged_write_impl(cache, k, sk_t, sk_h, sk_d, v, sv_t, sv_h, sv_d, cu_new, lens, table, st_b, B, T,
+                          max_pages, nullptr, nullptr, stream);
+}
+
+int ugbsa_paged_write_rotary(const ugbsa_paged_cache* cache, const void* k, int64_t sk_t, int64_t sk_h,
+                             int64_t sk_d, const void* v, int64_t sv_t, int64_t sv_h, int64_t sv_d,
+                             const int32_t* cu_new, const int32_t* lens, const int32_t* table,
+                             int64_t st_b, int B, int T, int max_pages, const ugbsa_rotary_table* rotary,
+                             const int32_t* positions, void* stream) {
+  ugbsa::RotaryTable t;
+  if (cache == nullptr) return fail(UGBSA_EARG, "cache is null");
+  const int rc = rotary_table(rotary, cache->D, &t);
+  if (rc) return rc;
+  if (reinterpret_cast<uintptr_t>(positions) & 3) return fail(UGBSA_ELAYOUT, "positions must be 4-byte aligned");
+  return paged_write_impl(cache, k, sk_t, sk_h, sk_d, v, sv_t, sv_h, sv_d, cu_new, lens, table, st_b, B, T,
+                          max_pages, &t, positions, stream);
 }
 
 int ugbsa_paged_read(const ugbsa_paged_cache* cache, const int32_t* lens, const int32_t* table,
@@ -699,7 +723,7 @@ int ugbsa_paged_select(const ugbsa_paged_cache* cache, const void* q, int64_t sq
 
 int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int units, int cache_dtype) {
   if (check_dims(B, H, Hk, D, UGBSA_DTYPE_BF16) || units < 1) return 0;
-  return ugbsa::paged_decode_ws_elems(B, H, Hk, D, cache_dtype == UGBSA_CACHE_E4M3, units);
+  return ugbsa::paged_decode_ws_elems(B, H, Hk, D, cache_dtype, units);
 }
 
 int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,

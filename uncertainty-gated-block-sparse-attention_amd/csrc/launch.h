@@ -175,8 +175,11 @@ struct RotaryHeads {
 hipError_t launch_rotary(const RotaryTable& t, const int32_t* positions, int64_t sp_b, const RotaryHeads& q,
                          const RotaryHeads& k, int B, int M, int D, int elem, bool inverse, hipStream_t stream);
 
-// The paged cache of a call (paged.h): element strides of K and V, the scales
-// and planes contiguous; elem as above, e4m3: K and V hold e4m3 bytes.
+// The paged cache of a call (paged.h): element strides of K and V (bytes where they
+// hold codes), the scales and planes contiguous; elem as above, kind: kPages*.
+constexpr int kPagesModel = 0;    // the C ABI's UGBSA_CACHE_* values
+constexpr int kPagesE4m3 = 1;
+constexpr int kPagesE2m1 = 2;
 struct PagedCache {
   void* k = nullptr;
   void* v = nullptr;
@@ -184,7 +187,7 @@ struct PagedCache {
   uint8_t* k_scale = nullptr;
   uint8_t* v_scale = nullptr;
   uint16_t* planes = nullptr;
-  int num_pages = 0, Hk = 0, D = 0, elem = 0, e4m3 = 0;
+  int num_pages = 0, Hk = 0, D = 0, elem = 0, kind = kPagesModel;
 };
 
 // Workgroups per KV head of a write: B (cu_new null: a token a sequence) or a
@@ -193,7 +196,8 @@ int64_t paged_write_units(int B, int T, bool ragged);
 hipError_t launch_paged_write(const PagedCache& c, const uint16_t* k, int64_t sk_t, int64_t sk_h,
                               const uint16_t* v, int64_t sv_t, int64_t sv_h, const int32_t* cu_new,
                               const int32_t* lens, const int32_t* table, int64_t st_b, int B, int T,
-                              int max_pages, hipStream_t stream);
+                              int max_pages, hipStream_t stream, const RotaryTable* rot = nullptr,
+                              const int32_t* positions = nullptr);
 hipError_t launch_paged_read(const PagedCache& c, const int32_t* lens, const int32_t* table,
                              int64_t st_b, int B, int max_pages, int N, uint16_t* ko, int64_t sok_b,
                              int64_t sok_h, int64_t sok_n, uint16_t* vo, int64_t sov_b, int64_t sov_h,
@@ -208,7 +212,7 @@ hipError_t launch_paged_select(const PagedCache& c, const uint16_t* q, int64_t s
 
 // Decode attention over pages: all of them (kv_idx null) or lists of k_slots;
 // ws holds paged_decode_ws_elems fp32 (units: max_pages or k_slots).
-int64_t paged_decode_ws_elems(int B, int H, int Hk, int D, bool e4m3, int units);
+int64_t paged_decode_ws_elems(int B, int H, int Hk, int D, int kind, int units);
 hipError_t launch_paged_decode(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h,
                                int B, int H, const int32_t* lens, const int32_t* table, int64_t st_b,
                                int max_pages, const int32_t* kv_idx, const int32_t* counts, int k_slots,

@@ -5,6 +5,7 @@
 // tokens, 4 heads, into e4m3 (232 MB): 48 us, 4.8 TB/s; 64K tokens of 8 heads back
 // (404 MB): 74.7 us, 5.4 TB/s; a copy of 256 MiB runs at 5.3.
 #include "paged.h"
+#include "rotary.h"
 
 namespace ugbsa {
 
@@ -13,15 +14,67 @@ __device__ __forceinline__ int touched_pages(int len, int n_new) {
   return n_new > 0 ? (len + n_new - 1) / kBlock - len / kBlock + 1 : 0;
 }
 
+// A thread's eight dims d0 .. of the token at src + 0 .. (raw: their 16-bit values, src
+// their address), turned.
+template <typename E>
+__device__ __forceinline__ u32x4 turned8(u32x4 raw, const uint16_t* src, int d0, const RotaryTable& t, int position) {
+  const int pairs = t.pairs;
+  if (d0 >= 2 * pairs) return raw;
+  const double pos = position;
+  if (t.interleaved) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int j = d0 / 2 + w;
+      float cs, sn, a, b;
+      turn_cos_sin(pos, t.turns[min(j, pairs - 1)], t.attention, cs, sn);
+      turn_pair(E::to_f32(raw[w] & 0xFFFFu), E::to_f32(raw[w] >> 16), cs, sn, a, b);
+      if (j < pairs) raw[w] = E::pack2(a, b);
+    }
+    return raw;
+  }
+  // the other halves: eight values in a row where the halves are whole vectors
+  u32x4 other = {0u, 0u, 0u, 0u};
+  if (pairs % 8 == 0) {
+    other = *reinterpret_cast<const u32x4*>(src + (d0 < pairs ? pairs : -pairs));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = d0 + i, o = d < pairs ? d + pairs : d - pairs;
+      if (d < 2 * pairs) other[i / 2] |= static_cast<uint32_t>(src[o - d0]) << (16 * (i % 2));
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    float y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = d0 + 2 * w + i;
+      const bool low = d < pairs;
+      const float mine = E::to_f32(i ? raw[w] >> 16 : raw[w] & 0xFFFFu);
+      const float peer = E::to_f32(i ? other[w] >> 16 : other[w] & 0xFFFFu);
+      float cs, sn, a, b;
+      turn_cos_sin(pos, t.turns[min(low ? d : d - pairs, pairs - 1)], t.attention, cs, sn);
+      turn_pair(low ? mine : peer, low ? peer : mine, cs, sn, a, b);
+      y[i] = low ? a : b;
+    }
+    const uint32_t p = E::pack2(y[0], y[1]);
+    const int d = d0 + 2 * w;
+    raw[w] = d + 1 < 2 * pairs ? p : raw[w];     // 2 pairs is even: both of a word turn, or none
+  }
+  return raw;
+}
+
 // One workgroup per (touched page, KV head): it alone writes the page's head, so
 // the summary needs no atomics.  A thread takes 8 dims of every (256 / (D / 8))-th
-// token; a token's scale is a maximum over its D / 8 neighbouring lanes.
-template <typename E, int D, bool F8>
+// token; a scale is a maximum over neighbouring lanes, the D / 8 of a token or the four
+// of 32 dims.  TURN: keys are turned by their positions first (rotary.h) and rounded to
+// the 16-bit format, as ugbsa_rotary does: a thread loads its pairs' other halves too.
+template <typename E, int D, int KIND, bool TURN>
 __global__ __launch_bounds__(256) void paged_write_kernel(
     PagedCache c, const uint16_t* __restrict__ k, int64_t sk_t, int64_t sk_h,
     const uint16_t* __restrict__ v, int64_t sv_t, int64_t sv_h, const int32_t* __restrict__ cu_new,
     const int32_t* __restrict__ lens, const int32_t* __restrict__ table, int64_t st_b, int B, int T,
-    int max_pages) {
+    int max_pages, RotaryTable rot, const int32_t* __restrict__ positions) {
   constexpr int CH = D / 8, RG = 256 / CH;
   __shared__ float red[2][RG][D + 1];
   __shared__ int s_sum[4], s_unit[4];
@@ -87,9 +140,13 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       const uint16_t* src = (kv ? v + tok * sv_t + h * sv_h : k + tok * sk_t + h * sk_h) + 8 * ch;
-      const u32x4 raw = stream_load<true>(reinterpret_cast<const u32x4*>(src));
+      u32x4 raw = stream_load<true>(reinterpret_cast<const u32x4*>(src));
+      if constexpr (TURN) {
+        if (kv == 0)
+          raw = turned8<E>(raw, src, 8 * ch, rot, positions != nullptr ? positions[tok] : blk * kBlock + s);
+      }
       const int64_t at = page * (kv ? c.sv_p : c.sk_p) + h * (kv ? c.sv_h : c.sk_h) +
-                         s * (kv ? c.sv_n : c.sk_n) + 8 * ch;
+                         s * (kv ? c.sv_n : c.sk_n) + (KIND == kPagesE2m1 ? 4 * ch : 8 * ch);
       float x[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -100,8 +157,40 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
 #pragma unroll
         for (int j = 0; j < 8; ++j) mx[j] = fmaxf(mx[j], x[j]), mn[j] = fminf(mn[j], x[j]);
       }
-      if constexpr (!F8) {
+      if constexpr (KIND == kPagesModel) {
         *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(kv ? c.v : c.k) + at) = raw;
+      } else if constexpr (KIND == kPagesE2m1) {
+        // the largest magnitude that reads back finite from two bits; a group with a NaN
+        // is NaN throughout, as its codes have no room for one
+        constexpr float kMost = E::code == ElemF16::code ? 49152.f : 1.5f * 0x1p127f;
+        float top = 0.f;
+        uint32_t nan = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          nan |= x[j] != x[j] ? 1u : 0u;
+          x[j] = x[j] > kMost ? kMost : (x[j] < -kMost ? -kMost : x[j]);
+          top = fmaxf(top, fabsf(x[j]));
+        }
+#pragma unroll
+        for (int off = 2; off >= 1; off >>= 1) {
+          top = fmaxf(top, __shfl_xor(top, off, 64));
+          nan |= __shfl_xor(nan, off, 64);
+        }
+        // smallest e with top <= 6 2^e = 1.5 2^(e + 2), as a byte e + 127
+        const uint32_t bits = __float_as_uint(top);
+        const int e = static_cast<int>(bits >> 23) - 2 + ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 0);
+        const int byte = bits == 0u ? 127 : max(e, 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = nan ? 0.f : ldexpf(x[j], 127 - byte);   // exact, or below half a step
+        uint32_t code = 0u;
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], 1.f, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], 1.f, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[4], x[5], 1.f, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[6], x[7], 1.f, 3);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kv ? c.v : c.k) + at) = code;
+        if (ch % 4 == 0)
+          (kv ? c.v_scale : c.k_scale)[(head * (D / 32) + ch / 4) * kBlock + s] =
+              static_cast<uint8_t>(nan ? 255 : byte);
       } else {
         // the largest magnitude whose four-bit rounding reads back finite (infinities
         // are held there too; NaN stays NaN and does not count for the scale)
@@ -176,7 +265,7 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
 // One workgroup per (64 output rows, KV head, sequence): rows past the length are
 // zeros.  NT: an output that the 256 MB memory-side cache does not hold goes past it,
 // as do the pages it comes from.
-template <typename E, int D, bool F8, bool NT>
+template <typename E, int D, int KIND, bool NT>
 __global__ __launch_bounds__(256) void paged_read_kernel(
     PagedCache c, const int32_t* __restrict__ lens, const int32_t* __restrict__ table, int64_t st_b,
     int max_pages, int N, uint16_t* __restrict__ ko, int64_t sok_b, int64_t sok_h, int64_t sok_n,
@@ -196,8 +285,13 @@ __global__ __launch_bounds__(256) void paged_read_kernel(
       u32x4 x = {0u, 0u, 0u, 0u};
       if (s < held) {
         const int64_t at = page * (kv ? c.sv_p : c.sk_p) + h * (kv ? c.sv_h : c.sk_h) +
-                           s * (kv ? c.sv_n : c.sk_n) + 8 * ch;
-        if constexpr (!F8) {
+                           s * (kv ? c.sv_n : c.sk_n) + (KIND == kPagesE2m1 ? 4 * ch : 8 * ch);
+        if constexpr (KIND == kPagesE2m1) {
+          const uint32_t code =
+              stream_load<NT>(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(kv ? c.v : c.k) + at));
+          const float scale = e8m0((kv ? c.v_scale : c.k_scale)[(head * (D / 32) + ch / 4) * kBlock + s]);
+          x = e2m1_x8<E>(code, scale);
+        } else if constexpr (KIND == kPagesModel) {
           x = stream_load<NT>(reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(kv ? c.v : c.k) + at));
         } else {
           const u32x2 code = stream_load<NT>(reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(kv ? c.v : c.k) + at));
@@ -215,18 +309,20 @@ __global__ __launch_bounds__(256) void paged_read_kernel(
 #define UGBSA_PAGED_INSTANCES(CALL)                                       \
   do {                                                                    \
     if (c.elem == ElemF16::code) {                                        \
-      if (c.e4m3) { UGBSA_PAGED_D(CALL, ElemF16, true); }                 \
-      else { UGBSA_PAGED_D(CALL, ElemF16, false); }                       \
+      if (c.kind == kPagesE2m1) { UGBSA_PAGED_D(CALL, ElemF16, kPagesE2m1); }    \
+      else if (c.kind == kPagesE4m3) { UGBSA_PAGED_D(CALL, ElemF16, kPagesE4m3); } \
+      else { UGBSA_PAGED_D(CALL, ElemF16, kPagesModel); }                 \
     } else {                                                              \
-      if (c.e4m3) { UGBSA_PAGED_D(CALL, ElemBf16, true); }                \
-      else { UGBSA_PAGED_D(CALL, ElemBf16, false); }                      \
+      if (c.kind == kPagesE2m1) { UGBSA_PAGED_D(CALL, ElemBf16, kPagesE2m1); }   \
+      else if (c.kind == kPagesE4m3) { UGBSA_PAGED_D(CALL, ElemBf16, kPagesE4m3); } \
+      else { UGBSA_PAGED_D(CALL, ElemBf16, kPagesModel); }                \
     }                                                                     \
     return hipErrorInvalidValue;                                          \
   } while (0)
-#define UGBSA_PAGED_D(CALL, E_, F8_)                                      \
-  if (c.D == 64) { CALL(E_, 64, F8_); return hipGetLastError(); }         \
-  if (c.D == 128) { CALL(E_, 128, F8_); return hipGetLastError(); }       \
-  if (c.D == 256) { CALL(E_, 256, F8_); return hipGetLastError(); }
+#define UGBSA_PAGED_D(CALL, E_, K_)                                       \
+  if (c.D == 64) { CALL(E_, 64, K_); return hipGetLastError(); }          \
+  if (c.D == 128) { CALL(E_, 128, K_); return hipGetLastError(); }        \
+  if (c.D == 256) { CALL(E_, 256, K_); return hipGetLastError(); }
 
 int64_t paged_write_units(int B, int T, bool ragged) {
   if (!ragged) return B;
@@ -238,11 +334,14 @@ int64_t paged_write_units(int B, int T, bool ragged) {
 hipError_t launch_paged_write(const PagedCache& c, const uint16_t* k, int64_t sk_t, int64_t sk_h,
                               const uint16_t* v, int64_t sv_t, int64_t sv_h, const int32_t* cu_new,
                               const int32_t* lens, const int32_t* table, int64_t st_b, int B, int T,
-                              int max_pages, hipStream_t stream) {
+                              int max_pages, hipStream_t stream, const RotaryTable* rot,
+                              const int32_t* positions) {
   const dim3 grid(static_cast<uint32_t>(paged_write_units(B, T, cu_new != nullptr)), c.Hk);
-#define UGBSA_CALL(E_, D_, F8_)                                                                  \
-  paged_write_kernel<E_, D_, F8_><<<grid, 256, 0, stream>>>(c, k, sk_t, sk_h, v, sv_t, sv_h, cu_new, \
-                                                            lens, table, st_b, B, T, max_pages)
+  const RotaryTable t = rot != nullptr ? *rot : RotaryTable{};
+#define UGBSA_CALL(E_, D_, K_)                                                                            \
+  (rot != nullptr ? paged_write_kernel<E_, D_, K_, true> : paged_write_kernel<E_, D_, K_, false>)         \
+      <<<grid, 256, 0, stream>>>(c, k, sk_t, sk_h, v, sv_t, sv_h, cu_new, lens, table, st_b, B, T, max_pages, t, \
+                                 positions)
   UGBSA_PAGED_INSTANCES(UGBSA_CALL);
 #undef UGBSA_CALL
 }
@@ -254,8 +353,8 @@ hipError_t launch_paged_read(const PagedCache& c, const int32_t* lens, const int
   const dim3 grid((N + kBlock - 1) / kBlock, c.Hk, B);
   // 64K tokens of 8 heads from e4m3 (268 MB): 86 -> 81.6 us
   const bool past_cache = 4 * static_cast<int64_t>(B) * c.Hk * N * c.D >= 256 << 20;
-#define UGBSA_CALL(E_, D_, F8_)                                                                     \
-  (past_cache ? paged_read_kernel<E_, D_, F8_, true> : paged_read_kernel<E_, D_, F8_, false>)       \
+#define UGBSA_CALL(E_, D_, K_)                                                                      \
+  (past_cache ? paged_read_kernel<E_, D_, K_, true> : paged_read_kernel<E_, D_, K_, false>)         \
       <<<grid, 256, 0, stream>>>(c, lens, table, st_b, max_pages, N, ko, sok_b, sok_h, sok_n, vo, sov_b, \
                                  sov_h, sov_n)
   UGBSA_PAGED_INSTANCES(UGBSA_CALL);

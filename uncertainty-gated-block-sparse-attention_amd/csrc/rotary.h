@@ -37,8 +37,7 @@ __device__ __forceinline__ void turn_cos_sin(double pos, double turns, float m, 
   sn *= quarter >= 2 ? -m : m;
 }
 
-// Two 16-bit values (a low, b high) of one pair, turned and rounded once.
-template <typename E>
+// The two values of a pair, turned.
 __device__ __forceinline__ void turn_pair(float a, float b, float cs, float sn, float& ya, float& yb) {
   ya = __builtin_fmaf(a, cs, -(b * sn));
   yb = __builtin_fmaf(b, cs, a * sn);

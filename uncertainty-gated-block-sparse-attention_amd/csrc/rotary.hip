@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads 
         for (int w = 0; w < 8; ++w) {
           const uint32_t p = w < 4 ? va[i][w & 3] : vb[i][w & 3];
           float a, c;
-          turn_pair<E>(E::to_f32(p & 0xFFFFu), E::to_f32(p >> 16), cs[w], sn[w], a, c);
+          turn_pair(E::to_f32(p & 0xFFFFu), E::to_f32(p >> 16), cs[w], sn[w], a, c);
           const uint32_t y = j0 + w < pairs ? E::pack2(a, c) : p;
           if (w < 4) va[i][w & 3] = y;
           else vb[i][w & 3] = y;
@@ -66,8 +66,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads 
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           float a0, a1, b0, b1;
-          turn_pair<E>(E::to_f32(va[i][w] & 0xFFFFu), E::to_f32(vb[i][w] & 0xFFFFu), cs[2 * w], sn[2 * w], a0, b0);
-          turn_pair<E>(E::to_f32(va[i][w] >> 16), E::to_f32(vb[i][w] >> 16), cs[2 * w + 1], sn[2 * w + 1], a1, b1);
+          turn_pair(E::to_f32(va[i][w] & 0xFFFFu), E::to_f32(vb[i][w] & 0xFFFFu), cs[2 * w], sn[2 * w], a0, b0);
+          turn_pair(E::to_f32(va[i][w] >> 16), E::to_f32(vb[i][w] >> 16), cs[2 * w + 1], sn[2 * w + 1], a1, b1);
           va[i][w] = E::pack2(a0, a1);
           vb[i][w] = E::pack2(b0, b1);
         }
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256) void rotary_odd_kernel(RotaryHeads q, RotaryHe
                          : k.y + b * k.sy_b + hh * k.sy_h + m * k.sy_m;
       if (turn) {
         float a, c;
-        turn_pair<E>(E::to_f32(x[j]), E::to_f32(x[j + pairs]), cs, sn, a, c);
+        turn_pair(E::to_f32(x[j]), E::to_f32(x[j + pairs]), cs, sn, a, c);
         const uint32_t p = E::pack2(a, c);
         y[j] = static_cast<uint16_t>(p & 0xFFFFu);
         y[j + pairs] = static_cast<uint16_t>(p >> 16);

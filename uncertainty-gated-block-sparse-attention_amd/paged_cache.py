@@ -2,9 +2,9 @@
 
 The dispatcher's decode attends to a contiguous ``[B, Hk, N, D]`` cache; a server keeps keys and
 values in pages of 64 tokens, the selection block, that a block table names.  Pages hold the
-model's dtype or e4m3 codes with a power-of-two scale per token and head, and beside them stands
-each page's Quest summary (K-max, K-min of the keys as given, before e4m3 rounds them), kept up to
-date as tokens are written:
+model's dtype, e4m3 codes with a power-of-two scale per token and head, or e2m1 codes (four bits) with one per
+32 dims of it, and beside them stands each page's Quest summary (K-max, K-min of the keys as given,
+before they are rounded to codes), kept up to date as tokens are written:
 
     cache = PagedCache.empty(num_pages, Hk, D, torch.bfloat16, "cuda", e4m3=True)
     paged_write(cache, k, v, block_table, seq_lens, cu_new=cu)     # prompts [T, Hk, D], packed
@@ -35,6 +35,7 @@ from torch.autograd import forward_ad
 import _capi
 
 PAGE = 64    # tokens per page: the selection block
+GROUP = 32   # dims of a token's head that share an e2m1 scale
 
 _tracing_state = torch._C._get_tracing_state
 
@@ -44,10 +45,11 @@ class PagedCache:
     """Pages of one layer and their summaries.  The handle keeps the tensors and their addresses:
     they are written in place, never resized or pointed elsewhere.
 
-    k_pages, v_pages : [P, Hk, 64, D] in ``dtype`` or ``torch.float8_e4m3fn`` (unit stride on
-    head_dim, 16-byte aligned rows, any other strides; expanded pages, or one tensor for both, can
-    be read but not written)
-    k_scale, v_scale : [P, Hk, 64] uint8 contiguous, for e4m3 pages: a value is code * 2^(byte - 127)
+    k_pages, v_pages : [P, Hk, 64, D] in ``dtype`` or ``torch.float8_e4m3fn``, or [P, Hk, 64, D / 2] uint8,
+    two e2m1 codes a byte, the even dim in its low four bits (unit stride on head_dim, 16-byte aligned
+    rows, any other strides; expanded pages, or one tensor for both, can be read but not written)
+    k_scale, v_scale : uint8 contiguous, [P, Hk, 64] for e4m3 pages, [P, Hk, D / 32, 64] for e2m1: a value
+    is code * 2^(byte - 127) (e2m1: NaN where the byte is 255)
     planes : [P, Hk, 2, D] in ``dtype``, contiguous: K-max and K-min of each page.  Optional where
     nothing is selected; a cache of planes alone (no pages) serves ``paged_select`` only.
     dtype : bf16 or fp16, the format of q, k, v and of every result
@@ -70,17 +72,21 @@ class PagedCache:
         assert k is not None or planes is not None, "pages or planes required"
         dtype = self.dtype
         e4m3 = k is not None and k.dtype == torch.float8_e4m3fn
+        e2m1 = k is not None and k.dtype == torch.uint8
+        codes = e4m3 or e2m1
         if dtype is None:
-            assert not e4m3 or planes is not None, "dtype required (e4m3 pages do not tell it)"
+            assert not codes or planes is not None, "dtype required (codes do not tell it)"
             dtype = planes.dtype if planes is not None else k.dtype
             object.__setattr__(self, "dtype", dtype)
         code = _capi.dtype_code(dtype)
         s = _capi.PagedCacheStruct(dtype=code,
-                                   cache_dtype=_capi.CACHE_E4M3 if e4m3 else _capi.CACHE_MODEL)
+                                   cache_dtype=_capi.CACHE_E2M1 if e2m1 else _capi.CACHE_E4M3 if e4m3
+                                   else _capi.CACHE_MODEL)
         if k is not None:
             assert k.dim() == 4 and k.shape == v.shape and k.shape[2] == PAGE, "pages [P, Hk, 64, D] expected"
-            assert k.dtype == v.dtype and (e4m3 or k.dtype == dtype), f"pages: {dtype} or e4m3 required"
+            assert k.dtype == v.dtype and (codes or k.dtype == dtype), f"pages: {dtype}, e4m3 or uint8 required"
             s.num_pages, s.Hk, _, s.D = k.shape
+            s.D *= 2 if e2m1 else 1
             unit = 16 // k.element_size()
             for t in (k, v):
                 assert t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(x % unit for x in t.stride()[:3]), \
@@ -88,12 +94,13 @@ class PagedCache:
             s.k_pages, s.v_pages = k.data_ptr(), v.data_ptr()
             s.sk_p, s.sk_h, s.sk_n, _ = k.stride()
             s.sv_p, s.sv_h, s.sv_n, _ = v.stride()
-            assert e4m3 == (self.k_scale is not None) == (self.v_scale is not None), \
-                "scales go with e4m3 pages"
-            if e4m3:
+            assert codes == (self.k_scale is not None) == (self.v_scale is not None), \
+                "scales go with quantised pages"
+            if codes:
+                want = (s.num_pages, s.Hk, s.D // GROUP, PAGE) if e2m1 else (s.num_pages, s.Hk, PAGE)
                 for t in (self.k_scale, self.v_scale):
-                    assert t.shape == k.shape[:3] and t.dtype == torch.uint8 and t.is_contiguous() \
-                        and t.data_ptr() % 8 == 0, "scales [P, Hk, 64] uint8 contiguous expected"
+                    assert t.shape == want and t.dtype == torch.uint8 and t.is_contiguous() \
+                        and t.data_ptr() % 8 == 0, f"scales {list(want)} uint8 contiguous expected"
                 s.k_scale, s.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
         if planes is not None:
             if k is None:
@@ -114,12 +121,14 @@ class PagedCache:
         object.__setattr__(self, "_call", (ctypes.addressof(s), tensors[0].get_device(), s.Hk, s.D))
 
     @classmethod
-    def empty(cls, num_pages, Hk, D, dtype, device, e4m3=False, summaries=True):
+    def empty(cls, num_pages, Hk, D, dtype, device, e4m3=False, summaries=True, e2m1=False):
         """Uninitialised pages: every slot a sequence reads is written first."""
-        shape = (num_pages, Hk, PAGE, D)
-        pages = torch.float8_e4m3fn if e4m3 else dtype
+        assert not (e4m3 and e2m1), "pages are e4m3 or e2m1"
+        shape = (num_pages, Hk, PAGE, D // 2 if e2m1 else D)
+        pages = torch.uint8 if e2m1 else torch.float8_e4m3fn if e4m3 else dtype
+        scales = (num_pages, Hk, D // GROUP, PAGE) if e2m1 else shape[:3]
         k, v = (torch.empty(shape, dtype=pages, device=device) for _ in range(2))
-        ks, vs = (torch.empty(shape[:3], dtype=torch.uint8, device=device) if e4m3 else None for _ in range(2))
+        ks, vs = (torch.empty(scales, dtype=torch.uint8, device=device) if e4m3 or e2m1 else None for _ in range(2))
         planes = torch.empty(num_pages, Hk, 2, D, dtype=dtype, device=device) if summaries else None
         return cls(k, v, ks, vs, planes, dtype)
 
@@ -207,13 +216,15 @@ def _launch(cache, what, fn, *args):
         _capi.check(rc, what)
 
 
-def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
-    """New tokens into the cache, quantised if it holds e4m3, and its page summaries.
+def paged_write(cache, k, v, block_table, seq_lens, cu_new=None, rotary=None, positions=None):
+    """New tokens into the cache, quantised if it holds codes, and its page summaries.
 
     k, v : [T, Hk, D], the new tokens of all sequences, packed
     cu_new : [B + 1] int32, ascending: sequence b's are rows cu_new[b] .. cu_new[b + 1] - 1; None:
     one token each, row b
     seq_lens : tokens cached before this call; the new ones follow them (the caller adds them up)
+    rotary : a ``rotary.Rotary``: keys are turned by ``positions`` [T] int32 on the way, to the bits that
+    ``rotary.rotary`` gives; without positions by their places in their sequences
 
     Rows behind the last sequence and tokens past the table are left out.  Two sequences may share
     pages, but no page that a call writes to may be named twice by the entries it writes through.
@@ -228,9 +239,19 @@ def paged_write(cache, k, v, block_table, seq_lens, cu_new=None):
         _check_unwatched(k, v)
     if cu_new is not None:
         _check_ints("cu_new", cu_new, cache, (B + 1,))
-    _launch(cache, "paged_write", _capi.lib().ugbsa_paged_write, k.data_ptr(), *k.stride(),
+    fn, turn = _capi.lib().ugbsa_paged_write, ()
+    if rotary is not None:
+        address, index, dims = rotary._call
+        assert index == cache._call[1], "rotary must be on the cache's device"
+        assert dims <= shape[2], f"rotary: head_dim {shape[2]} must hold the table's {dims} dims"
+        if positions is not None:
+            _check_ints("positions", positions, cache, (shape[0],))
+        fn, turn = _capi.lib().ugbsa_paged_write_rotary, (address, _capi.ptr(positions))
+    else:
+        assert positions is None, "positions without rotary"
+    _launch(cache, "paged_write", fn, k.data_ptr(), *k.stride(),
             v.data_ptr(), *v.stride(), None if cu_new is None else cu_new.data_ptr(), seq_lens.data_ptr(),
-            block_table.data_ptr(), st_b, B, shape[0], max_pages)
+            block_table.data_ptr(), st_b, B, shape[0], max_pages, *turn)
 
 
 def paged_read(cache, block_table, seq_lens, n, out=None):
