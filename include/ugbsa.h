@@ -441,6 +441,37 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
                        int64_t so_b, int64_t so_h, int64_t so_d, float* workspace,
                        int64_t workspace_elems, void* stream);
 
+/* ugbsa_paged_decode, and the weights of each cached token followed: mass [B, Hk,
+ * 64 * max_pages] fp32 (rows b and h at strides sm_b and sm_h, 16-byte aligned, each its
+ * own memory): mass[b][h][i] grows by the sum over the KV head's query heads of the
+ * softmax weight of token i (fp32, unrounded, in the heads' order).  Tokens that a row
+ * does not attend to, and entries from lens[b] on, keep theirs. */
+int64_t ugbsa_paged_decode_mass_workspace_elems(int B, int H, int Hk, int D, int units,
+                                                int cache_dtype);
+int ugbsa_paged_decode_mass(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b,
+                            int64_t sq_h, int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                            const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
+                            const int32_t* kv_idx, const int32_t* counts, int k_slots, float* mass,
+                            int64_t sm_b, int64_t sm_h, void* out, int64_t so_b, int64_t so_h,
+                            int64_t so_d, float* workspace, int64_t workspace_elems, void* stream);
+
+/* Sequences cut back to keep tokens, each KV head to its own: the first `first`, the
+ * newest `recent` and, of the others, the largest by (mass desc, token asc; NaN before
+ * numbers) — all of them where the sequence has no more.  Tokens of absent pages are not
+ * kept.  The kept tokens go, in their order and as they are stored, to slots 0, 1, ... of
+ * the pages that new_table [B, new_pages] names, whose summaries (if the cache has planes)
+ * become those of their keys as stored.  No page that new_table names may be one that
+ * table names for a token, nor be named twice.  Out: kept [B, Hk, keep] int32, the tokens,
+ * ascending, then 64 * max_pages; new_lens [B] int32; new_mass [B, Hk, 64 * new_pages], the
+ * kept tokens' mass, then zeros (mass and new_mass: rows as above).  Keys keep the
+ * positions they were turned by: a later token's position is no longer its length.
+ * 1 <= keep <= 64 * new_pages; recent + first <= keep. */
+int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t sm_b,
+                      int64_t sm_h, const int32_t* lens, const int32_t* table, int64_t st_b, int B,
+                      int max_pages, const int32_t* new_table, int64_t sn_b, int new_pages,
+                      int keep, int recent, int first, int32_t* kept, int32_t* new_lens,
+                      float* new_mass, int64_t so_b, int64_t so_h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -726,12 +726,17 @@ int64_t ugbsa_paged_decode_workspace_elems(int B, int H, int Hk, int D, int unit
   return ugbsa::paged_decode_ws_elems(B, H, Hk, D, cache_dtype, units);
 }
 
-int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
-                       int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
-                       const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
-                       const int32_t* kv_idx, const int32_t* counts, int k_slots, void* out,
-                       int64_t so_b, int64_t so_h, int64_t so_d, float* workspace,
-                       int64_t workspace_elems, void* stream) {
+int64_t ugbsa_paged_decode_mass_workspace_elems(int B, int H, int Hk, int D, int units, int cache_dtype) {
+  if (check_dims(B, H, Hk, D, UGBSA_DTYPE_BF16) || units < 1) return 0;
+  return ugbsa::paged_mass_ws_elems(B, H, Hk, D, cache_dtype, units);
+}
+
+// What the decode calls share: all but the workspace.
+static int check_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                              int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                              const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
+                              const int32_t* kv_idx, const int32_t* counts, int k_slots, const void* out,
+                              int64_t so_b, int64_t so_h, int64_t so_d) {
   int rc = check_paged(cache, H, lens, table, st_b, B, max_pages);
   if (rc || (rc = check_pages(cache))) return rc;
   if ((rc = check_bf16_operand("q", q, sq_b, sq_h, sq_m, sq_d))) return rc;
@@ -746,18 +751,88 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
   if ((reinterpret_cast<uintptr_t>(out) & 3) || so_b % 2 || so_h % 2)
     return fail(UGBSA_ELAYOUT, "out must have 4-byte aligned rows");
   if (static_cast<int64_t>(B) * H >= 1 << 24) return fail(UGBSA_EARG, "B * H must be below 2^24");
+  return UGBSA_OK;
+}
+
+static int check_decode_workspace(const char* query, int64_t need, const float* workspace, int64_t workspace_elems) {
+  if (need > 0 && (workspace == nullptr || workspace_elems < need))
+    return fail(UGBSA_EARG, "workspace of %lld floats is smaller than %s (%lld)", (long long)workspace_elems, query,
+                (long long)need);
+  if (!aligned16(workspace)) return fail(UGBSA_ELAYOUT, "workspace must be 16-byte aligned");
+  return UGBSA_OK;
+}
+
+int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                       int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                       const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
+                       const int32_t* kv_idx, const int32_t* counts, int k_slots, void* out,
+                       int64_t so_b, int64_t so_h, int64_t so_d, float* workspace,
+                       int64_t workspace_elems, void* stream) {
+  int rc = check_paged_decode(cache, q, sq_b, sq_h, sq_m, sq_d, H, lens, table, st_b, B, max_pages, scale, kv_idx,
+                              counts, k_slots, out, so_b, so_h, so_d);
+  if (rc) return rc;
   const int64_t need = ugbsa_paged_decode_workspace_elems(B, H, cache->Hk, cache->D,
                                                           kv_idx != nullptr ? k_slots : max_pages,
                                                           cache->cache_dtype);
-  if (need > 0 && (workspace == nullptr || workspace_elems < need))
-    return fail(UGBSA_EARG, "workspace of %lld floats is smaller than ugbsa_paged_decode_workspace_elems (%lld)",
-                (long long)workspace_elems, (long long)need);
-  if (!aligned16(workspace)) return fail(UGBSA_ELAYOUT, "workspace must be 16-byte aligned");
+  if ((rc = check_decode_workspace("ugbsa_paged_decode_workspace_elems", need, workspace, workspace_elems))) return rc;
   return hip_result(ugbsa::launch_paged_decode(paged_cache(cache), static_cast<const uint16_t*>(q), sq_b,
                                                sq_h, B, H, lens, table, st_b, max_pages, kv_idx, counts,
                                                k_slots, scale, static_cast<uint16_t*>(out), so_b, so_h,
                                                workspace, static_cast<hipStream_t>(stream)),
                     "paged_decode");
+}
+
+// Rows of weights [B, Hk, 64 * pages], each its own memory, read and written four at a time.
+static int check_mass(const char* name, const float* mass, int64_t sm_b, int64_t sm_h) {
+  if (mass == nullptr) return fail(UGBSA_EARG, "%s is null", name);
+  if (!aligned16(mass) || sm_b % 4 || sm_h % 4 || sm_b < 0 || sm_h < 0)
+    return fail(UGBSA_ELAYOUT, "%s must have 16-byte aligned rows", name);
+  return UGBSA_OK;
+}
+
+int ugbsa_paged_decode_mass(const ugbsa_paged_cache* cache, const void* q, int64_t sq_b, int64_t sq_h,
+                            int64_t sq_m, int64_t sq_d, int H, const int32_t* lens,
+                            const int32_t* table, int64_t st_b, int B, int max_pages, float scale,
+                            const int32_t* kv_idx, const int32_t* counts, int k_slots, float* mass,
+                            int64_t sm_b, int64_t sm_h, void* out, int64_t so_b, int64_t so_h,
+                            int64_t so_d, float* workspace, int64_t workspace_elems, void* stream) {
+  int rc = check_paged_decode(cache, q, sq_b, sq_h, sq_m, sq_d, H, lens, table, st_b, B, max_pages, scale, kv_idx,
+                              counts, k_slots, out, so_b, so_h, so_d);
+  if (rc || (rc = check_mass("mass", mass, sm_b, sm_h))) return rc;
+  const int64_t need = ugbsa_paged_decode_mass_workspace_elems(B, H, cache->Hk, cache->D,
+                                                               kv_idx != nullptr ? k_slots : max_pages,
+                                                               cache->cache_dtype);
+  if ((rc = check_decode_workspace("ugbsa_paged_decode_mass_workspace_elems", need, workspace, workspace_elems)))
+    return rc;
+  return hip_result(ugbsa::launch_paged_mass(paged_cache(cache), static_cast<const uint16_t*>(q), sq_b, sq_h, B, H,
+                                             lens, table, st_b, max_pages, kv_idx, counts, k_slots, scale, mass, sm_b,
+                                             sm_h, static_cast<uint16_t*>(out), so_b, so_h, workspace,
+                                             static_cast<hipStream_t>(stream)),
+                    "paged_decode_mass");
+}
+
+int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t sm_b, int64_t sm_h,
+                      const int32_t* lens, const int32_t* table, int64_t st_b, int B, int max_pages,
+                      const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
+                      int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
+                      void* stream) {
+  int rc = check_paged(cache, cache ? cache->Hk : 1, lens, table, st_b, B, max_pages);
+  if (rc || (rc = check_pages(cache)) || (rc = check_mass("mass", mass, sm_b, sm_h)) ||
+      (rc = check_mass("new_mass", new_mass, so_b, so_h)))
+    return rc;
+  if (new_table == nullptr || kept == nullptr || new_lens == nullptr)
+    return fail(UGBSA_EARG, "new_table, kept or new_lens is null");
+  if (sn_b < 0) return fail(UGBSA_ELAYOUT, "new_table: negative row stride");
+  if (new_pages < 1 || new_pages > 1 << 24) return fail(UGBSA_EARG, "new_pages must lie in [1, 2^24] (%d)", new_pages);
+  if (keep < 1 || keep > static_cast<int64_t>(new_pages) * ugbsa::kBlock)
+    return fail(UGBSA_EARG, "keep must lie in [1, 64 * new_pages] (%d, new_pages %d)", keep, new_pages);
+  if (recent < 0 || first < 0 || static_cast<int64_t>(recent) + first > keep)
+    return fail(UGBSA_EARG, "recent and first must not be negative, nor more than keep together (%d, %d, keep %d)",
+                recent, first, keep);
+  return hip_result(ugbsa::launch_paged_evict(paged_cache(cache), mass, sm_b, sm_h, lens, table, st_b, B, max_pages,
+                                              new_table, sn_b, new_pages, keep, recent, first, kept, new_lens,
+                                              new_mass, so_b, so_h, static_cast<hipStream_t>(stream)),
+                    "paged_evict");
 }
 
 int ugbsa_rotary(const ugbsa_rotary_table* table, const int32_t* positions, int64_t sp_b, const void* q,

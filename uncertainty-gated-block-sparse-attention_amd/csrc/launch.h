@@ -219,4 +219,21 @@ hipError_t launch_paged_decode(const PagedCache& c, const uint16_t* q, int64_t s
                                float scale, uint16_t* out, int64_t so_b, int64_t so_h, float* ws,
                                hipStream_t stream);
 
+// The same, the weights added to mass [B, Hk, 64 max_pages] fp32; ws holds
+// paged_mass_ws_elems fp32.
+int64_t paged_mass_ws_elems(int B, int H, int Hk, int D, int kind, int units);
+hipError_t launch_paged_mass(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h, int B, int H,
+                             const int32_t* lens, const int32_t* table, int64_t st_b, int max_pages,
+                             const int32_t* kv_idx, const int32_t* counts, int k_slots, float scale, float* mass,
+                             int64_t sm_b, int64_t sm_h, uint16_t* out, int64_t so_b, int64_t so_h, float* ws,
+                             hipStream_t stream);
+
+// The first, the newest and the heaviest tokens of each (sequence, KV head) into other
+// pages (paged_evict.hip).
+hipError_t launch_paged_evict(const PagedCache& c, const float* mass, int64_t sm_b, int64_t sm_h,
+                              const int32_t* lens, const int32_t* table, int64_t st_b, int B, int max_pages,
+                              const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
+                              int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
+                              hipStream_t stream);
+
 }  // namespace ugbsa

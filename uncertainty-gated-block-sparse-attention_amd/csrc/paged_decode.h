@@ -476,7 +476,7 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
 constexpr int kPdMaxWorkgroups = 1024;
 constexpr int kPdCombineThreads = 256;
 template <typename E, int D>
-__global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
+static __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
     const int* __restrict__ starts, const float* __restrict__ part, const float* __restrict__ ml,
     PagedGroups gr, int grp, int chunks, bool lists, uint16_t* __restrict__ out, int64_t so_b,
     int64_t so_h, float* __restrict__ row_ml) {

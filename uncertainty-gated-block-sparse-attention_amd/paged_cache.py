@@ -310,7 +310,21 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
     return PagedSelection(kv_idx, counts, sigma, uncertain)
 
 
-def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=None, out=None):
+def _check_mass(name, t, cache, shape):
+    """Weights [B, Hk, >= 64 * pages] fp32 that a call reads or adds to in place, each row its own memory."""
+    assert t.dim() == 3 and t.shape[:2] == shape[:2] and t.shape[2] >= shape[2] and t.dtype is torch.float32 \
+        and t.get_device() == cache._call[1], f"{name} [{shape[0]}, {shape[1]}, >= {shape[2]}] fp32 on the cache's device expected"
+    assert t.stride(2) == 1 and t.data_ptr() % 16 == 0 and not any(s % 4 for s, n in zip(t.stride()[:2], shape) if n > 1), \
+        f"{name}: contiguous, 16-byte aligned rows required"
+    assert not (t.is_neg() or t.requires_grad), f"{name}: a plain tensor without gradients required"
+
+
+def _rows(t):
+    """Row strides of a tensor of weights: of a dimension of one element any will do."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:2], t.shape))
+
+
+def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=None, out=None, mass=None):
     """Attention of one new token per sequence over its cached tokens, of every page or of the
     listed ones.
 
@@ -318,6 +332,8 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     kv_idx : [B, Hk, k_slots >= 1] int32, the pages (numbered within the sequence, each at most once)
     that the KV head's query heads attend to; counts [B, Hk] int32: how many entries count (None:
     all).  Entries that are no page of the sequence are skipped.
+    mass : [B, Hk, >= 64 * max_pages] fp32, what each cached token's weight adds up to, for ``paged_evict``:
+    entry i of a row grows by the sum over the KV head's query heads of token i's softmax weight
     Returns [B, 1, H, D] contiguous, the dispatcher's layout (``out`` if given).  A sequence without
     a key gives zeros.  Weights are rounded to ``dtype`` before the product with V.  The launch is
     shaped by the table's (or list's) width: pass a table cut to the longest sequence where the batch
@@ -329,7 +345,7 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     H = q.shape[1] if q.dim() == 4 else 0
     q = _operand("q", q, cache, (B, H, 1, D))
     if _watched():
-        _check_unwatched(q, out)
+        _check_unwatched(q, out, mass)
     slots = 0
     if kv_idx is not None:
         slots = kv_idx.shape[-1] if kv_idx.dim() == 3 else 0
@@ -343,9 +359,67 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
         _check_out(out, cache, (B, 1, H, D))
     so_b, _, so_h, so_d = out.stride()
     lib = _capi.lib()
+    if mass is not None:
+        _check_mass("mass", mass, cache, (B, Hk, PAGE * max_pages))
+        sm_b, sm_h = mass.stride()[:2]
+        assert (B == 1 or sm_b) and (Hk == 1 or sm_h), "mass: rows share memory"
+        assert B == 1 or Hk == 1 or max(sm_b, sm_h) >= mass.shape[2] + (mass.shape[1 if sm_b > sm_h else 0] - 1) * min(sm_b, sm_h), \
+            "mass: rows share memory"
+        n = lib.ugbsa_paged_decode_mass_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
+        ws = torch.empty(n, dtype=torch.float32, device=cache.device)
+        torch.autograd.graph.increment_version(mass)
+        _launch(cache, "paged_decode_mass", lib.ugbsa_paged_decode_mass, q.data_ptr(), *q.stride(), H,
+                seq_lens.data_ptr(), block_table.data_ptr(), st_b, B, max_pages, scale, _capi.ptr(kv_idx),
+                _capi.ptr(counts), slots, mass.data_ptr(), *_rows(mass), out.data_ptr(), so_b, so_h, so_d,
+                ws.data_ptr(), n)
+        return out
     n = lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
     ws = torch.empty(n, dtype=torch.float32, device=cache.device) if n else None
     _launch(cache, "paged_decode", lib.ugbsa_paged_decode, q.data_ptr(), *q.stride(), H, seq_lens.data_ptr(),
             block_table.data_ptr(), st_b, B, max_pages, scale, _capi.ptr(kv_idx), _capi.ptr(counts), slots,
             out.data_ptr(), so_b, so_h, so_d, _capi.ptr(ws), n)
     return out
+
+
+@dataclass
+class PagedEviction:
+    kept: torch.Tensor         # int32 [B, Hk, keep] tokens that stayed, ascending, then 64 * max_pages
+    seq_lens: torch.Tensor     # int32 [B] tokens of each sequence now
+    mass: torch.Tensor         # fp32 [B, Hk, 64 * new_pages] their weights, then zeros
+
+
+def paged_evict(cache, mass, block_table, seq_lens, new_table, keep, recent=0, first=0):
+    """Sequences cut back to ``keep`` tokens, packed into other pages: each KV head keeps the first
+    ``first`` tokens, the newest ``recent`` and, of the others, those of the largest ``mass``.
+
+    mass : [B, Hk, >= 64 * max_pages] fp32 as ``paged_decode`` adds it up.  Ties stay by the lower token,
+    NaN before numbers; tokens of absent pages do not stay
+    new_table : [B, new_pages] int32, 64 * new_pages >= keep: the pages that take the kept tokens, in
+    their order.  None may be a page that the call reads (those are free afterwards, unless another
+    sequence shares them), nor be named twice
+
+    A sequence of no more than ``keep`` tokens keeps all of them (call with the rows of ``block_table``
+    that are to be cut back).  Codes and scales are copied as they are; page summaries become those of
+    the keys as stored.  Keys keep the positions that turned them: pass later tokens' positions to
+    ``rotary`` and ``paged_write``, whose lengths are shorter now.  Returns a ``PagedEviction``.
+    """
+    assert cache.k_pages is not None, "a cache of planes alone has no pages"
+    assert cache._writable, "pages whose elements share memory cannot be written"
+    B, max_pages, st_b = _table(cache, block_table, seq_lens)
+    _, _, Hk, _ = cache._call
+    assert new_table.dim() == 2 and new_table.shape[0] == B and new_table.dtype is torch.int32 \
+        and new_table.get_device() == cache._call[1] and new_table.shape[1] >= 1, \
+        "new_table [B, new_pages] int32 on the cache's device expected"
+    new_pages = new_table.shape[1]
+    assert new_table.stride(1) == 1 or new_pages == 1, "new_table: a row's entries must be contiguous"
+    _check_mass("mass", mass, cache, (B, Hk, PAGE * max_pages))
+    if _watched():
+        _check_unwatched(mass)
+    device = cache.device
+    kept = torch.empty((B, Hk, max(keep, 0)), dtype=torch.int32, device=device)
+    lens = torch.empty(B, dtype=torch.int32, device=device)
+    new_mass = torch.empty((B, Hk, PAGE * new_pages), dtype=torch.float32, device=device)
+    _launch(cache, "paged_evict", _capi.lib().ugbsa_paged_evict, mass.data_ptr(), *_rows(mass), seq_lens.data_ptr(),
+            block_table.data_ptr(), st_b, B, max_pages, new_table.data_ptr(), new_table.stride(0), new_pages, keep,
+            recent, first, kept.data_ptr(), lens.data_ptr(), new_mass.data_ptr(), *new_mass.stride()[:2])
+    return PagedEviction(kept, lens, new_mass)
