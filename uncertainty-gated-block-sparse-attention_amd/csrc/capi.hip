@@ -105,8 +105,10 @@ int check_pages(const ugbsa_paged_cache* c) {
     if (s < 0 || s >= int64_t{1} << 35) return fail(UGBSA_ELAYOUT, "the pages' strides must lie in [0, 2^35)");
   if (codes && (c->k_scale == nullptr || c->v_scale == nullptr))
     return fail(UGBSA_EARG, "a quantised cache needs k_scale and v_scale");
-  if (codes && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 7)
-    return fail(UGBSA_ELAYOUT, "scales must be 8-byte aligned");
+  // read 8 bytes at a time, 16 of e2m1
+  const uintptr_t low = c->cache_dtype == UGBSA_CACHE_E2M1 ? 15 : 7;
+  if (codes && (reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & low)
+    return fail(UGBSA_ELAYOUT, "scales must be 8-byte aligned, 16-byte of e2m1");
   if (!aligned16(c->planes)) return fail(UGBSA_ELAYOUT, "planes must be 16-byte aligned");
   return UGBSA_OK;
 }

@@ -32,7 +32,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef const __attribute__((address_space(1))) u32x4 gu32x4;
 typedef const __attribute__((address_space(1))) u32x2 gu32x2;
 typedef const __attribute__((address_space(1))) uint32_t gu32;
-typedef const __attribute__((address_space(1))) uint16_t gu16;
+typedef const __attribute__((address_space(1))) void gvoid;
+typedef const __attribute__((address_space(4))) int32_t cint;   // read by scalar loads where the address is uniform
 
 // A load, NT: of data read once, which need not displace other data from the caches.
 template <bool NT, typename T>

@@ -100,7 +100,7 @@ class PagedCache:
                 want = (s.num_pages, s.Hk, s.D // GROUP, PAGE) if e2m1 else (s.num_pages, s.Hk, PAGE)
                 for t in (self.k_scale, self.v_scale):
                     assert t.shape == want and t.dtype == torch.uint8 and t.is_contiguous() \
-                        and t.data_ptr() % 8 == 0, f"scales {list(want)} uint8 contiguous expected"
+                        and t.data_ptr() % (16 if e2m1 else 8) == 0, f"scales {list(want)} uint8 contiguous expected"
                 s.k_scale, s.v_scale = self.k_scale.data_ptr(), self.v_scale.data_ptr()
         if planes is not None:
             if k is None:
