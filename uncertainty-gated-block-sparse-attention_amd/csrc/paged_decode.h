@@ -1,10 +1,10 @@
 // Paged decode attention: one query row per head over the pages of its sequence,
 // all of them or those of a list per KV head (paged.h has the cache's layout).
 //
-// The products are decode.hip's: a wavefront takes 32-key steps (half pages; whole
-// pages of e2m1, which are as many bytes as half a page of e4m3) and computes S^T = K . Q^T
-// and O^T += V^T . P^T on 16x16x32 MFMAs with the KV head's query heads as the columns,
-// K and V straight from the pages into operand registers.  Codes are widened there, times their scales, which is exact in either
+// The products are decode.hip's: a wavefront takes 32-key steps (half pages) and
+// computes S^T = K . Q^T and O^T += V^T . P^T on 16x16x32 MFMAs with the KV
+// head's query heads as the columns, K and V straight from the pages into operand
+// registers (V of e2m1 through LDS).  Codes are widened there, times their scales, which is exact in either
 // 16-bit format.
 //
 // Bound by memory: 32 sequences of 64K tokens, 40/8 heads, e4m3 (4.3 GB) 698 us, 6.2
@@ -21,6 +21,7 @@
 namespace ugbsa {
 
 constexpr int kPdWaves = 4;       // wavefronts per workgroup
+constexpr int kPdStep = 32;       // keys per wavefront step: half a page
 
 // Four dims of a head, over their weights' sum; a row without a key, or whose every
 // weight is 0, gives zeros.
@@ -77,16 +78,13 @@ __device__ __forceinline__ int group_units(const PagedRows& r, int Hk, int i) {
 // Units of a row of n pages on the line.
 __device__ __forceinline__ int row_units(int n) { return n > 0 ? n + kPdRowCost : 0; }
 
-// Steps of e2m1 are whole pages (2 halves) or half ones.
-__host__ __device__ constexpr int pd_halves(int D, int one) { return D == 256 ? 1 : 2; }
-
 // Wavefronts per SIMD that the registers allow, which is also the workgroups per CU
 // that a call launches: a line cut into more than are resident leaves a second round
 // of them (us, 256 / 512 / 768 / 1024 workgroups: 24 sequences of up to 16K tokens,
 // 40/8 heads, bf16 86.1 / 78.4 / 88.1 / 80.1; 32 x 64K in e4m3 1127 / 758 / 727 / 858; 4
 // of up to 64K at 16/2 heads, head_dim 256 44.1 / 50.3 / 55.1 / 64.5).
 __host__ __device__ constexpr int pd_occupancy(int D, int kind) {
-  return D == 64 ? 4 : (D == 128 ? (kind ? 3 : 2) : (kind ? 2 : 1));
+  return D == 64 ? 4 : (D == 128 ? (kind == kPagesE4m3 ? 3 : 2) : (kind ? 2 : 1));
 }
 
 // Where a MASS call leaves its scores and rows' statistics (null otherwise).
@@ -110,8 +108,6 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
   constexpr int SZ = CODES ? 1 : 2, WAVES = ONE ? ONE : kPdWaves;   // bytes of a stride's element
   constexpr int VB = F4 ? VW / 2 : VW * SZ;      // bytes of a load of V
   constexpr int KB = F4 && D == 64 ? 8 : 16;     // and of K
-  constexpr int HS = F4 ? pd_halves(D, ONE) : 1, MT = 2 * HS, NK = 8 * HS;   // 32s of keys a step, S^T tiles, keys a lane
-  constexpr int kPdStep = 32 * HS, SPP = kBlock / kPdStep;   // keys a step, steps a page
   constexpr int KL = F4 ? D / (8 * KB) : D * SZ / (4 * KB);   // loads of a lane's share of a K row
   __shared__ float s_o[WAVES][NH][D + 4];
   __shared__ float s_ml[WAVES][NH][2];
@@ -192,21 +188,21 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
   }
 
   // MFMA row R of S^T tile mt is key 8 (R >> 2) + 4 mt + (R & 3) of the step: the lane
-  // then holds keys 8 g4 + 4 mt + i.  e2m1: key MT R + mt, and the lane holds keys
-  // NK g4 + MT i + mt, so that the scales it reads of K, and of V, lie side by side.
-  const int krow = F4 ? MT * r16 : 8 * (r16 >> 2) + (r16 & 3);
-  auto key_at = [&](int e) { return F4 ? NK * g4 + MT * (e & 3) + (e >> 2) : 8 * g4 + e; };
+  // then holds keys 8 g4 + 4 mt + i.  e2m1: key 2 R + mt, and the lane holds keys
+  // 8 g4 + 2 i + mt, so that the scales it reads of K, and of V, lie side by side.
+  const int krow = F4 ? 2 * r16 : 8 * (r16 >> 2) + (r16 & 3);
+  auto key_of = [](int e) { return F4 ? 2 * (e & 3) + (e >> 2) : e; };   // of the lane's eight
   // byte offsets of the lane's K and V rows within a step (the strides fit, checked on the host)
   uint32_t k_lane = static_cast<uint32_t>(krow * c.sk_n * SZ + KB * g4);
   uint32_t v_lane = static_cast<uint32_t>(8 * g4 * c.sv_n * SZ + VB * r16);
   // e2m1: V goes through the wavefront's share of LDS, 16 bytes a lane from memory (4 bytes
   // a lane, as the products take it, left the memory idle: the loads alone of 32 x 64K tokens
-  // 391 us, these 342).  Row NK g + k lies at place 4 k + g there, so that a read of one k
+  // 391 us, these 342).  Row 8 g + k lies at place 4 k + g there, so that a read of one k
   // by all lanes has a run of banks.
   constexpr int RB = D / 2, LPR = RB / 16, RPI = 64 / LPR, NI = kPdStep / RPI;   // bytes and lanes a row, rows and loads
   char* const v_lds = reinterpret_cast<char*>(&s_o[wave][0][0]);
   static_assert(!F4 || kPdStep * RB <= NH * (D + 4) * 4, "V of a step fits the wavefront's share");
-  if constexpr (F4) v_lane = static_cast<uint32_t>((NK * (lane / LPR % 4) + lane / LPR / 4) * c.sv_n + 16 * (lane % LPR));
+  if constexpr (F4) v_lane = static_cast<uint32_t>((8 * (lane / LPR % 4) + lane / LPR / 4) * c.sv_n + 16 * (lane % LPR));
   const uint32_t k_row = static_cast<uint32_t>(c.sk_n * SZ), v_row = static_cast<uint32_t>(c.sv_n * SZ);
 
   for (;;) {
@@ -249,7 +245,7 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
     // flight need not drain for.
     struct Step { int64_t page; int base, left; };
     auto block_at = [&](int st) {
-      const int x = st / SPP;
+      const int x = st >> 1;
       if constexpr (F4) return list == nullptr ? x : ((cint*)list)[x];
       else return list == nullptr ? x : list[x];
     };
@@ -268,7 +264,7 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       const bool there = page >= 0 && page < c.num_pages;
       Step s;
       s.page = there ? page : 0;             // an absent page: page 0's keys, none of them live
-      s.base = kPdStep * (st % SPP);
+      s.base = kPdStep * (st & 1);
       s.left = there ? len - blk * kBlock - s.base : 0;
       return s;
     };
@@ -277,16 +273,16 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       return step_of(st, blk, entry_at(blk));
     };
 
-    u32x4 kf[MT][KL];
-    uint32_t kby[F4 ? KL : 1];               // e2m1: the scales of the lane's four keys, a byte each
+    u32x4 kf[2][KL];
+    uint32_t kby[F4 ? KL : 1];               // e2m1: the scales of the lane's two keys, a byte each
     float ksc[2], vsc[8];
-    uint32_t vby[NK / 4], vcur[NK / 4];      // and of the NK keys it reads of V: the next step's, this one's
+    u32x2 vby, vcur;                         // and of the eight keys it reads of V: the next step's, this one's
     constexpr int VR = VB * VL < 4 ? 1 : VB * VL / 4;
-    uint32_t vr[NK][VR];                     // V[key_at(e)][the lane's dims]
+    uint32_t vr[8][VR];                      // V[8 g4 + key_of(e)][the lane's dims]
     auto load_k = [&](const Step& s) {
       gchar* half = kg + s.page * c.sk_p * SZ + static_cast<uint32_t>(s.base) * k_row;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int mt = 0; mt < 2; ++mt) {
         gchar* row = half + (F4 ? 1u : 4u) * mt * k_row;
 #pragma unroll
         for (int j = 0; j < KL; ++j) {
@@ -301,22 +297,17 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
           ksc[mt] = e8m0(c.k_scale[(s.page * gr.Hk + g) * kBlock + s.base + krow + 4 * mt]);
       }
       if constexpr (F4) {
-        using Bytes = std::conditional_t<MT == 4, uint32_t, uint16_t>;
         const uint8_t* at = c.k_scale + (s.page * gr.Hk + g) * (D / 32 * kBlock) + s.base + krow;
 #pragma unroll
         for (int j = 0; j < KL; ++j)
-          kby[j] = *reinterpret_cast<const Bytes*>(at + (D == 64 ? g4 >> 1 : 4 * j + g4) * kBlock);
+          kby[j] = *reinterpret_cast<const uint16_t*>(at + (D == 64 ? g4 >> 1 : 4 * j + g4) * kBlock);
       }
     };
     auto load_v = [&](const Step& s) {
       gchar* half = vg + s.page * c.sv_p * SZ + static_cast<uint32_t>(s.base) * v_row;
-      if constexpr (F4) {
-        typedef uint32_t Bytes __attribute__((ext_vector_type(NK / 4)));
-        const Bytes x = *reinterpret_cast<const Bytes*>(
-            c.v_scale + ((s.page * gr.Hk + g) * (D / 32) + DPL * r16 / 32) * kBlock + s.base + NK * g4);
-#pragma unroll
-        for (int j = 0; j < NK / 4; ++j) vby[j] = x[j];
-      }
+      if constexpr (F4)
+        vby = *reinterpret_cast<const u32x2*>(
+            c.v_scale + ((s.page * gr.Hk + g) * (D / 32) + DPL * r16 / 32) * kBlock + s.base + 8 * g4);
       if constexpr (F8) {
         const u32x2 bytes =
             *reinterpret_cast<const u32x2*>(c.v_scale + (s.page * gr.Hk + g) * kBlock + s.base + 8 * g4);
@@ -355,8 +346,8 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;  // of head r16; l over this lane's keys
 
-    const int st1 = SPP * p1;
-    int st = SPP * p0 + wave;
+    const int st1 = 2 * p1;
+    int st = 2 * p0 + wave;
     Step cur{}, nxt{}, far{};
     if (st < st1) {
       cur = step_at(st);
@@ -376,13 +367,11 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       } else {
         if (st + 2 * WAVES < st1) far = step_at(st + 2 * WAVES);
       }
-      f32x4 s[MT];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < 2; ++mt) {
           bf16x8 a;
           if constexpr (F8)
             a = e4m3_x8<E>(kf[mt][ks / 2][2 * (ks % 2)], kf[mt][ks / 2][2 * (ks % 2) + 1], ksc[mt]);
@@ -396,8 +385,8 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
         // V out of LDS, then the next step's K and V into registers and LDS
         const char* at = v_lds + RB * g4 + VB * r16;
 #pragma unroll
-        for (int e = 0; e < NK; ++e) {
-          const char* row = at + 4 * RB * (MT * (e & 3) + (e >> 2));
+        for (int e = 0; e < 8; ++e) {
+          const char* row = at + 4 * RB * key_of(e);
           if constexpr (VB == 8) {
             const u32x2 y = *reinterpret_cast<const u32x2*>(row);
             vr[e][0] = y[0], vr[e][1] = y[1];
@@ -407,25 +396,24 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
             vr[e][0] = *reinterpret_cast<const uint16_t*>(row);
           }
         }
-#pragma unroll
-        for (int j = 0; j < NK / 4; ++j) vcur[j] = vby[j];
+        vcur = vby;
         asm volatile("" ::: "memory");
         wait_lds_reads();
         asm volatile("" ::: "memory");
       }
       if (more) load_k(nxt);
       if (F4 && more) load_v(nxt);
-      float x[NK];
+      float x[8];
 #pragma unroll
-      for (int e = 0; e < NK; ++e) x[e] = s[e >> 2][e & 3] * scale_log2;
+      for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * scale_log2;
       if (cur.left < kPdStep) {     // keys past the end, or an absent page
 #pragma unroll
-        for (int e = 0; e < NK; ++e)
-          if (key_at(e) >= cur.left) {
+        for (int e = 0; e < 8; ++e)
+          if (8 * g4 + key_of(e) >= cur.left) {
             x[e] = -INFINITY;
             if constexpr (F8) vsc[e] = 1.f;
             if constexpr (F4) {
-              const int k = MT * (e & 3) + (e >> 2), sh = 8 * (k & 3);
+              const int k = key_of(e), sh = 8 * (k & 3);
               vcur[k >> 2] = (vcur[k >> 2] & ~(0xFFu << sh)) | 127u << sh;
             }
 #pragma unroll
@@ -434,32 +422,29 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       }
       if constexpr (MASS) {
         if (r16 < heads) {
-          float* to = sc.x + ((static_cast<int64_t>(b) * gr.Hk * grp + h0 + r16) * sc.units + st / SPP) * kBlock +
-                      kPdStep * (st % SPP) + NK * g4;
+          float* to = sc.x + ((static_cast<int64_t>(b) * gr.Hk * grp + h0 + r16) * sc.units + (st >> 1)) * kBlock +
+                      kPdStep * (st & 1) + 8 * g4;
 #pragma unroll
-          for (int j = 0; j < NK / 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
             f32x4 y;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = 4 * j + i;           // the lane's k-th key in order
-              y[i] = x[F4 ? 4 * (k % MT) + k / MT : k];
-            }
+            for (int i = 0; i < 4; ++i) y[i] = x[F4 ? 4 * (i & 1) + 2 * j + (i >> 1) : 4 * j + i];   // keys 4 j + i
             *reinterpret_cast<f32x4*>(to + 4 * j) = y;
           }
         }
       }
       float mx = x[0];
 #pragma unroll
-      for (int e = 1; e < NK; ++e) mx = fmaxf(mx, x[e]);
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
       const float m_new = fmaxf(m, quad_rows_max(mx));
       const float off = m_new == -INFINITY ? 0.f : m_new;   // no finite score so far: weights 0
       const float alpha = __builtin_amdgcn_exp2f(m - off);
       // O moves with the maximum; after a row's first pages it hardly does
       const bool moved = !F4 || __ballot(m_new != m) != 0;
       m = m_new;
-      float p[NK], sum = 0.f;
+      float p[8], sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < NK; ++e) {
+      for (int e = 0; e < 8; ++e) {
         p[e] = __builtin_amdgcn_exp2f(x[e] - off);
         sum += p[e];
       }
@@ -467,43 +452,35 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       if (moved)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      // P rounded once to the element format, as the other attention kernels do
+      u32x4 pw;
 #pragma unroll
-      for (int hs = 0; hs < HS; ++hs) {
-        // P rounded once to the element format, as the other attention kernels do
-        u32x4 pw;
+      for (int j = 0; j < 4; ++j) pw[j] = E::pack2(p[2 * j], p[2 * j + 1]);
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
+      if constexpr (F4)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pw[j] = E::pack2(p[8 * hs + 2 * j], p[8 * hs + 2 * j + 1]);
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
-        float fsc[8];
-        if constexpr (F4)
+        for (int e = 0; e < 8; ++e) vsc[e] = scale_of(vcur[key_of(e) >> 2], key_of(e) & 3);
+      // operand dt: the lane's dim dt of the eight keys
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int k = MT * (i & 3) + 2 * hs + (i >> 2);
-            fsc[i] = scale_of(vcur[k >> 2], k & 3);
-          }
-        // operand dt: the lane's dim dt of the eight keys
+      for (int d2 = 0; d2 < DT / 2; ++d2) {
+        uint32_t w[8];
 #pragma unroll
-        for (int d2 = 0; d2 < DT / 2; ++d2) {
-          uint32_t w[8];
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (F8) w[i] = e4m3_pair<E>(vr[i][d2 / 2], vsc[i], d2 % 2);
+          else if constexpr (F4)
+            w[i] = d2 % 4 == 0   ? e2m1_pair<E, 0>(vr[i][d2 / 4], vsc[i])
+                   : d2 % 4 == 1 ? e2m1_pair<E, 1>(vr[i][d2 / 4], vsc[i])
+                   : d2 % 4 == 2 ? e2m1_pair<E, 2>(vr[i][d2 / 4], vsc[i])
+                                 : e2m1_pair<E, 3>(vr[i][d2 / 4], vsc[i]);
+          else w[i] = vr[i][d2];
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t* v = vr[8 * hs + i];
-            if constexpr (F8) w[i] = e4m3_pair<E>(v[d2 / 2], vsc[i], d2 % 2);
-            else if constexpr (F4)
-              w[i] = d2 % 4 == 0   ? e2m1_pair<E, 0>(v[d2 / 4], fsc[i])
-                     : d2 % 4 == 1 ? e2m1_pair<E, 1>(v[d2 / 4], fsc[i])
-                     : d2 % 4 == 2 ? e2m1_pair<E, 2>(v[d2 / 4], fsc[i])
-                                   : e2m1_pair<E, 3>(v[d2 / 4], fsc[i]);
-            else w[i] = v[d2];
-          }
+        for (int odd = 0; odd < 2; ++odd) {
+          u32x4 a;
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
-            u32x4 a;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              a[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], odd ? 0x07060302u : 0x05040100u);
-            o[2 * d2 + odd] = E::mfma(__builtin_bit_cast(bf16x8, a), pb, o[2 * d2 + odd]);
-          }
+          for (int j = 0; j < 4; ++j)
+            a[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], odd ? 0x07060302u : 0x05040100u);
+          o[2 * d2 + odd] = E::mfma(__builtin_bit_cast(bf16x8, a), pb, o[2 * d2 + odd]);
         }
       }
       if (!F4 && more) load_v(nxt);
@@ -721,7 +698,7 @@ hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& rows, con
   // 72); smaller calls may find theirs in it (4 of up to 64K, head_dim 256, 41.1 and
   // 42.2).  The table's width bounds the lengths, which are on the device.
   const int64_t most = static_cast<int64_t>(B) * c.Hk * units * paged_bytes(D, KIND);
-  const auto kernel = most > 768ll << 20 ? paged_decode_kernel<E, D, KIND, true, 0, MASS>
+  const auto kernel = most > (KIND == kPagesE2m1 ? 384ll : 768ll) << 20 ? paged_decode_kernel<E, D, KIND, true, 0, MASS>
                                          : paged_decode_kernel<E, D, KIND, false, 0, MASS>;
   kernel<<<dim3(wgs), 64 * kPdWaves, 0, stream>>>(c, rows, gr, q, sq_b, sq_h, grp, chunks, scale * kLog2e, out,
                                                   so_b, so_h, starts, part, ml, sc);
