@@ -10,125 +10,333 @@ namespace ugbsa {
 
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
 constexpr int kPickBins = 2048;        // 11, 11 and 10 bits of the key
+constexpr int kPickList = 4096;        // keys of the cut's bin that are listed
 
-// Order of a row's tokens, larger first: tokens that stay whatever they weigh, NaN, then
-// by weight (zeros of either sign alike); 0: the page is absent, the token is not kept.
-struct PickRow {
-  const float* mass;
-  const int32_t* table;
-  int n, first, last, num_pages;       // tokens below first or from last on stay
-  __device__ __forceinline__ uint32_t key(int i, float x) const {
-    const int page = table[i / kBlock];
-    if (i >= n || page < 0 || page >= num_pages) return 0u;
-    if (i < first || i >= last) return 0xFFFFFFFFu;
-    return x != x ? 0xFFFFFFFEu : float_key(x + 0.f);
-  }
-  // keys of tokens i .. i + 3 (i a multiple of 4, below n)
-  __device__ __forceinline__ void keys4(int i, uint32_t* to) const {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(mass + i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) to[j] = key(i + j, x[j]);
-  }
-};
+// Order of the tokens that compete, larger first: NaN, then by weight, zeros of either
+// sign alike.
+constexpr uint32_t kPickNan = 0xFFFFFFFEu, kPickInf = 0xFF800000u;
+__device__ __forceinline__ uint32_t pick_key(float x) { return x != x ? kPickNan : float_key(x + 0.f); }
 
-// One workgroup per (KV head, sequence).  The k-th largest key by three digits, then each
-// wavefront counts what it keeps of its share of the row and writes it behind the others'.
+// One workgroup per (KV head, sequence).  The first tokens and the newest stay; of the
+// others, c0 .. c1 - 1, the `want` largest do: a histogram of their keys' top digit, then of
+// the lower ones over the keys of the cut's bin, which are listed in LDS where it holds
+// them, fewer digits where the cut falls between two bins.  Then each wavefront goes over a
+// run of the row's pages, a token a lane, counts what it keeps and writes it behind the
+// others'.
+//
+// A row is one CU's, and its instructions bound it: how many (a pass over 32K tokens at 40
+// of them per 64 tokens took 8.6 us), and that they are fetched (loops unrolled over loads
+// in flight are code that runs once).  So rows of up to ROW tokens are copied to LDS and
+// gone over by small loops; four tokens a lane and load; membership in a bin, and in what
+// stays, by comparing weights with its ends, not keys; what is the same for all lanes in
+// scalar registers; and what only some tokens need (ends of the range, absent pages, NaN)
+// behind scalar branches.
+//
+// 64 rows of up to 32K tokens (2.6 MB) XX us; one of 600 XX.
+template <int ROW>
 __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     const float* __restrict__ mass, int64_t sm_b, int64_t sm_h, const int32_t* __restrict__ lens,
     const int32_t* __restrict__ table, int64_t st_b, int max_pages, int num_pages, int keep, int recent, int first,
     int32_t* __restrict__ kept, int32_t* __restrict__ new_lens) {
-  __shared__ uint32_t s_hist[kPickBins], s_wave[2][kPickWaves], s_found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x, b = blockIdx.y;
+  __shared__ uint32_t s_hist[kPickBins], s_list[kPickList], s_wave[2][kPickWaves], s_found[3], s_listed, s_stay;
+  __shared__ uint8_t s_from[kPickList];
+  __shared__ f32x4 s_row[ROW > 0 ? ROW / 4 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = blockIdx.x, b = blockIdx.y;
   const int n = cached_len(lens, b, max_pages);
-  const PickRow row{mass + b * sm_b + g * sm_h, table + b * st_b, n, first, max(n - recent, 0), num_pages};
+  const int c0 = min(first, n), c1 = max(n - recent, c0);
+  mass += b * sm_b + g * sm_h;
+  table += b * st_b;
   int32_t* out = kept + (static_cast<int64_t>(b) * gridDim.x + g) * keep;
 
-  uint32_t prefix = 0u, mask = 0u, want = keep;      // want-th largest among the keys of the prefix
+  const int pages = (n + kBlock - 1) / kBlock;
+  auto there = [&](int page) { return page >= 0 && page < num_pages; };
+  if constexpr (ROW > 0) {
+    for (int i = 4 * tid; i < n; i += 16 * kPickThreads) {
+      f32x4 x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x[r] = *reinterpret_cast<const f32x4*>(mass + min(i + 4 * kPickThreads * r, (n - 1) & ~3));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (i + 4 * kPickThreads * r < n) s_row[i / 4 + kPickThreads * r] = x[r];
+    }
+  }
+  bool gap = false;                                   // a page of the row is absent
+  for (int p = tid; p < pages; p += kPickThreads) gap |= !there(table[p]);
+  for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0u;
+  if (tid == 0) s_listed = 0u, s_stay = 0u;
+  const bool absent = __builtin_amdgcn_readfirstlane(__syncthreads_or(gap)) != 0;
+
+  // four weights from token i on (the row's last four where it ends before)
+  constexpr int RUN = ROW > 0 ? 1 : 4;                // loads in flight together
+  auto weights = [&](int i) __attribute__((always_inline)) {
+    const int at = min(i, (n - 1) & ~3);
+    if constexpr (ROW > 0) return s_row[at / 4];
+    else return *reinterpret_cast<const f32x4*>(mass + at);
+  };
+  // f(four weights of the lane, masks of the lanes whose j-th competes, whether all do), 256 tokens a time
+  auto visit = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int w0 = (c0 & ~3) + 256 * wave; w0 < c1; w0 += 4 * RUN * kPickThreads) {
+      f32x4 x[RUN];
+#pragma unroll
+      for (int r = 0; r < RUN; ++r) x[r] = weights(w0 + 4 * kPickThreads * r + 4 * lane);
+#pragma unroll
+      for (int r = 0; r < RUN; ++r) {
+        const int i0 = w0 + 4 * kPickThreads * r, i = i0 + 4 * lane;
+        if (i0 >= c1) break;
+        uint64_t in[4] = {~0ull, ~0ull, ~0ull, ~0ull};
+        const bool all = i0 >= c0 && i0 + 256 <= c1 && !absent;
+        if (!all) {
+          const bool page = i < n && there(table[i / kBlock]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) in[j] = __ballot(page && i + j >= c0 && i + j < c1);
+        }
+        f(x[r], in, all);
+      }
+    }
+  };
+  auto mine = [&](uint64_t m) { return (m >> lane & 1) != 0; };
+  // f(first of 256 tokens, the lane's first, its four weights) over this wavefront's part of the row
+  const int runs = (n + 255) / 256, share = (runs + kPickWaves - 1) / kPickWaves;
+  const int q0 = min(wave * share, runs), q1 = min(q0 + share, runs);
+  auto run_over = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int at = q0; at < q1; at += RUN) {
+      f32x4 x[RUN];
+#pragma unroll
+      for (int r = 0; r < RUN; ++r) x[r] = weights(256 * (at + r) + 4 * lane);
+#pragma unroll
+      for (int r = 0; r < RUN; ++r) {
+        if (at + r >= q1) break;
+        f(256 * (at + r), 256 * (at + r) + 4 * lane, x[r]);
+      }
+    }
+  };
+  int more = 0, same = 0;                             // of this lane's: above the cut, and tied
+
+  uint32_t prefix = 0u, mask = 0u, want = 0u;        // want-th largest among the keys of the prefix
+  uint32_t least = 0u, ties = 0u;                     // keys above least stay, and the first ties equal to it
+  uint32_t top = 0u;                                  // keys of the cut's bin of the top digit
   int total = 0;                                      // tokens with a page
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0u;
-    __syncthreads();
-    for (int i = 4 * tid; i < n; i += 4 * kPickThreads) {
-      uint32_t k[4];
-      row.keys4(i, k);
+    if (pass == 0) {
+      if (absent) {                                   // those that stay and are there
+        uint32_t stay = 0u;
+        for (int i = tid; i < n - (c1 - c0); i += kPickThreads) {
+          const int t = i < c0 ? i : i + (c1 - c0);
+          stay += there(table[t / kBlock]) ? 1u : 0u;
+        }
+        if (stay != 0u) atomicAdd(&s_stay, stay);
+      }
+      visit([&](f32x4 x, const uint64_t* in, bool all) __attribute__((always_inline)) {
+        // the bits' top digit, which the scan below puts in order: -0 as 0, NaN as the top bin
+        uint32_t d[4];
+        const float any = x[0] + x[1] + x[2] + x[3];
+        const bool nan = __ballot(any != any) != 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j < n && (k[j] & mask) == prefix) atomicAdd(&s_hist[(k[j] >> shift) & (bins - 1)], 1u);
+        for (int j = 0; j < 4; ++j) {
+          d[j] = __float_as_uint(x[j] + 0.f) >> 21;
+          if (nan && x[j] != x[j]) d[j] = 0x3FFu;
+        }
+        // one bin for all of them, as of tokens that were never looked at: one addition
+        const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
+        if (all) {
+          if (__ballot(d[0] != d0) == 0 && __ballot(d[1] != d0 || d[2] != d0 || d[3] != d0) == 0) {
+            if (lane == 0) atomicAdd(&s_hist[d0], 256u);
+            return;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) atomicAdd(&s_hist[d[j]], 1u);
+          return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (mine(in[j])) atomicAdd(&s_hist[d[j]], 1u);
+      });
+    } else if (top <= kPickList) {
+      const uint32_t listed = min(s_listed, static_cast<uint32_t>(kPickList));
+      for (uint32_t i = tid; i < listed; i += kPickThreads) {
+        const uint32_t k = s_list[i];
+        if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+      }
+    } else {
+      visit([&](f32x4 x, const uint64_t* in, bool) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t k = pick_key(x[j]);
+          if (mine(in[j]) && (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+        }
+      });
     }
     __syncthreads();
-    // bins from the largest: thread t holds bins - 1 - 2 t and the one below it
+    // bins from the largest: thread t holds bins - 1 - 2 t and the one below it; the bits of
+    // a positive weight's key are its own but for the sign, those of a negative one's turned
     const int hi = bins - 1 - 2 * tid;
-    const uint32_t c0 = hi >= 0 ? s_hist[hi] : 0u, c1 = hi >= 1 ? s_hist[hi - 1] : 0u;
-    const uint32_t ex = wave_excl_scan(c0 + c1, lane);
-    if (lane == 63) s_wave[0][wave] = ex + c0 + c1;
+    auto held = [&](int bin) { return pass > 0 ? bin : (bin >= 1024 ? bin - 1024 : 2047 - bin); };
+    const uint32_t h0 = hi >= 0 ? s_hist[held(hi)] : 0u, h1 = hi >= 1 ? s_hist[held(hi - 1)] : 0u;
+    const uint32_t ex = wave_excl_scan(h0 + h1, lane);
+    if (lane == 63) s_wave[0][wave] = ex + h0 + h1;
     __syncthreads();
     uint32_t before = ex;
     for (int w = 0; w < wave; ++w) before += s_wave[0][w];
     if (pass == 0) {
+      const int stay = absent ? __builtin_amdgcn_readfirstlane(s_stay) : n - (c1 - c0);
       uint32_t all = 0u;
       for (int w = 0; w < kPickWaves; ++w) all += s_wave[0][w];
-      // the keys of tokens with a page lie above 0x007F0000: the lowest bin holds the absent ones
-      total = static_cast<int>(all - s_hist[0]);
-      if (total <= keep) break;                       // all of them stay
+      total = stay + __builtin_amdgcn_readfirstlane(all);
+      want = keep - stay;
+      if (total <= keep || want == 0u) break;         // all that compete stay, or none
     }
-    if (before < want && want <= before + c0) s_found[0] = hi, s_found[1] = before;
-    else if (before + c0 < want && want <= before + c0 + c1) s_found[0] = hi - 1, s_found[1] = before + c0;
+    if (before < want && want <= before + h0) s_found[0] = hi, s_found[1] = before, s_found[2] = h0;
+    else if (before + h0 < want && want <= before + h0 + h1) s_found[0] = hi - 1, s_found[1] = before + h0, s_found[2] = h1;
+    for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0u;
     __syncthreads();
-    prefix |= s_found[0] << shift;
+    prefix |= static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(s_found[0])) << shift;
     mask |= static_cast<uint32_t>(bins - 1) << shift;
-    want -= s_found[1];
+    want -= __builtin_amdgcn_readfirstlane(s_found[1]);
+    const uint32_t bin = __builtin_amdgcn_readfirstlane(s_found[2]);
+    least = prefix, ties = want;
+    if (want == bin) {                                // the whole bin stays
+      least = prefix - 1u, ties = 0u;
+      break;
+    }
+    if (pass == 0) {
+      top = bin;
+      // the bin's keys, and what each wavefront holds above the bin
+      const bool finite = prefix >= ~kPickInf && prefix < kPickInf, fits = top <= kPickList;
+      const float lo = key_float(prefix), end = key_float(prefix + (1u << 21));
+      run_over([&](int i0, int i, f32x4 x) __attribute__((always_inline)) {
+        bool over[4], in[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          over[j] = !(x[j] < end);                            // finite: or NaN
+          in[j] = x[j] >= lo && x[j] < end;
+        }
+        if (!finite) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t k = pick_key(x[j]);
+            over[j] = (k & mask) > prefix, in[j] = (k & mask) == prefix;
+          }
+        }
+        if (absent || i0 < c0 || i0 + 256 > c1) {             // not all of them compete, or are there
+          const bool page = i < n && there(table[i / kBlock]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool have = page && i + j < n, mid = i + j >= c0 && i + j < c1;
+            over[j] = have && (over[j] || !mid);
+            in[j] = in[j] && have && mid;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) more += over[j] ? 1 : 0;
+        if (!fits || __ballot(in[0] || in[1] || in[2] || in[3]) == 0) return;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (in[j]) {
+            const uint32_t to = atomicAdd(&s_listed, 1u) % kPickList;
+            s_list[to] = pick_key(x[j]);
+            s_from[to] = static_cast<uint8_t>(wave);
+          }
+      });
+    }
     __syncthreads();
   }
-  // keys above the threshold stay, and the first `ties` equal to it
-  const bool all = total <= keep;
-  const uint32_t least = all ? 0u : prefix, ties = all ? 0u : want;
-  const int count = all ? total : keep;
+  const int count = min(total, keep);
   if (tid == 0 && g == 0) new_lens[b] = count;
+  if (total > keep && want == 0u && ties == 0u && least == 0u) least = 0xFFFFFFFFu;   // none that compete
   __syncthreads();
 
-  const int share = ((n + kPickWaves - 1) / kPickWaves + 255) / 256 * 256;
-  const int i0 = wave * share, i1 = min(i0 + share, n);
-  uint32_t above = 0u, equal = 0u;
-  for (int i = i0 + 4 * lane; i < i1; i += 256) {
-    uint32_t k[4];
-    row.keys4(i, k);
+  // In weights: keys above least are those not below `low`, or only NaN, or none; equal to it
+  // those equal to `tie`, or NaN.
+  const bool none = least >= kPickNan, only_nan = !none && least + 1u > kPickInf;
+  const float low = total <= keep ? __uint_as_float(0x7FC00000u) : key_float(least + 1u), tie = key_float(least);
+  const bool plain = !none && !only_nan && !absent;
+  // f(the lane's first token, masks of the lanes whose j-th stays above the cut, and ties)
+  auto pass_over = [&](auto f) __attribute__((always_inline)) {
+    run_over([&](int i0, int i, f32x4 x) __attribute__((always_inline)) {
+      uint64_t gt[4], eq[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) above += k[j] > least ? 1u : 0u, equal += k[j] == least && i + j < n ? 1u : 0u;
+      for (int j = 0; j < 4; ++j) {
+        gt[j] = __ballot(!(x[j] < low));
+        eq[j] = ties != 0u ? __ballot(x[j] == tie) : 0;
+      }
+      if (!plain) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t nan = __ballot(x[j] != x[j]);
+          gt[j] = none ? 0 : (only_nan ? nan : gt[j]);
+          eq[j] = ties != 0u && least == kPickNan ? nan : eq[j];
+        }
+      }
+      if (absent || i0 < c0 || i0 + 256 > c1) {             // not all of them compete, or are there
+        const bool page = i < n && there(table[i / kBlock]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t have = __ballot(page && i + j < n), in = __ballot(i + j >= c0 && i + j < c1);
+          gt[j] = have & (gt[j] | ~in);
+          eq[j] &= have & in;
+        }
+      }
+      f(i, gt, eq);
+    });
+  };
+  // what the wavefront keeps: from the list where there is one
+  if (total > keep && top != 0u && top <= kPickList) {
+    const uint32_t listed = min(s_listed, static_cast<uint32_t>(kPickList));
+    for (uint32_t at = 0; at < listed; at += 64) {
+      const bool own = at + lane < listed && s_from[min(at + lane, listed - 1u)] == wave;
+      const uint32_t k = s_list[min(at + lane, listed - 1u)];
+      more += own && k > least ? 1 : 0;
+      same += own && k == least ? 1 : 0;
+    }
+  } else {
+    more = 0;
+    pass_over([&](int, const uint64_t* gt, const uint64_t* eq) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        more += mine(gt[j]) ? 1 : 0;
+        same += mine(eq[j]) ? 1 : 0;
+      }
+    });
   }
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) above += shfl_xor_u(above, off), equal += shfl_xor_u(equal, off);
-  if (lane == 0) s_wave[0][wave] = above, s_wave[1][wave] = equal;
+  for (int off = 32; off >= 1; off >>= 1) more += __shfl_xor(more, off, 64), same += __shfl_xor(same, off, 64);
+  if (lane == 0) s_wave[0][wave] = more, s_wave[1][wave] = same;
   __syncthreads();
-  uint32_t at = 0u, tied = 0u;                        // kept and tied tokens of the wavefronts before
+  int at = 0, tied = 0;                               // kept and tied tokens of the wavefronts before
   for (int w = 0; w < wave; ++w) at += s_wave[0][w], tied += s_wave[1][w];
-  at += min(tied, ties);
-  for (int base = i0; base < i1; base += 256) {
-    const int i = base + 4 * lane;
-    uint32_t k[4] = {0u, 0u, 0u, 0u};
-    if (i < i1) row.keys4(i, k);
-    uint32_t eq = 0u;
+  at = __builtin_amdgcn_readfirstlane(at + min(tied, static_cast<int>(ties)));
+  tied = __builtin_amdgcn_readfirstlane(tied);
+  pass_over([&](int i, const uint64_t* gt, const uint64_t* eq) __attribute__((always_inline)) {
+    uint64_t stay[4] = {gt[0], gt[1], gt[2], gt[3]};
+    if (ties != 0u && tied < static_cast<int>(ties) && (eq[0] | eq[1] | eq[2] | eq[3]) != 0) {
+      // the first `ties` of the row
+      int rank = tied;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) eq += i + j < n && k[j] == least ? 1u : 0u;
-    const uint32_t eq_before = wave_excl_scan(eq, lane);
-    uint32_t t = tied + eq_before, mine = 0u;
-    bool stay[4];
+      for (int j = 0; j < 4; ++j) rank += lanes_below(eq[j]), tied += __builtin_popcountll(eq[j]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool tie = i + j < n && k[j] == least;
-      stay[j] = k[j] > least || (tie && t < ties);
-      t += tie ? 1u : 0u;
-      mine += stay[j] ? 1u : 0u;
+      for (int j = 0; j < 4; ++j) {
+        stay[j] |= __ballot(mine(eq[j]) && rank < static_cast<int>(ties));
+        rank += mine(eq[j]) ? 1 : 0;
+      }
     }
-    uint32_t to = at + wave_excl_scan(mine, lane);
+    if ((stay[0] | stay[1] | stay[2] | stay[3]) == 0) return;
+    int to = at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to += lanes_below(stay[j]), at += __builtin_popcountll(stay[j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (stay[j]) out[to++] = i + j;
-    at = __builtin_amdgcn_readlane(to, 63);
-    tied += __builtin_amdgcn_readlane(eq_before + eq, 63);
-  }
-  const int none = max_pages * kBlock;
-  for (int i = count + tid; i < keep; i += kPickThreads) out[i] = none;
+      if (mine(stay[j])) {
+        if (to < count) out[to] = i + j;
+        ++to;
+      }
+  });
+  const int end = max_pages * kBlock;
+  for (int i = count + tid; i < keep; i += kPickThreads) out[i] = end;
 }
 
 // One workgroup per (new page, KV head, sequence): it alone writes them.  A thread moves 8
@@ -136,22 +344,25 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
 template <typename E, int D, int KIND>
 __global__ __launch_bounds__(256) void paged_move_kernel(
     PagedCache c, const float* __restrict__ mass, int64_t sm_b, int64_t sm_h, const int32_t* __restrict__ table,
-    int64_t st_b, const int32_t* __restrict__ new_table, int64_t sn_b, const int32_t* __restrict__ kept, int keep,
-    const int32_t* __restrict__ new_lens, float* __restrict__ new_mass, int64_t so_b, int64_t so_h) {
-  constexpr int CH = D / 8, RG = 256 / CH;
+    int64_t st_b, int tokens, const int32_t* __restrict__ new_table, int64_t sn_b, const int32_t* __restrict__ kept,
+    int keep, const int32_t* __restrict__ new_lens, float* __restrict__ new_mass, int64_t so_b, int64_t so_h) {
+  constexpr int CH = D / 8, RG = 256 / CH, IT = kBlock / RG;
   __shared__ float red[2][RG][D + 1];
-  __shared__ int s_token[kBlock];
+  __shared__ int s_slot[kBlock], s_page[kBlock];
   const int tid = threadIdx.x, ch = tid % CH, rg = tid / CH;
   const int j = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int count = min(new_lens[b] - j * kBlock, kBlock);        // tokens of this page
   if (tid < kBlock) {
-    int token = -1;
     float x = 0.f;
     if (tid < count) {
-      token = kept[(static_cast<int64_t>(b) * gridDim.y + h) * keep + j * kBlock + tid];
+      // (in range, and with a page, unless mass changed while the call ran)
+      int token = kept[(static_cast<int64_t>(b) * gridDim.y + h) * keep + j * kBlock + tid];
+      token = token < 0 || token >= tokens ? 0 : token;
+      const int from = table[b * st_b + token / kBlock];
+      s_slot[tid] = token % kBlock;
+      s_page[tid] = from >= 0 && from < c.num_pages ? from : 0;
       x = mass[b * sm_b + h * sm_h + token];
     }
-    s_token[tid] = token;
     new_mass[b * so_b + h * so_h + j * kBlock + tid] = x;
   }
   if (count <= 0) return;
@@ -166,40 +377,55 @@ __global__ __launch_bounds__(256) void paged_move_kernel(
   typedef uint32_t words __attribute__((ext_vector_type(W)));
   constexpr int CB = 4 * W / (KIND == kPagesModel ? 2 : 1);                     // elements of a stride
   using Elem = std::conditional_t<KIND == kPagesModel, uint16_t, uint8_t>;
-  for (int s = rg; s < count; s += RG) {
-    const int token = s_token[s], from = table[b * st_b + token / kBlock], slot = token % kBlock;
-    const int64_t src_head = static_cast<int64_t>(from) * c.Hk + h;
+  Elem* const kp = static_cast<Elem*>(c.k) + h * c.sk_h + CB * ch;
+  Elem* const vp = static_cast<Elem*>(c.v) + h * c.sv_h + CB * ch;
+  // scales: one a token of e4m3, one a token and 32 dims of e2m1
+  const int64_t groups = KIND == kPagesE2m1 ? D / 32 : 1;
+  const int grp = KIND == kPagesE2m1 ? ch / 4 : 0;
+  const bool holds = KIND == kPagesE2m1 ? ch % 4 == 0 : ch == 0;
+  // all of the page's loads, then its stores
+  words rk[IT], rv[IT];
+  uint32_t bk[IT], bv[IT];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      Elem* pages = static_cast<Elem*>(kv ? c.v : c.k);
-      const int64_t sp = kv ? c.sv_p : c.sk_p, sh = h * (kv ? c.sv_h : c.sk_h) + CB * ch, sn = kv ? c.sv_n : c.sk_n;
-      const words raw = *reinterpret_cast<const words*>(pages + from * sp + sh + slot * sn);
-      *reinterpret_cast<words*>(pages + page * sp + sh + s * sn) = raw;
-      uint8_t* scales = kv ? c.v_scale : c.k_scale;
-      uint32_t byte = 127u;
-      if constexpr (KIND == kPagesE4m3) {
-        byte = scales[src_head * kBlock + slot];
-        if (ch == 0) scales[head * kBlock + s] = static_cast<uint8_t>(byte);
+  for (int it = 0; it < IT; ++it) {
+    const int s = rg + RG * it;
+    if (s < count) {
+      const int64_t from = s_page[s];
+      const int slot = s_slot[s];
+      rk[it] = *reinterpret_cast<const words*>(kp + from * c.sk_p + slot * c.sk_n);
+      rv[it] = *reinterpret_cast<const words*>(vp + from * c.sv_p + slot * c.sv_n);
+      if constexpr (KIND != kPagesModel) {
+        const int64_t at = ((from * c.Hk + h) * groups + grp) * kBlock + slot;
+        bk[it] = c.k_scale[at];
+        bv[it] = c.v_scale[at];
       }
-      if constexpr (KIND == kPagesE2m1) {
-        byte = scales[(src_head * (D / 32) + ch / 4) * kBlock + slot];
-        if (ch % 4 == 0) scales[(head * (D / 32) + ch / 4) * kBlock + s] = static_cast<uint8_t>(byte);
-      }
-      if (kv == 0) {
-        u32x4 x;
-        if constexpr (KIND == kPagesModel) {
-          x = u32x4{raw[0], raw[1], raw[2], raw[3]};
-        } else if constexpr (KIND == kPagesE4m3) {
-          x = __builtin_bit_cast(u32x4, e4m3_x8<E>(raw[0], raw[1], e8m0(byte)));
-        } else {
-          x = e2m1_x8<E>(raw[0], e8m0(byte));
-        }
+    }
+  }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float lo = E::to_f32(x[i] & 0xFFFFu), hi = E::to_f32(x[i] >> 16);
-          mx[2 * i] = fmaxf(mx[2 * i], lo), mn[2 * i] = fminf(mn[2 * i], lo);
-          mx[2 * i + 1] = fmaxf(mx[2 * i + 1], hi), mn[2 * i + 1] = fminf(mn[2 * i + 1], hi);
+  for (int it = 0; it < IT; ++it) {
+    const int s = rg + RG * it;
+    if (s < count) {
+      *reinterpret_cast<words*>(kp + page * c.sk_p + s * c.sk_n) = rk[it];
+      *reinterpret_cast<words*>(vp + page * c.sv_p + s * c.sv_n) = rv[it];
+      u32x4 x;
+      if constexpr (KIND == kPagesModel) {
+        x = u32x4{rk[it][0], rk[it][1], rk[it][2], rk[it][3]};
+      } else {
+        if (holds) {
+          const int64_t at = (head * groups + grp) * kBlock + s;
+          c.k_scale[at] = static_cast<uint8_t>(bk[it]);
+          c.v_scale[at] = static_cast<uint8_t>(bv[it]);
         }
+        if constexpr (KIND == kPagesE4m3)
+          x = __builtin_bit_cast(u32x4, e4m3_x8<E>(rk[it][0], rk[it][1], e8m0(bk[it])));
+        else
+          x = e2m1_x8<E>(rk[it][0], e8m0(bk[it]));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lo = E::to_f32(x[i] & 0xFFFFu), hi = E::to_f32(x[i] >> 16);
+        mx[2 * i] = fmaxf(mx[2 * i], lo), mn[2 * i] = fminf(mn[2 * i], lo);
+        mx[2 * i + 1] = fmaxf(mx[2 * i + 1], hi), mn[2 * i + 1] = fminf(mn[2 * i + 1], hi);
       }
     }
   }
@@ -221,15 +447,20 @@ hipError_t launch_paged_evict(const PagedCache& c, const float* mass, int64_t sm
                               const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
                               int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
                               hipStream_t stream) {
-  paged_pick_kernel<<<dim3(c.Hk, B), kPickThreads, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages,
-                                                                c.num_pages, keep, recent, first, kept, new_lens);
+  // 8192 and 32768 weights fit the LDS of half a CU and of one
+  const auto pick = max_pages <= 128   ? paged_pick_kernel<8192>
+                    : max_pages <= 512 ? paged_pick_kernel<32768>
+                                       : paged_pick_kernel<0>;
+  pick<<<dim3(c.Hk, B), kPickThreads, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages, c.num_pages, keep,
+                                                   recent, first, kept, new_lens);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid(new_pages, c.Hk, B);
 #define UGBSA_EV(E_, D_, K_)                                                                                      \
   do {                                                                                                            \
-    paged_move_kernel<E_, D_, K_><<<grid, 256, 0, stream>>>(c, mass, sm_b, sm_h, table, st_b, new_table, sn_b, kept, \
-                                                            keep, new_lens, new_mass, so_b, so_h);                \
+    paged_move_kernel<E_, D_, K_><<<grid, 256, 0, stream>>>(c, mass, sm_b, sm_h, table, st_b, max_pages * kBlock,    \
+                                                            new_table, sn_b, kept, keep, new_lens, new_mass, so_b, \
+                                                            so_h);                                                \
     return hipGetLastError();                                                                                     \
   } while (0)
 #define UGBSA_EV_D(E_, K_)              \
