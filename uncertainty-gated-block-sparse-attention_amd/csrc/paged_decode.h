@@ -11,10 +11,20 @@
 // TB/s; 24 of up to 16K, bf16 (375 MB) 69.5 us, 5.4 TB/s with the joining launch; one of
 // 1000 tokens 11 us, two launches of about 4 us.
 //
-// MASS: the scaled scores go to a scratch [B, H, units, 64] on the way (units: the row's
-// pages or list entries), and each row's (m, l) beside it, from which paged_mass.hip adds
-// up the weights.
+// MASS: each cached token of a KV head gets the sum over its query heads of the weight
+// that the token had,
+//
+//   mass[b, g, i] += sum over the heads h of g of exp2(x_hi - m_h) / l_h.
+//
+// A weight is known when its row's maximum and sum are, so the attention launch leaves its
+// scaled scores in a scratch [B, H, units, 64] on the way (units: the row's pages or list
+// entries), and the (m, l) of the rows it writes whole; the launch that joins the others'
+// pieces adds the weights up, in the heads' order and without atomics: a sequence has its
+// own row of mass.  Scores again from K instead would read 2 D bytes a token in 16 bits,
+// this writes and reads 8 a query head.
 #pragma once
+
+#include <algorithm>
 
 #include "paged.h"
 
@@ -90,8 +100,10 @@ __host__ __device__ constexpr int pd_occupancy(int D, int kind) {
 // Where a MASS call leaves its scores and rows' statistics (null otherwise).
 struct PagedScores {
   float* x;        // [B, H, units, 64]
-  float* ml;       // [B, H, 2]
+  float* ml;       // [B, H, 2], of rows in one piece
   int units;
+  float* mass;     // [B, Hk, 64 max_pages]
+  int64_t sm_b, sm_h;
 };
 
 // ONE: the wavefronts of a workgroup that has a row to itself, 0: workgroups on the line.
@@ -563,10 +575,9 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
 constexpr int kPdMaxWorkgroups = 1024;
 constexpr int kPdCombineThreads = 256;
 template <typename E, int D>
-static __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
-    const int* __restrict__ starts, const float* __restrict__ part, const float* __restrict__ ml,
-    PagedGroups gr, int grp, int chunks, bool lists, uint16_t* __restrict__ out, int64_t so_b,
-    int64_t so_h, float* __restrict__ row_ml) {
+__device__ __forceinline__ void combine_row(const int* __restrict__ starts, const float* __restrict__ part,
+                                            const float* __restrict__ ml, PagedGroups gr, int grp, int chunks,
+                                            bool lists, uint16_t* __restrict__ out, int64_t so_b, int64_t so_h) {
   constexpr int RUNS = 4 * kPdCombineThreads / D, NH = pd_heads(D), PT = kPdMaxWorkgroups / kPdCombineThreads;
   __shared__ float s_w[kPdMaxWorkgroups];
   __shared__ float s_red[kPdCombineThreads / 64][2];
@@ -617,11 +628,6 @@ static __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel
 #pragma unroll
   for (int w = 0; w < kPdCombineThreads / 64; ++w) total += s_red[w][1];
 
-  if (row_ml != nullptr && tid == 0) {
-    float* to = row_ml + 2 * (static_cast<int64_t>(b) * H + h);
-    to[0] = mx, to[1] = total;
-  }
-
   const int run = tid / (D / 4), d4 = tid % (D / 4);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -634,6 +640,132 @@ static __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel
     for (int r = 1; r < RUNS; ++r) acc += s_acc[r][tid];
     store4<E>(o + 4 * tid, acc, total);
   }
+}
+
+template <typename E, int D>
+static __global__ __launch_bounds__(kPdCombineThreads) void paged_combine_kernel(
+    const int* __restrict__ starts, const float* __restrict__ part, const float* __restrict__ ml,
+    PagedGroups gr, int grp, int chunks, bool lists, uint16_t* __restrict__ out, int64_t so_b,
+    int64_t so_h) {
+  combine_row<E, D>(starts, part, ml, gr, grp, chunks, lists, out, so_b, so_h);
+}
+
+// Weights of a row's tiles tile .. tile + count - 1, 1024 tokens (16 pages or list entries)
+// each, four a thread; f(first, heads) fills s_m, s_inv with the maximum and the inverse
+// sum of the KV head's heads first .. .
+constexpr int kPdMassHeads = 8;
+template <typename F>
+__device__ __forceinline__ void add_mass(const PagedRows& rows, int Hk, int grp, const PagedScores& sc, int tile,
+                                         int count, int g, int b, const float* s_m, const float* s_inv, F f) {
+  const int len = cached_len(rows.lens, b, rows.max_pages);
+  int n = (len + kBlock - 1) / kBlock;
+  if (rows.kv_idx != nullptr) {
+    n = rows.counts == nullptr ? rows.k_slots : rows.counts[b * Hk + g];
+    n = len == 0 ? 0 : min(n, rows.k_slots);
+  }
+  const int64_t row0 = (static_cast<int64_t>(b) * Hk + g) * grp;
+  for (int t = tile; t < tile + count && t * 16 < n; ++t) {
+    const int i = 4 * (t * 256 + static_cast<int>(threadIdx.x)), unit = i / kBlock;
+    int blk = -1;
+    if (unit < n)
+      blk = rows.kv_idx == nullptr ? unit : rows.kv_idx[(static_cast<int64_t>(b) * Hk + g) * rows.k_slots + unit];
+    const int tok = blk * kBlock + i % kBlock;
+    const bool live = blk >= 0 && blk < rows.max_pages && tok < len;
+    float* to = sc.mass + b * sc.sm_b + g * sc.sm_h + tok;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f}, old = sum;
+    for (int h0 = 0; h0 < grp; h0 += kPdMassHeads) {
+      const int heads = min(kPdMassHeads, grp - h0);
+      // the scores are on the way while the statistics are worked out
+      f32x4 x[kPdMassHeads];
+      const float* at = sc.x + (row0 + h0) * sc.units * kBlock + i;
+#pragma unroll
+      for (int h = 0; h < kPdMassHeads; ++h)
+        if (live && h < heads) x[h] = *reinterpret_cast<const f32x4*>(at + static_cast<int64_t>(h) * sc.units * kBlock);
+      if (h0 == 0 && live) old = *reinterpret_cast<const f32x4*>(to);
+      if (t == tile || grp > kPdMassHeads) {
+        __syncthreads();
+        f(h0, heads);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int h = 0; h < kPdMassHeads; ++h)
+        if (h < heads) {
+          const float m = s_m[h], inv = s_inv[h];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sum[j] += x[h][j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[h][j] - m) * inv;   // no key: no weight
+        }
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (tok + j < len) old[j] += sum[j];
+    *reinterpret_cast<f32x4*>(to) = old;
+  }
+}
+// Tiles of a workgroup: some thousand workgroups in all, which start faster than more do.
+inline int pd_mass_tiles(int64_t tiles) { return static_cast<int>(std::min<int64_t>((tiles + 1023) / 1024, 8)); }
+
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// After a call whose rows have a workgroup each.
+static __global__ __launch_bounds__(256) void paged_mass_kernel(PagedRows rows, int Hk, int grp, int count, PagedScores sc) {
+  __shared__ float s_m[kPdMassHeads], s_inv[kPdMassHeads];
+  const int g = blockIdx.y, b = blockIdx.z;
+  const float* ml = sc.ml + 2 * (static_cast<int64_t>(b) * Hk + g) * grp;
+  add_mass(rows, Hk, grp, sc, blockIdx.x * count, count, g, b, s_m, s_inv, [&](int h0, int heads) {
+    for (int h = threadIdx.x; h < heads; h += 256) s_m[h] = ml[2 * (h0 + h)], s_inv[h] = inverse_sum(ml[2 * (h0 + h) + 1]);
+  });
+}
+
+// After a call on the line: the first B * H workgroups join a row's pieces, as
+// paged_combine_kernel, the others add weights, each working out the (m, l) of its heads.
+template <typename E, int D>
+static __global__ __launch_bounds__(kPdCombineThreads) void paged_finish_kernel(
+    const int* __restrict__ starts, const float* __restrict__ part, const float* __restrict__ ml, PagedRows rows,
+    PagedGroups gr, int grp, int chunks, int B, int parts, int count, uint16_t* __restrict__ out, int64_t so_b, int64_t so_h,
+    PagedScores sc) {
+  const bool lists = rows.kv_idx != nullptr;
+  const int joins = B * gr.Hk * grp;
+  if (static_cast<int>(blockIdx.x) < joins) {
+    combine_row<E, D>(starts, part, ml, gr, grp, chunks, lists, out, so_b, so_h);
+    return;
+  }
+  constexpr int NH = pd_heads(D);
+  __shared__ float s_m[kPdMassHeads], s_inv[kPdMassHeads];
+  const int at = blockIdx.x - joins, tile = at % parts * count, g = at / parts % gr.Hk, b = at / parts / gr.Hk;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float* row_ml = sc.ml + 2 * (static_cast<int64_t>(b) * gr.Hk + g) * grp;
+  add_mass(rows, gr.Hk, grp, sc, tile, count, g, b, s_m, s_inv, [&](int h0, int heads) {
+    const int group = lists ? b * gr.Hk + g : b;
+    const uint32_t s0 = starts[group], s1 = starts[group + 1], per = starts[gr.groups + 1];
+    const uint32_t n = (s1 - s0) / static_cast<uint32_t>(gr.members);
+    for (int h = wave; h < heads; h += kPdCombineThreads / 64) {
+      const int ck = (h0 + h) / NH, hh = (h0 + h) % NH, member = lists ? ck : g * chunks + ck;
+      const uint32_t first = s0 + member * n;
+      const int wa = static_cast<int>((first + kPdRowCost) / per);
+      const int pieces = n == 0 ? 0 : static_cast<int>((first + n - 1) / per) - wa + 1;
+      float m = -INFINITY, l = 0.f;
+      if (pieces == 1) {
+        m = row_ml[2 * (h0 + h)], l = row_ml[2 * (h0 + h) + 1];
+      } else {
+        for (int i = lane; i < pieces; i += 64) {       // the maximum and the sum so far, as over pages
+          const float* p = ml + 2 * (static_cast<int64_t>(2 * (wa + i) + (i == 0 ? 1 : 0)) * NH + hh);
+          const float top = fmaxf(m, p[0]), off = top == -INFINITY ? 0.f : top;
+          l = l * __builtin_amdgcn_exp2f(m - off) + p[1] * __builtin_amdgcn_exp2f(p[0] - off);
+          m = top;
+        }
+#pragma unroll
+        for (int s = 32; s >= 1; s >>= 1) {
+          const float m2 = __shfl_xor(m, s, 64), l2 = __shfl_xor(l, s, 64);
+          const float top = fmaxf(m, m2), off = top == -INFINITY ? 0.f : top;
+          l = l * __builtin_amdgcn_exp2f(m - off) + l2 * __builtin_amdgcn_exp2f(m2 - off);
+          m = top;
+        }
+      }
+      if (lane == 0) s_m[h] = m, s_inv[h] = inverse_sum(l);
+    }
+  });
 }
 
 // Whether each row gets a workgroup to itself, with no line to find and nothing to
@@ -685,6 +817,10 @@ hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& rows, con
     kernel<<<dim3(c.Hk * chunks, B), 64 * (four ? 4 : 8), 0, stream>>>(c, rows, gr, q, sq_b, sq_h, grp, chunks,
                                                                        scale * kLog2e, out, so_b, so_h, nullptr,
                                                                        nullptr, nullptr, sc);
+    const hipError_t e = hipGetLastError();
+    if (!MASS || e != hipSuccess) return e;
+    const int tiles = (units + 15) / 16, count = pd_mass_tiles(static_cast<int64_t>(tiles) * c.Hk * B);
+    paged_mass_kernel<<<dim3((tiles + count - 1) / count, c.Hk, B), 256, 0, stream>>>(rows, c.Hk, grp, count, sc);
     return hipGetLastError();
   }
   const int wgs = paged_decode_workgroups(B, H, c.Hk, D, KIND, units);
@@ -704,8 +840,16 @@ hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& rows, con
                                                   so_b, so_h, starts, part, ml, sc);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  paged_combine_kernel<E, D><<<dim3(B * H), kPdCombineThreads, 0, stream>>>(starts, part, ml, gr, grp, chunks, lists,
-                                                                            out, so_b, so_h, sc.ml);
+  if constexpr (MASS) {
+    const int tiles = (units + 15) / 16, count = pd_mass_tiles(static_cast<int64_t>(tiles) * c.Hk * B);
+    const int parts = (tiles + count - 1) / count;
+    const int64_t grid = static_cast<int64_t>(B) * H + static_cast<int64_t>(parts) * c.Hk * B;
+    paged_finish_kernel<E, D><<<dim3(static_cast<uint32_t>(grid)), kPdCombineThreads, 0, stream>>>(
+        starts, part, ml, rows, gr, grp, chunks, B, parts, count, out, so_b, so_h, sc);
+  } else {
+    paged_combine_kernel<E, D><<<dim3(B * H), kPdCombineThreads, 0, stream>>>(starts, part, ml, gr, grp, chunks,
+                                                                              lists, out, so_b, so_h);
+  }
   return hipGetLastError();
 }
 

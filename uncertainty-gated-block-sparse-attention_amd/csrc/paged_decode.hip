@@ -26,7 +26,7 @@ hipError_t launch_paged_decode(const PagedCache& c, const uint16_t* q, int64_t s
                                hipStream_t stream) {
   const PagedRows rows{lens, table, st_b, max_pages, kv_idx, counts, k_slots};
   const auto launch = c.kind == kPagesE2m1 ? launch_paged_decode_e2m1 : launch_paged_decode_16;
-  return launch(c, rows, q, sq_b, sq_h, B, H, scale, out, so_b, so_h, ws, PagedScores{nullptr, nullptr, 0}, stream);
+  return launch(c, rows, q, sq_b, sq_h, B, H, scale, out, so_b, so_h, ws, PagedScores{}, stream);
 }
 
 }  // namespace ugbsa

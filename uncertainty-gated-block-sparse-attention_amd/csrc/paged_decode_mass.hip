@@ -1,50 +1,7 @@
-// Paged decode attention (paged_decode.h) whose weights are followed: each cached token
-// of a KV head gets the sum over its query heads of the weight that the token had,
-//
-//   mass[b, g, i] += sum over the heads h of g of exp2(x_hi - m_h) / l_h.
-//
-// A weight is known when its row's maximum and sum are, so the attention launch leaves
-// its scaled scores (4 bytes a query head and token) and the rows' statistics, and a third
-// launch adds them up, in the heads' order and without atomics: a sequence has its own row.
+// Paged decode attention whose weights are followed: the MASS instances (paged_decode.h).
 #include "paged_decode.h"
 
 namespace ugbsa {
-
-// Four tokens (of a page or list entry) per thread, over the heads of a KV head.
-__global__ __launch_bounds__(256) void paged_mass_kernel(PagedRows rows, int Hk, int grp, PagedScores sc,
-                                                         float* __restrict__ mass, int64_t sm_b, int64_t sm_h) {
-  const int g = blockIdx.y, b = blockIdx.z;
-  const int i = 4 * (blockIdx.x * 256 + threadIdx.x), unit = i / kBlock;
-  const int len = cached_len(rows.lens, b, rows.max_pages);
-  int n = rows.max_pages;
-  if (rows.kv_idx != nullptr) {
-    n = rows.counts == nullptr ? rows.k_slots : rows.counts[b * Hk + g];
-    n = min(n, rows.k_slots);
-  }
-  if (len == 0 || unit >= n) return;
-  const int blk =
-      rows.kv_idx == nullptr ? unit : rows.kv_idx[(static_cast<int64_t>(b) * Hk + g) * rows.k_slots + unit];
-  if (blk < 0 || blk >= rows.max_pages) return;
-  const int tok = blk * kBlock + i % kBlock;
-  if (tok >= len) return;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  const int64_t row0 = (static_cast<int64_t>(b) * Hk + g) * grp;
-#pragma unroll 4
-  for (int h = 0; h < grp; ++h) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(sc.x + (row0 + h) * sc.units * kBlock + i);
-    const float m = sc.ml[2 * (row0 + h)], l = sc.ml[2 * (row0 + h) + 1];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      sum[j] += x[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[j] - m) * inv;   // no key: no weight
-  }
-  float* to = mass + b * sm_b + g * sm_h + tok;
-  f32x4 old = *reinterpret_cast<const f32x4*>(to);
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (tok + j < len) old[j] += sum[j];
-  *reinterpret_cast<f32x4*>(to) = old;
-}
 
 hipError_t launch_paged_decode_mass(UGBSA_PD_ARGS) {
   if (c.kind == kPagesE4m3) {
@@ -74,11 +31,8 @@ hipError_t launch_paged_mass(const PagedCache& c, const uint16_t* q, int64_t sq_
   const PagedRows rows{lens, table, st_b, max_pages, kv_idx, counts, k_slots};
   const int units = kv_idx != nullptr ? k_slots : max_pages;
   float* ml = ws + decode_elems(B, H, c.Hk, c.D, c.kind, units);
-  const PagedScores sc{ml + (2 * static_cast<int64_t>(B) * H + 3) / 4 * 4, ml, units};
-  const hipError_t e = launch_paged_decode_mass(c, rows, q, sq_b, sq_h, B, H, scale, out, so_b, so_h, ws, sc, stream);
-  if (e != hipSuccess) return e;
-  paged_mass_kernel<<<dim3((units + 15) / 16, c.Hk, B), 256, 0, stream>>>(rows, c.Hk, H / c.Hk, sc, mass, sm_b, sm_h);
-  return hipGetLastError();
+  const PagedScores sc{ml + (2 * static_cast<int64_t>(B) * H + 3) / 4 * 4, ml, units, mass, sm_b, sm_h};
+  return launch_paged_decode_mass(c, rows, q, sq_b, sq_h, B, H, scale, out, so_b, so_h, ws, sc, stream);
 }
 
 }  // namespace ugbsa
