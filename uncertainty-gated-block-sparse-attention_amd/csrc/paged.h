@@ -67,6 +67,15 @@ __device__ __forceinline__ uint32_t e2m1_pair(uint32_t codes, float scale) {
   else
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, SEL));
 }
+// A pair of E's values over scale, rounded to the nearest even code, as codes 2 SEL and
+// 2 SEL + 1 of a word; magnitudes past 6 (and NaN) give 6.
+template <typename E, int SEL>
+__device__ __forceinline__ uint32_t e2m1_codes(uint32_t word, uint32_t pair, float scale) {
+  if constexpr (E::code == ElemF16::code)
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, __builtin_bit_cast(f16x2, pair), scale, SEL);
+  else
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, __builtin_bit_cast(bf16x2, pair), scale, SEL);
+}
 template <typename E>
 __device__ __forceinline__ u32x4 e2m1_x8(uint32_t codes, float scale) {
   return u32x4{e2m1_pair<E, 0>(codes, scale), e2m1_pair<E, 1>(codes, scale), e2m1_pair<E, 2>(codes, scale),

@@ -160,37 +160,34 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
       if constexpr (KIND == kPagesModel) {
         *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(kv ? c.v : c.k) + at) = raw;
       } else if constexpr (KIND == kPagesE2m1) {
-        // the largest magnitude that reads back finite from two bits; a group with a NaN
-        // is NaN throughout, as its codes have no room for one
-        constexpr float kMost = E::code == ElemF16::code ? 49152.f : 1.5f * 0x1p127f;
-        float top = 0.f;
-        uint32_t nan = 0u;
+        // A group's largest magnitude from the 16-bit patterns, whose order is the magnitudes':
+        // a pattern past infinity's is a NaN, and the group is NaN throughout, as its codes have
+        // no room for one; past the largest that reads back finite from two bits it counts as
+        // that, and the conversion holds its code at 6.
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        constexpr uint32_t kInf = E::code == ElemF16::code ? 0x7C00u : 0x7F80u;
+        constexpr uint32_t kMost = E::code == ElemF16::code ? 0x7A00u : 0x7F40u;   // 1.5 2^15, 1.5 2^127
+        u16x2 mv = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          nan |= x[j] != x[j] ? 1u : 0u;
-          x[j] = x[j] > kMost ? kMost : (x[j] < -kMost ? -kMost : x[j]);
-          top = fmaxf(top, fabsf(x[j]));
-        }
-#pragma unroll
-        for (int off = 2; off >= 1; off >>= 1) {
-          top = fmaxf(top, __shfl_xor(top, off, 64));
-          nan |= __shfl_xor(nan, off, 64);
-        }
+        for (int j = 0; j < 4; ++j)
+          mv = __builtin_elementwise_max(mv, __builtin_bit_cast(u16x2, raw[j] & 0x7FFF7FFFu));
+        uint32_t top = max(static_cast<uint32_t>(mv[0]), static_cast<uint32_t>(mv[1]));
+        top = max(top, xor_lanes<1>(top, tid & 63));
+        top = max(top, xor_lanes<2>(top, tid & 63));
         // smallest e with top <= 6 2^e = 1.5 2^(e + 2), as a byte e + 127
-        const uint32_t bits = __float_as_uint(top);
+        const uint32_t bits = __float_as_uint(E::to_f32(min(top, kMost)));
         const int e = static_cast<int>(bits >> 23) - 2 + ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 0);
         const int byte = bits == 0u ? 127 : max(e, 0);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = nan ? 0.f : ldexpf(x[j], 127 - byte);   // exact, or below half a step
+        const float scale = e8m0(static_cast<uint32_t>(byte));
         uint32_t code = 0u;
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], 1.f, 0);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], 1.f, 1);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[4], x[5], 1.f, 2);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[6], x[7], 1.f, 3);
+        code = e2m1_codes<E, 0>(code, raw[0], scale);
+        code = e2m1_codes<E, 1>(code, raw[1], scale);
+        code = e2m1_codes<E, 2>(code, raw[2], scale);
+        code = e2m1_codes<E, 3>(code, raw[3], scale);
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kv ? c.v : c.k) + at) = code;
         if (ch % 4 == 0)
           (kv ? c.v_scale : c.k_scale)[(head * (D / 32) + ch / 4) * kBlock + s] =
-              static_cast<uint8_t>(nan ? 255 : byte);
+              static_cast<uint8_t>(top > kInf ? 255 : byte);
       } else {
         // the largest magnitude whose four-bit rounding reads back finite (infinities
         // are held there too; NaN stays NaN and does not count for the scale)

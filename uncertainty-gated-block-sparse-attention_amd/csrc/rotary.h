@@ -37,10 +37,13 @@ __device__ __forceinline__ void turn_cos_sin(double pos, double turns, float m, 
   sn *= quarter >= 2 ? -m : m;
 }
 
-// The two values of a pair, turned.
+// The two values of a pair, turned, as fp32 values that no instruction has rounded to 16 bits
+// in the same step: the caller's rounding is the same whatever is compiled around it, so
+// that keys turned as they are written have the bits of keys turned before.
 __device__ __forceinline__ void turn_pair(float a, float b, float cs, float sn, float& ya, float& yb) {
   ya = __builtin_fmaf(a, cs, -(b * sn));
   yb = __builtin_fmaf(b, cs, a * sn);
+  asm("" : "+v"(ya), "+v"(yb));
 }
 
 }  // namespace ugbsa
