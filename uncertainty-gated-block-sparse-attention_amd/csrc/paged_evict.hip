@@ -8,9 +8,7 @@
 
 namespace ugbsa {
 
-constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64;
 constexpr int kPickBins = 2048;        // 11, 11 and 10 bits of the key
-constexpr int kPickList = 4096;        // keys of the cut's bin that are listed
 
 // Order of the tokens that compete, larger first: NaN, then by weight, zeros of either
 // sign alike.
@@ -32,12 +30,14 @@ __device__ __forceinline__ uint32_t pick_key(float x) { return x != x ? kPickNan
 // scalar registers; and what only some tokens need (ends of the range, absent pages, NaN)
 // behind scalar branches.
 //
-// 64 rows of up to 32K tokens (2.6 MB) XX us; one of 600 XX.
-template <int ROW>
+// 64 rows of up to 32K tokens (2.6 MB) 26.7 us; four of 600 9.3.
+template <int ROW, int kPickThreads>
 __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     const float* __restrict__ mass, int64_t sm_b, int64_t sm_h, const int32_t* __restrict__ lens,
     const int32_t* __restrict__ table, int64_t st_b, int max_pages, int num_pages, int keep, int recent, int first,
     int32_t* __restrict__ kept, int32_t* __restrict__ new_lens) {
+  constexpr int kPickWaves = kPickThreads / 64, kEach = kPickBins / kPickThreads;
+  constexpr int kPickList = ROW == 0 || ROW > 4096 ? 4096 : ROW;       // keys of the cut's bin that are listed
   __shared__ uint32_t s_hist[kPickBins], s_list[kPickList], s_wave[2][kPickWaves], s_found[3], s_listed, s_stay;
   __shared__ uint8_t s_from[kPickList];
   __shared__ f32x4 s_row[ROW > 0 ? ROW / 4 : 1];
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
   uint32_t top = 0u;                                  // keys of the cut's bin of the top digit
   int total = 0;                                      // tokens with a page
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : kPickBins;
     if (pass == 0) {
       if (absent) {                                   // those that stay and are there
         uint32_t stay = 0u;
@@ -172,13 +172,15 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
       });
     }
     __syncthreads();
-    // bins from the largest: thread t holds bins - 1 - 2 t and the one below it; the bits of
-    // a positive weight's key are its own but for the sign, those of a negative one's turned
-    const int hi = bins - 1 - 2 * tid;
+    // bins from the largest: thread t holds kEach from 2047 - kEach t down; the bits of a positive
+    // weight's key are its own but for the sign, those of a negative one's turned
+    const int hi = kPickBins - 1 - kEach * tid;
     auto held = [&](int bin) { return pass > 0 ? bin : (bin >= 1024 ? bin - 1024 : 2047 - bin); };
-    const uint32_t h0 = hi >= 0 ? s_hist[held(hi)] : 0u, h1 = hi >= 1 ? s_hist[held(hi - 1)] : 0u;
-    const uint32_t ex = wave_excl_scan(h0 + h1, lane);
-    if (lane == 63) s_wave[0][wave] = ex + h0 + h1;
+    uint32_t h[kEach], sum = 0u;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) sum += h[j] = s_hist[held(hi - j)];
+    const uint32_t ex = wave_excl_scan(sum, lane);
+    if (lane == 63) s_wave[0][wave] = ex + sum;
     __syncthreads();
     uint32_t before = ex;
     for (int w = 0; w < wave; ++w) before += s_wave[0][w];
@@ -190,8 +192,11 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
       want = keep - stay;
       if (total <= keep || want == 0u) break;         // all that compete stay, or none
     }
-    if (before < want && want <= before + h0) s_found[0] = hi, s_found[1] = before, s_found[2] = h0;
-    else if (before + h0 < want && want <= before + h0 + h1) s_found[0] = hi - 1, s_found[1] = before + h0, s_found[2] = h1;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (before < want && want <= before + h[j]) s_found[0] = hi - j, s_found[1] = before, s_found[2] = h[j];
+      before += h[j];
+    }
     for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0u;
     __syncthreads();
     prefix |= static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(s_found[0])) << shift;
@@ -447,12 +452,16 @@ hipError_t launch_paged_evict(const PagedCache& c, const float* mass, int64_t sm
                               const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
                               int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
                               hipStream_t stream) {
-  // 8192 and 32768 weights fit the LDS of half a CU and of one
-  const auto pick = max_pages <= 128   ? paged_pick_kernel<8192>
-                    : max_pages <= 512 ? paged_pick_kernel<32768>
-                                       : paged_pick_kernel<0>;
-  pick<<<dim3(c.Hk, B), kPickThreads, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages, c.num_pages, keep,
-                                                   recent, first, kept, new_lens);
+  // Rows of up to 2048 tokens have four wavefronts, whose barriers are shorter and several of
+  // which share a CU (512 rows of 1000 tokens 10.8 us, 128 of 4096 12.4; with 16 wavefronts the
+  // 512 took 18.9); 8192 and 32768 weights fit the LDS of half a CU and of one.
+  const int threads = max_pages <= 32 ? 256 : 1024;
+  const auto pick = max_pages <= 32    ? paged_pick_kernel<2048, 256>
+                    : max_pages <= 128 ? paged_pick_kernel<8192, 1024>
+                    : max_pages <= 512 ? paged_pick_kernel<32768, 1024>
+                                       : paged_pick_kernel<0, 1024>;
+  pick<<<dim3(c.Hk, B), threads, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages, c.num_pages, keep,
+                                              recent, first, kept, new_lens);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid(new_pages, c.Hk, B);

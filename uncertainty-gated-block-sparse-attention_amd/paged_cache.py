@@ -311,17 +311,17 @@ def paged_select(q, cache, block_table, seq_lens, scaling, k_base, k_slots, tau=
 
 
 def _check_mass(name, t, cache, shape):
-    """Weights [B, Hk, >= 64 * pages] fp32 that a call reads or adds to in place, each row its own memory."""
-    assert t.dim() == 3 and t.shape[:2] == shape[:2] and t.shape[2] >= shape[2] and t.dtype is torch.float32 \
-        and t.get_device() == cache._call[1], f"{name} [{shape[0]}, {shape[1]}, >= {shape[2]}] fp32 on the cache's device expected"
-    assert t.stride(2) == 1 and t.data_ptr() % 16 == 0 and not any(s % 4 for s, n in zip(t.stride()[:2], shape) if n > 1), \
+    """Strides (b, h) of weights [B, Hk, >= 64 * pages] fp32 that a call reads or adds to in place."""
+    B, Hk, n = shape
+    size = t.shape
+    assert len(size) == 3 and size[0] == B and size[1] == Hk and size[2] >= n and t.dtype is torch.float32 \
+        and t.get_device() == cache._call[1], f"{name} [{B}, {Hk}, >= {n}] fp32 on the cache's device expected"
+    st_b, st_h, st_n = t.stride()
+    st_b, st_h = st_b if B > 1 else 0, st_h if Hk > 1 else 0      # of one element any will do
+    assert st_n == 1 and not (t.data_ptr() & 15 or st_b & 3 or st_h & 3), \
         f"{name}: contiguous, 16-byte aligned rows required"
     assert not (t.is_neg() or t.requires_grad), f"{name}: a plain tensor without gradients required"
-
-
-def _rows(t):
-    """Row strides of a tensor of weights: of a dimension of one element any will do."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:2], t.shape))
+    return st_b, st_h
 
 
 def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=None, out=None, mass=None):
@@ -360,17 +360,16 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     so_b, _, so_h, so_d = out.stride()
     lib = _capi.lib()
     if mass is not None:
-        _check_mass("mass", mass, cache, (B, Hk, PAGE * max_pages))
-        sm_b, sm_h = mass.stride()[:2]
-        assert (B == 1 or sm_b) and (Hk == 1 or sm_h), "mass: rows share memory"
-        assert B == 1 or Hk == 1 or max(sm_b, sm_h) >= mass.shape[2] + (mass.shape[1 if sm_b > sm_h else 0] - 1) * min(sm_b, sm_h), \
-            "mass: rows share memory"
+        sm_b, sm_h = _check_mass("mass", mass, cache, (B, Hk, PAGE * max_pages))
+        outer, inner = (sm_b, sm_h * (Hk - 1)) if sm_b > sm_h else (sm_h, sm_b * (B - 1))
+        assert (B == 1 or sm_b >= mass.shape[2]) and (Hk == 1 or sm_h >= mass.shape[2]) and (
+            B == 1 or Hk == 1 or outer >= inner + mass.shape[2]), "mass: rows share memory"
         n = lib.ugbsa_paged_decode_mass_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
         ws = torch.empty(n, dtype=torch.float32, device=cache.device)
         torch.autograd.graph.increment_version(mass)
         _launch(cache, "paged_decode_mass", lib.ugbsa_paged_decode_mass, q.data_ptr(), *q.stride(), H,
                 seq_lens.data_ptr(), block_table.data_ptr(), st_b, B, max_pages, scale, _capi.ptr(kv_idx),
-                _capi.ptr(counts), slots, mass.data_ptr(), *_rows(mass), out.data_ptr(), so_b, so_h, so_d,
+                _capi.ptr(counts), slots, mass.data_ptr(), sm_b, sm_h, out.data_ptr(), so_b, so_h, so_d,
                 ws.data_ptr(), n)
         return out
     n = lib.ugbsa_paged_decode_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
@@ -412,14 +411,14 @@ def paged_evict(cache, mass, block_table, seq_lens, new_table, keep, recent=0, f
         "new_table [B, new_pages] int32 on the cache's device expected"
     new_pages = new_table.shape[1]
     assert new_table.stride(1) == 1 or new_pages == 1, "new_table: a row's entries must be contiguous"
-    _check_mass("mass", mass, cache, (B, Hk, PAGE * max_pages))
+    sm_b, sm_h = _check_mass("mass", mass, cache, (B, Hk, PAGE * max_pages))
     if _watched():
         _check_unwatched(mass)
     device = cache.device
     kept = torch.empty((B, Hk, max(keep, 0)), dtype=torch.int32, device=device)
     lens = torch.empty(B, dtype=torch.int32, device=device)
     new_mass = torch.empty((B, Hk, PAGE * new_pages), dtype=torch.float32, device=device)
-    _launch(cache, "paged_evict", _capi.lib().ugbsa_paged_evict, mass.data_ptr(), *_rows(mass), seq_lens.data_ptr(),
+    _launch(cache, "paged_evict", _capi.lib().ugbsa_paged_evict, mass.data_ptr(), sm_b, sm_h, seq_lens.data_ptr(),
             block_table.data_ptr(), st_b, B, max_pages, new_table.data_ptr(), new_table.stride(0), new_pages, keep,
             recent, first, kept.data_ptr(), lens.data_ptr(), new_mass.data_ptr(), *new_mass.stride()[:2])
     return PagedEviction(kept, lens, new_mass)
