@@ -124,3 +124,19 @@ def test_keys_are_turned_by_whole_arguments_only(monkeypatch):
                dict(rotary=rot, positions=torch.zeros(2, dtype=torch.int32))):
         with pytest.raises(AssertionError):
             pc.paged_write(cache, k, k, table, lens, **kw)
+
+
+def test_tensors_made_for_inference(monkeypatch):
+    """They keep no version that a call in place could raise."""
+    import rotary as ro
+    from types import SimpleNamespace
+    monkeypatch.setattr(pc, "_launch", lambda *a: None)
+    monkeypatch.setattr(ro, "_launch", lambda *a: None)
+    with torch.inference_mode():
+        cache, q = host_cache(), torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+        table, lens, mass = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 2, 128)
+        pc.paged_decode(q, cache, table, lens, 0.1, mass=mass)
+        pc.paged_evict(cache, mass, table, lens, torch.ones(1, 2, dtype=torch.int32), 64)
+        x = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+        ro.rotary(SimpleNamespace(_call=(None, -1, 64)), lens, x, out=x)
+    pc.paged_decode(q, cache, table, lens, 0.1, mass=mass)

@@ -366,7 +366,8 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
             B == 1 or Hk == 1 or outer >= inner + mass.shape[2]), "mass: rows share memory"
         n = lib.ugbsa_paged_decode_mass_workspace_elems(B, H, Hk, D, slots or max_pages, cache._struct.cache_dtype)
         ws = torch.empty(n, dtype=torch.float32, device=cache.device)
-        torch.autograd.graph.increment_version(mass)
+        if not mass.is_inference():       # those have no version for autograd to look at
+            torch.autograd.graph.increment_version(mass)
         _launch(cache, "paged_decode_mass", lib.ugbsa_paged_decode_mass, q.data_ptr(), *q.stride(), H,
                 seq_lens.data_ptr(), block_table.data_ptr(), st_b, B, max_pages, scale, _capi.ptr(kv_idx),
                 _capi.ptr(counts), slots, mass.data_ptr(), sm_b, sm_h, out.data_ptr(), so_b, so_h, so_d,

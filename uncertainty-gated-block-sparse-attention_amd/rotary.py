@@ -253,7 +253,8 @@ def _turn(rot, positions, q, k, out, inverse):
         assert len(outs) == (1 if k is None else 2), "out: a tensor for each of q and k expected"
         _check_out(outs, (q,) if k is None else (q, k))
         for o in outs:
-            torch.autograd.graph.increment_version(o)
+            if not o.is_inference():      # those have no version for autograd to look at
+                torch.autograd.graph.increment_version(o)
         qo, ko = (*outs, None)[:2]
     if M:
         kv = _NONE if k is None else (kc.data_ptr(), *_strides(kc), ko.data_ptr(), *_strides(ko), Hk)
