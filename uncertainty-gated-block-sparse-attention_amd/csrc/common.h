@@ -214,6 +214,9 @@ __device__ __forceinline__ void buffer_load_lds16(__amdgpu_buffer_rsrc_t r, void
 // s_waitcnt lgkmcnt(0): every LDS read of this wave has returned.
 __device__ __forceinline__ void wait_lds_reads() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
+// s_waitcnt vmcnt(0): every load of this wave has returned, those into LDS among them.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // Monotone uint32 key of an fp32 value (larger float -> larger key); NaN is
 // mapped above +inf, matching torch.topk / kthvalue's NaN-is-largest order.
 __device__ __forceinline__ uint32_t float_key(float x) {

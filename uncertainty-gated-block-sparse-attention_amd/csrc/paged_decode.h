@@ -394,7 +394,10 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
           s[mt] = E::mfma(a, qf[ks], s[mt]);
         }
       if constexpr (F4) {
-        // V out of LDS, then the next step's K and V into registers and LDS
+        // V out of LDS, once it is there, then the next step's K and V into registers and LDS
+        asm volatile("" ::: "memory");
+        wait_loads();
+        asm volatile("" ::: "memory");
         const char* at = v_lds + RB * g4 + VB * r16;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
