@@ -465,12 +465,15 @@ int ugbsa_paged_decode_mass(const ugbsa_paged_cache* cache, const void* q, int64
  * ascending, then 64 * max_pages; new_lens [B] int32; new_mass [B, Hk, 64 * new_pages], the
  * kept tokens' mass, then zeros (mass and new_mass: rows as above).  Keys keep the
  * positions they were turned by: a later token's position is no longer its length.
- * 1 <= keep <= 64 * new_pages; recent + first <= keep. */
+ * 1 <= keep <= 64 * new_pages; recent + first <= keep.
+ * workspace: 16-byte aligned floats, as many as the query says (none for most sizes). */
+int64_t ugbsa_paged_evict_workspace_elems(int B, int Hk, int max_pages);
 int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t sm_b,
                       int64_t sm_h, const int32_t* lens, const int32_t* table, int64_t st_b, int B,
                       int max_pages, const int32_t* new_table, int64_t sn_b, int new_pages,
                       int keep, int recent, int first, int32_t* kept, int32_t* new_lens,
-                      float* new_mass, int64_t so_b, int64_t so_h, void* stream);
+                      float* new_mass, int64_t so_b, int64_t so_h, float* workspace,
+                      int64_t workspace_elems, void* stream);
 
 #ifdef __cplusplus
 }

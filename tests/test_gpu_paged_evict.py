@@ -320,6 +320,58 @@ def test_evict_long_rows(hip_lib):
                 assert torch.equal(cache.v_scale[dst, h, :, to % 64], cache.v_scale[src, h, :, t % 64])
 
 
+def pick_ref(row, tokens, n, keep, recent, first):
+    """The tokens of one row that stay: `tokens` [n] true where there is a page."""
+    i = torch.arange(n, device=DEV)
+    sure = (i < first) | (i >= n - recent)
+    x = row[:n] + 0.0
+    # a rank: those that stay in any case, NaN, then by weight; the stable sort keeps ties in order
+    x = torch.where(sure, INF, torch.where(x.isnan(), INF, x))
+    order = x.sort(descending=True, stable=True)[1]
+    cls = torch.where(sure, 0, torch.where(row[:n].isnan(), 1, 2))
+    cls = torch.where(tokens, cls, 3)
+    order = order[cls[order].sort(stable=True)[1]]
+    return order[:min(keep, int(tokens.sum()))].sort()[0]
+
+
+@pytest.mark.parametrize("width,B,Hk", [(129, 2, 3), (260, 2, 3), (520, 3, 2), (260, 11, 6), (520, 11, 6)])
+def test_evict_rows_of_many_pages(hip_lib, width, B, Hk):
+    """Few rows of many pages are picked by several workgroups each, many by one: cuts at the ends of
+    their parts, first and newest tokens over several of them, absent pages, ties, NaN."""
+    print(f"[case] rows of {width} pages, {B} x {Hk}", flush=True)
+    g = gen(width + B)
+    W = 64 * width
+    cache = filled(g, 400, Hk, 64, BF, "e4m3")
+    lens = [[W, 4097], [4096, 8192], [W - 1, 8193], [0, 1], [63, -3]]
+    special = torch.tensor([NAN, INF, -INF, 0.0, -0.0, 1e-42, -1e-42, 1.0, -1.0, 3e38], device=DEV)
+
+    def masses():
+        yield torch.exp(3 * torch.randn(B, Hk, W, generator=g, device=DEV))
+        yield torch.zeros(B, Hk, W, device=DEV)
+        yield torch.randint(0, 3, (B, Hk, W), generator=g, device=DEV).float()
+        yield special[torch.randint(0, 10, (B, Hk, W), generator=g, device=DEV)]
+        yield torch.where(torch.rand(B, Hk, W, generator=g, device=DEV) < 0.3, NAN, 1.0)
+        yield 1 + 2.0 ** -23 * torch.randint(0, 9, (B, Hk, W), generator=g, device=DEV)
+        yield torch.rand(B, Hk, W, generator=g, device=DEV)
+
+    for i, mass in enumerate(masses()):
+        pages = torch.randint(0, 300, (B, width), generator=g, device=DEV, dtype=torch.int32)
+        if i % 2:
+            pages = torch.where(torch.rand(B, width, generator=g, device=DEV) < 0.2, -1, pages)
+        lengths = [lens[i % 5][b % 2] for b in range(B)]
+        for keep, recent, first in ((1, 0, 0), (200, 30, 4), (5000, 4500, 300), (5000, 0, 5000), (6000, 0, 0), (W, 0, 0)):
+            new_table = torch.full((B, (keep + 63) // 64), -1, dtype=torch.int32, device=DEV)
+            r = pc.paged_evict(cache, mass, pages, i32(lengths), new_table, keep, recent=recent, first=first)
+            for b in {0, 1, B - 1}:
+                n = min(max(lengths[b], 0), W)
+                there = (pages[b] >= 0).repeat_interleave(64)[:n]
+                want = [pick_ref(mass[b, h], there, n, keep, recent, first) for h in range(Hk)]
+                assert int(r.seq_lens[b]) == len(want[0])
+                for h in range(Hk):
+                    assert torch.equal(r.kept[b, h, :len(want[h])].long(), want[h])
+                    assert (r.kept[b, h, len(want[h]):] == W).all()
+
+
 def test_evict_of_a_shared_prefix(hip_lib):
     """Two sequences that share pages keep different tokens of them; the pages stay as they are."""
     g = gen(36)

@@ -28,9 +28,9 @@ def mass_call(lib, c, B=1, H=4, pages=8, mass=16, sm_b=1024, sm_h=512, kv=None, 
 
 
 def evict_call(lib, c, mass=16, sm=512, lens=16, table=16, new=16, sn=4, pages=4, keep=100, recent=0, first=0, kept=16,
-               new_lens=16, new_mass=16, so=256):
-    return lib.ugbsa_paged_evict(ctypes.addressof(c) if c else None, mass, sm, sm, lens, table, 8, 1, 8, new, sn, pages,
-                                 keep, recent, first, kept, new_lens, new_mass, so, so, None)
+               new_lens=16, new_mass=16, so=256, max_pages=8, ws=None, n=0):
+    return lib.ugbsa_paged_evict(ctypes.addressof(c) if c else None, mass, sm, sm, lens, table, 8, 1, max_pages, new, sn,
+                                 pages, keep, recent, first, kept, new_lens, new_mass, so, so, ws, n, None)
 
 
 def test_four_bit_caches(lib):
@@ -68,6 +68,12 @@ def test_evict_refusals(lib):
                            (dict(keep=257), -1, "keep"), (dict(recent=-1), -1, "recent"), (dict(first=-1), -1, "recent"),
                            (dict(recent=60, first=41), -1, "recent"), (dict(recent=(1 << 31) - 1, first=(1 << 31) - 1), -1, "recent")):
         refused(lib, evict_call(lib, four(), **kw), code, word)
+    assert lib.ugbsa_paged_evict_workspace_elems(1, 2, 8) == lib.ugbsa_paged_evict_workspace_elems(1, 2, 0) == 0
+    assert lib.ugbsa_paged_evict_workspace_elems(1, 2, (1 << 24) + 1) == 0
+    need = lib.ugbsa_paged_evict_workspace_elems(1, 2, 512)
+    assert need > 0
+    for kw, code in ((dict(ws=None, n=need), -1), (dict(ws=16, n=need - 1), -1), (dict(ws=8, n=need), -2)):
+        refused(lib, evict_call(lib, four(), max_pages=512, **kw), code, "workspace")
 
 
 def test_write_rotary_refusals(lib):

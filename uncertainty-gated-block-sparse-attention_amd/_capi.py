@@ -95,8 +95,9 @@ SIGNATURES = {
     "ugbsa_paged_decode_mass_workspace_elems": (_i64, [_i, _i, _i, _i, _i, _i]),
     "ugbsa_paged_decode_mass": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i, _p, _p, _i64, _i, _i, _f, _p,
                                      _p, _i, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p]),
+    "ugbsa_paged_evict_workspace_elems": (_i64, [_i, _i, _i]),
     "ugbsa_paged_evict": (_i, [_p, _p, _i64, _i64, _p, _p, _i64, _i, _i, _p, _i64, _i, _i, _i, _i, _p,
-                               _p, _p, _i64, _i64, _p]),
+                               _p, _p, _i64, _i64, _p, _i64, _p]),
     "ugbsa_rotary": (_i, [_p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i,
                           _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i,
                           _i, _i, _p]),

@@ -813,11 +813,16 @@ int ugbsa_paged_decode_mass(const ugbsa_paged_cache* cache, const void* q, int64
                     "paged_decode_mass");
 }
 
+int64_t ugbsa_paged_evict_workspace_elems(int B, int Hk, int max_pages) {
+  if (check_dims(B, Hk, 1, 64, UGBSA_DTYPE_BF16) || max_pages < 1 || max_pages > 1 << 24) return 0;
+  return ugbsa::paged_evict_ws_elems(B, Hk, max_pages);
+}
+
 int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t sm_b, int64_t sm_h,
                       const int32_t* lens, const int32_t* table, int64_t st_b, int B, int max_pages,
                       const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
                       int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
-                      void* stream) {
+                      float* workspace, int64_t workspace_elems, void* stream) {
   int rc = check_paged(cache, cache ? cache->Hk : 1, lens, table, st_b, B, max_pages);
   if (rc || (rc = check_pages(cache)) || (rc = check_mass("mass", mass, sm_b, sm_h)) ||
       (rc = check_mass("new_mass", new_mass, so_b, so_h)))
@@ -831,9 +836,13 @@ int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t
   if (recent < 0 || first < 0 || static_cast<int64_t>(recent) + first > keep)
     return fail(UGBSA_EARG, "recent and first must not be negative, nor more than keep together (%d, %d, keep %d)",
                 recent, first, keep);
+  if ((rc = check_decode_workspace("ugbsa_paged_evict_workspace_elems",
+                                   ugbsa_paged_evict_workspace_elems(B, cache->Hk, max_pages), workspace,
+                                   workspace_elems)))
+    return rc;
   return hip_result(ugbsa::launch_paged_evict(paged_cache(cache), mass, sm_b, sm_h, lens, table, st_b, B, max_pages,
                                               new_table, sn_b, new_pages, keep, recent, first, kept, new_lens,
-                                              new_mass, so_b, so_h, static_cast<hipStream_t>(stream)),
+                                              new_mass, so_b, so_h, workspace, static_cast<hipStream_t>(stream)),
                     "paged_evict");
 }
 

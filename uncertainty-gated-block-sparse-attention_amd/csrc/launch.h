@@ -230,10 +230,11 @@ hipError_t launch_paged_mass(const PagedCache& c, const uint16_t* q, int64_t sq_
 
 // The first, the newest and the heaviest tokens of each (sequence, KV head) into other
 // pages (paged_evict.hip).
+int64_t paged_evict_ws_elems(int B, int Hk, int max_pages);
 hipError_t launch_paged_evict(const PagedCache& c, const float* mass, int64_t sm_b, int64_t sm_h,
                               const int32_t* lens, const int32_t* table, int64_t st_b, int B, int max_pages,
                               const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
                               int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
-                              hipStream_t stream);
+                              float* workspace, hipStream_t stream);
 
 }  // namespace ugbsa

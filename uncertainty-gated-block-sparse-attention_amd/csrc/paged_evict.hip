@@ -15,39 +15,158 @@ constexpr int kPickBins = 2048;        // 11, 11 and 10 bits of the key
 constexpr uint32_t kPickNan = 0xFFFFFFFEu, kPickInf = 0xFF800000u;
 __device__ __forceinline__ uint32_t pick_key(float x) { return x != x ? kPickNan : float_key(x + 0.f); }
 
-// One workgroup per (KV head, sequence).  The first tokens and the newest stay; of the
-// others, c0 .. c1 - 1, the `want` largest do: a histogram of their keys' top digit, then of
-// the lower ones over the keys of the cut's bin, which are listed in LDS where it holds
-// them, fewer digits where the cut falls between two bins.  Then each wavefront goes over a
-// run of the row's pages, a token a lane, counts what it keeps and writes it behind the
-// others'.
+// Top digits of four weights, in the order of their bits (the scan of the bins puts them in
+// that of the keys): -0 as 0, NaN as the top bin.
+__device__ __forceinline__ void top_digits(f32x4 x, uint32_t* d) {
+  const float any = x[0] + x[1] + x[2] + x[3];
+  const bool nan = __ballot(any != any) != 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    d[j] = __float_as_uint(x[j] + 0.f) >> 21;
+    if (nan && x[j] != x[j]) d[j] = 0x3FFu;
+  }
+}
+
+// Whether the wavefront's digits are one, as those of tokens that were never looked at.
+__device__ __forceinline__ bool one_digit(const uint32_t* d) {
+  const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
+  return __ballot(d[0] != d0) == 0 && __ballot(d[1] != d0 || d[2] != d0 || d[3] != d0) == 0;
+}
+
+// A row cut into parts of kPickPart tokens, a workgroup each, and what a part leaves for the
+// others: how many of its competing tokens each bin of the top digit holds and where they
+// begin, two bins a word; how many tokens stay in any case, and whether a page is absent; and
+// the keys, bin by bin.
+constexpr int kPickPart = 4096, kPickWords = kPickBins / 2;
+constexpr int kPickStarts = kPickWords, kPickStay = 2 * kPickWords, kPickKeys = kPickStay + 4;
+constexpr int kPickRecord = kPickKeys + kPickPart;
+constexpr int kPickMaxParts = 512;
+
+__global__ __launch_bounds__(kPickPart / 8) void paged_digits_kernel(
+    const float* __restrict__ mass, int64_t sm_b, int64_t sm_h, const int32_t* __restrict__ lens,
+    const int32_t* __restrict__ table, int64_t st_b, int max_pages, int num_pages, int recent, int first,
+    int Hk, int rows, int parts, uint32_t* __restrict__ records) {
+  constexpr int THREADS = kPickPart / 8, WAVES = THREADS / 64, EACH = kPickBins / THREADS;
+  __shared__ uint32_t s_hist[kPickBins], s_keys[kPickPart], s_wave[WAVES], s_stay;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x % rows, part = blockIdx.x / rows, g = row % Hk, b = row / Hk;
+  const int n = cached_len(lens, b, max_pages), t0 = part * kPickPart;
+  if (t0 >= n) return;
+  const int t1 = min(n - t0, kPickPart) + t0, c0 = min(first, n), c1 = max(n - recent, c0);
+  mass += b * sm_b + g * sm_h;
+  table += b * st_b;
+  f32x4 x[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+    x[r] = *reinterpret_cast<const f32x4*>(mass + min(t0 + 4 * (tid + THREADS * r), (n - 1) & ~3));
+  auto there = [&](int page) { return page >= 0 && page < num_pages; };
+  const int page0 = t0 / kBlock + tid;
+  const bool gap = page0 < (t1 + kBlock - 1) / kBlock && !there(table[page0]);
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) s_hist[tid + THREADS * j] = 0u;
+  if (tid == 0) s_stay = 0u;
+  const bool absent = __builtin_amdgcn_readfirstlane(__syncthreads_or(gap)) != 0;
+  // each token's bin and its place in it
+  uint32_t stay = 0u, d[2][4], rank[2][4];
+  bool in[2][4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int i = t0 + 4 * (tid + THREADS * r), i0 = __builtin_amdgcn_readfirstlane(i);
+    top_digits(x[r], d[r]);
+    const bool all = i0 >= c0 && i0 + 256 <= c1 && !absent;
+    const bool page = all || (i < n && there(table[i / kBlock]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool mid = i + j >= c0 && i + j < c1;
+      in[r][j] = page && mid;
+      stay += page && !mid && i + j < n ? 1u : 0u;
+    }
+    if (all && one_digit(d[r])) {
+      uint32_t at = 0u;
+      if (lane == 0) at = atomicAdd(&s_hist[d[r][0]], 256u);
+      at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rank[r][j] = at + 4 * lane + j;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (in[r][j]) rank[r][j] = atomicAdd(&s_hist[d[r][j]], 1u);
+    }
+  }
+  if (stay != 0u) atomicAdd(&s_stay, stay);
+  __syncthreads();
+  uint32_t* const rec = records + (static_cast<int64_t>(row) * parts + part) * kPickRecord;
+  uint32_t h[EACH], sum = 0u;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) sum += h[j] = s_hist[EACH * tid + j];
+  const uint32_t ex = wave_excl_scan(sum, lane);
+  if (lane == 63) s_wave[wave] = ex + sum;
+  __syncthreads();
+  uint32_t at = ex, total = 0u;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) at += w < wave ? s_wave[w] : 0u, total += s_wave[w];
+#pragma unroll
+  for (int j = 0; j < EACH; j += 2) {
+    rec[(EACH * tid + j) / 2] = h[j] | h[j + 1] << 16;
+    rec[kPickStarts + (EACH * tid + j) / 2] = at | (at + h[j]) << 16;
+    s_hist[EACH * tid + j] = at, s_hist[EACH * tid + j + 1] = at + h[j];
+    at += h[j] + h[j + 1];
+  }
+  if (tid == 0) rec[kPickStay] = s_stay, rec[kPickStay + 1] = absent ? 1u : 0u;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (in[r][j]) s_keys[s_hist[d[r][j]] + rank[r][j]] = pick_key(x[r][j]);
+  __syncthreads();
+  for (uint32_t i = 4 * tid; i < total; i += 4 * THREADS)
+    *reinterpret_cast<u32x4*>(rec + kPickKeys + i) = *reinterpret_cast<const u32x4*>(s_keys + i);
+}
+
+// One workgroup per (KV head, sequence), or, with PARTS, per part of its tokens.  The first
+// tokens and the newest stay; of the others, c0 .. c1 - 1, the `want` largest do: a histogram of
+// their keys' top digit, then of the lower ones over the keys of the cut's bin, which are
+// listed in LDS where it holds them, fewer digits where the cut falls between two bins.  Then
+// each wavefront goes over a run of the row's pages, a token a lane, counts what it keeps and
+// writes it behind the others'.
 //
-// A row is one CU's, and its instructions bound it: how many (a pass over 32K tokens at 40
-// of them per 64 tokens took 8.6 us), and that they are fetched (loops unrolled over loads
-// in flight are code that runs once).  So rows of up to ROW tokens are copied to LDS and
-// gone over by small loops; four tokens a lane and load; membership in a bin, and in what
-// stays, by comparing weights with its ends, not keys; what is the same for all lanes in
-// scalar registers; and what only some tokens need (ends of the range, absent pages, NaN)
-// behind scalar branches.
+// A whole row is one CU's, and its instructions bound it: how many (a pass over 32K tokens at
+// 40 of them per 64 tokens took 8.6 us), and that they are fetched (loops unrolled over loads
+// in flight are code that runs once).  So rows of up to ROW tokens are copied to LDS and gone
+// over by small loops; four tokens a lane and load; membership in a bin, and in what stays, by
+// comparing weights with its ends, not keys; what is the same for all lanes in scalar
+// registers; and what only some tokens need (ends of the range, absent pages, NaN) behind
+// scalar branches.
 //
-// 64 rows of up to 32K tokens (2.6 MB) 26.7 us; four of 600 9.3.
-template <int ROW, int kPickThreads>
+// With PARTS the launch before has counted and sorted each part by the top digit.  Every
+// workgroup adds the counts up, and finds the same cut in the row's keys of one bin; it goes
+// over its own tokens alone.  A read of what that launch left takes over 1 us, whoever wrote
+// it, so 16 parts' counts are on the way at once (four at once: 23 us for 4 rows of 128K
+// tokens where this takes 14).
+//
+// 64 rows of up to 32K tokens (2.6 MB) 9 us and 15, whole 26.7; four of 600 8.5.
+template <int ROW, int kPickThreads, bool PARTS = false>
 __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     const float* __restrict__ mass, int64_t sm_b, int64_t sm_h, const int32_t* __restrict__ lens,
     const int32_t* __restrict__ table, int64_t st_b, int max_pages, int num_pages, int keep, int recent, int first,
-    int32_t* __restrict__ kept, int32_t* __restrict__ new_lens) {
+    int32_t* __restrict__ kept, int32_t* __restrict__ new_lens, int Hk, int rows, int max_parts,
+    const uint32_t* __restrict__ records) {
+  static_assert(!PARTS || (ROW == 0 && kPickMaxParts <= kPickThreads), "parts are read where they are, a thread each");
   constexpr int kPickWaves = kPickThreads / 64, kEach = kPickBins / kPickThreads;
-  constexpr int kPickList = ROW == 0 || ROW > 4096 ? 4096 : ROW;       // keys of the cut's bin that are listed
-  __shared__ uint32_t s_hist[kPickBins], s_list[kPickList], s_wave[2][kPickWaves], s_found[3], s_listed, s_stay;
+  constexpr int kPickList = PARTS ? 1 : ROW == 0 || ROW > 4096 ? 4096 : ROW;       // keys of the cut's bin that are listed
+  __shared__ uint32_t s_hist[kPickBins], s_list[kPickList], s_wave[4][kPickWaves], s_found[3], s_listed, s_stay;
   __shared__ uint8_t s_from[kPickList];
+  __shared__ uint32_t s_seg[PARTS ? kPickMaxParts : 1];                // first key and number of the cut's bin, of each part
   __shared__ f32x4 s_row[ROW > 0 ? ROW / 4 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = blockIdx.x, b = blockIdx.y;
-  const int n = cached_len(lens, b, max_pages);
+  const int row = blockIdx.x % rows, part = PARTS ? blockIdx.x / rows : 0, g = row % Hk, b = row / Hk;
+  const int n = cached_len(lens, b, max_pages), t0 = part * kPickPart;
+  if (PARTS && part > 0 && t0 >= n) return;
   const int c0 = min(first, n), c1 = max(n - recent, c0);
   mass += b * sm_b + g * sm_h;
   table += b * st_b;
-  int32_t* out = kept + (static_cast<int64_t>(b) * gridDim.x + g) * keep;
+  int32_t* out = kept + static_cast<int64_t>(row) * keep;
 
   const int pages = (n + kBlock - 1) / kBlock;
   auto there = [&](int page) { return page >= 0 && page < num_pages; };
@@ -63,7 +182,50 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     }
   }
   bool gap = false;                                   // a page of the row is absent
-  for (int p = tid; p < pages; p += kPickThreads) gap |= !there(table[p]);
+  const int parts = (n + kPickPart - 1) / kPickPart, hi_bin = kPickBins - 1 - kEach * tid;  // this thread's largest bin
+  const bool positive = hi_bin >= kPickBins / 2;
+  auto held = [&](int bin) { return bin >= kPickBins / 2 ? bin - kPickBins / 2 : kPickBins - 1 - bin; };   // of pass 0
+  uint32_t whole[4] = {}, others[4] = {};     // this thread's bins: of the row, of the parts before
+  int stay = 0, base = 0;                             // that stay in any case: of the row, of the parts before
+  if constexpr (PARTS) {
+    records += static_cast<int64_t>(row) * max_parts * kPickRecord;
+    for (int p = lane; p < parts; p += 64) {
+      const uint32_t* rec = records + static_cast<int64_t>(p) * kPickRecord + kPickStay;
+      const int x = rec[0];
+      stay += x;
+      base += p < part ? x : 0;
+      gap |= rec[1] != 0u;
+    }
+    // (two words of a record: this thread's four bins, from the lesser raw digit)
+    static_assert(!PARTS || kEach == 4, "four bins a thread");
+    const uint32_t* mine_at = records + held(positive ? hi_bin - 3 : hi_bin) / 2;
+    for (int p0 = 0; p0 < parts; p0 += 16) {
+      u32x2 y[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        y[r] = *reinterpret_cast<const u32x2*>(mine_at + static_cast<int64_t>(min(p0 + r, parts - 1)) * kPickRecord);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t all = p0 + r < parts ? ~0u : 0u, prior = p0 + r < part ? ~0u : 0u;
+        const uint32_t z[4] = {y[r][0] & 0xFFFFu, y[r][0] >> 16, y[r][1] & 0xFFFFu, y[r][1] >> 16};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = z[j];
+          whole[j] += x & all, others[j] += x & prior;
+        }
+      }
+    }
+    if (positive) {                                   // their bins fall as the digits rise
+      const uint32_t w[4] = {whole[3], whole[2], whole[1], whole[0]}, o[4] = {others[3], others[2], others[1], others[0]};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) whole[j] = w[j], others[j] = o[j];
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) stay += __shfl_xor(stay, off, 64), base += __shfl_xor(base, off, 64);
+    stay = __builtin_amdgcn_readfirstlane(stay), base = __builtin_amdgcn_readfirstlane(base);
+  } else {
+    for (int p = tid; p < pages; p += kPickThreads) gap |= !there(table[p]);
+  }
   for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0u;
   if (tid == 0) s_listed = 0u, s_stay = 0u;
   const bool absent = __builtin_amdgcn_readfirstlane(__syncthreads_or(gap)) != 0;
@@ -98,20 +260,32 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     }
   };
   auto mine = [&](uint64_t m) { return (m >> lane & 1) != 0; };
-  // f(first of 256 tokens, the lane's first, its four weights) over this wavefront's part of the row
+  // this wavefront's runs of 256 tokens: of the row, and of the part, whose tokens it writes
   const int runs = (n + 255) / 256, share = (runs + kPickWaves - 1) / kPickWaves;
   const int q0 = min(wave * share, runs), q1 = min(q0 + share, runs);
-  auto run_over = [&](auto f) __attribute__((always_inline)) {
+  constexpr int PART_RUNS = kPickPart / 256, PART_SHARE = (PART_RUNS + kPickWaves - 1) / kPickWaves;
+  const int w0 = PARTS ? min(t0 / 256 + wave * PART_SHARE, runs) : q0, w1 = PARTS ? min(w0 + PART_SHARE, runs) : q1;
+  // f(first of 256 tokens, the lane's first, its four weights) over runs r0 .. r1 - 1
+  auto run_over = [&](int r0, int r1, auto f) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int at = q0; at < q1; at += RUN) {
+    for (int at = r0; at < r1; at += RUN) {
       f32x4 x[RUN];
 #pragma unroll
       for (int r = 0; r < RUN; ++r) x[r] = weights(256 * (at + r) + 4 * lane);
 #pragma unroll
       for (int r = 0; r < RUN; ++r) {
-        if (at + r >= q1) break;
+        if (at + r >= r1) break;
         f(256 * (at + r), 256 * (at + r) + 4 * lane, x[r]);
       }
+    }
+  };
+  // f(key) over the cut's bin of the first `upto` parts
+  auto segments = [&](int upto, auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int p = wave; p < upto; p += kPickWaves) {
+      const uint32_t seg = s_seg[p], size = seg >> 16;
+      const uint32_t* keys = records + static_cast<int64_t>(p) * kPickRecord + kPickKeys + (seg & 0xFFFFu);
+      for (uint32_t i = lane; i < size; i += 64) f(keys[i]);
     }
   };
   int more = 0, same = 0;                             // of this lane's: above the cut, and tied
@@ -120,41 +294,34 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
   uint32_t least = 0u, ties = 0u;                     // keys above least stay, and the first ties equal to it
   uint32_t top = 0u;                                  // keys of the cut's bin of the top digit
   int total = 0;                                      // tokens with a page
+  int sure = kPickBins;                               // tokens of this bin of the top digit and those above stay
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : kPickBins;
     if (pass == 0) {
-      if (absent) {                                   // those that stay and are there
-        uint32_t stay = 0u;
-        for (int i = tid; i < n - (c1 - c0); i += kPickThreads) {
-          const int t = i < c0 ? i : i + (c1 - c0);
-          stay += there(table[t / kBlock]) ? 1u : 0u;
+      if constexpr (!PARTS) {
+        if (absent) {                                 // those that stay and are there
+          uint32_t have = 0u;
+          for (int i = tid; i < n - (c1 - c0); i += kPickThreads) {
+            const int t = i < c0 ? i : i + (c1 - c0);
+            have += there(table[t / kBlock]) ? 1u : 0u;
+          }
+          if (have != 0u) atomicAdd(&s_stay, have);
         }
-        if (stay != 0u) atomicAdd(&s_stay, stay);
-      }
-      visit([&](f32x4 x, const uint64_t* in, bool all) __attribute__((always_inline)) {
-        // the bits' top digit, which the scan below puts in order: -0 as 0, NaN as the top bin
-        uint32_t d[4];
-        const float any = x[0] + x[1] + x[2] + x[3];
-        const bool nan = __ballot(any != any) != 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          d[j] = __float_as_uint(x[j] + 0.f) >> 21;
-          if (nan && x[j] != x[j]) d[j] = 0x3FFu;
-        }
-        // one bin for all of them, as of tokens that were never looked at: one addition
-        const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
-        if (all) {
-          if (__ballot(d[0] != d0) == 0 && __ballot(d[1] != d0 || d[2] != d0 || d[3] != d0) == 0) {
-            if (lane == 0) atomicAdd(&s_hist[d0], 256u);
+        visit([&](f32x4 x, const uint64_t* in, bool all) __attribute__((always_inline)) {
+          uint32_t d[4];
+          top_digits(x, d);
+          if (all && one_digit(d)) {
+            if (lane == 0) atomicAdd(&s_hist[d[0]], 256u);
             return;
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) atomicAdd(&s_hist[d[j]], 1u);
-          return;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (mine(in[j])) atomicAdd(&s_hist[d[j]], 1u);
+          for (int j = 0; j < 4; ++j)
+            if (mine(in[j])) atomicAdd(&s_hist[d[j]], 1u);
+        });
+      }
+    } else if (PARTS) {
+      segments(parts, [&](uint32_t k) {
+        if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
       });
     } else if (top <= kPickList) {
       const uint32_t listed = min(s_listed, static_cast<uint32_t>(kPickList));
@@ -174,27 +341,26 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     __syncthreads();
     // bins from the largest: thread t holds kEach from 2047 - kEach t down; the bits of a positive
     // weight's key are its own but for the sign, those of a negative one's turned
-    const int hi = kPickBins - 1 - kEach * tid;
-    auto held = [&](int bin) { return pass > 0 ? bin : (bin >= 1024 ? bin - 1024 : 2047 - bin); };
     uint32_t h[kEach], sum = 0u;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) sum += h[j] = s_hist[held(hi - j)];
+    for (int j = 0; j < kEach; ++j) sum += h[j] = PARTS && pass == 0 ? whole[j & 3] : s_hist[pass > 0 ? hi_bin - j : held(hi_bin - j)];
     const uint32_t ex = wave_excl_scan(sum, lane);
     if (lane == 63) s_wave[0][wave] = ex + sum;
     __syncthreads();
     uint32_t before = ex;
     for (int w = 0; w < wave; ++w) before += s_wave[0][w];
     if (pass == 0) {
-      const int stay = absent ? __builtin_amdgcn_readfirstlane(s_stay) : n - (c1 - c0);
+      if constexpr (!PARTS) stay = absent ? __builtin_amdgcn_readfirstlane(s_stay) : n - (c1 - c0);
       uint32_t all = 0u;
       for (int w = 0; w < kPickWaves; ++w) all += s_wave[0][w];
       total = stay + __builtin_amdgcn_readfirstlane(all);
       want = keep - stay;
+      if (total <= keep) sure = 0;
       if (total <= keep || want == 0u) break;         // all that compete stay, or none
     }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      if (before < want && want <= before + h[j]) s_found[0] = hi - j, s_found[1] = before, s_found[2] = h[j];
+      if (before < want && want <= before + h[j]) s_found[0] = hi_bin - j, s_found[1] = before, s_found[2] = h[j];
       before += h[j];
     }
     for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0u;
@@ -204,6 +370,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     want -= __builtin_amdgcn_readfirstlane(s_found[1]);
     const uint32_t bin = __builtin_amdgcn_readfirstlane(s_found[2]);
     least = prefix, ties = want;
+    if (pass == 0) sure = static_cast<int>(prefix >> 21) + (want == bin ? 0 : 1);
     if (want == bin) {                                // the whole bin stays
       least = prefix - 1u, ties = 0u;
       break;
@@ -213,7 +380,13 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
       // the bin's keys, and what each wavefront holds above the bin
       const bool finite = prefix >= ~kPickInf && prefix < kPickInf, fits = top <= kPickList;
       const float lo = key_float(prefix), end = key_float(prefix + (1u << 21));
-      run_over([&](int i0, int i, f32x4 x) __attribute__((always_inline)) {
+      if constexpr (PARTS) {
+        if (tid < parts) {
+          const uint32_t* rec = records + static_cast<int64_t>(tid) * kPickRecord;
+          const int at = held(prefix >> 21), sh = 16 * (at & 1);
+          s_seg[tid] = (rec[kPickStarts + at / 2] >> sh & 0xFFFFu) | (rec[at / 2] >> sh & 0xFFFFu) << 16;
+        }
+      } else run_over(q0, q1, [&](int i0, int i, f32x4 x) __attribute__((always_inline)) {
         bool over[4], in[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -251,7 +424,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     __syncthreads();
   }
   const int count = min(total, keep);
-  if (tid == 0 && g == 0) new_lens[b] = count;
+  if (tid == 0 && g == 0 && part == 0) new_lens[b] = count;
   if (total > keep && want == 0u && ties == 0u && least == 0u) least = 0xFFFFFFFFu;   // none that compete
   __syncthreads();
 
@@ -261,8 +434,8 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
   const float low = total <= keep ? __uint_as_float(0x7FC00000u) : key_float(least + 1u), tie = key_float(least);
   const bool plain = !none && !only_nan && !absent;
   // f(the lane's first token, masks of the lanes whose j-th stays above the cut, and ties)
-  auto pass_over = [&](auto f) __attribute__((always_inline)) {
-    run_over([&](int i0, int i, f32x4 x) __attribute__((always_inline)) {
+  auto pass_over = [&](int r0, int r1, auto f) __attribute__((always_inline)) {
+    run_over(r0, r1, [&](int i0, int i, f32x4 x) __attribute__((always_inline)) {
       uint64_t gt[4], eq[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -289,9 +462,23 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
       f(i, gt, eq);
     });
   };
-  // what the wavefront keeps: from the list where there is one
-  if (total > keep && top != 0u && top <= kPickList) {
-    const uint32_t listed = min(s_listed, static_cast<uint32_t>(kPickList));
+  auto count_over = [&](int r0, int r1, int& gts, int& eqs) __attribute__((always_inline)) {
+    pass_over(r0, r1, [&](int, const uint64_t* gt, const uint64_t* eq) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) gts += mine(gt[j]) ? 1 : 0, eqs += mine(eq[j]) ? 1 : 0;
+    });
+  };
+  const bool listed_all = total > keep && top != 0u && top <= kPickList;
+  const uint32_t listed = listed_all ? min(s_listed, static_cast<uint32_t>(kPickList)) : 0u;
+  int more0 = 0, same0 = 0;                           // and of the parts before
+  if constexpr (PARTS) {
+    count_over(w0, w1, more, same);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) more0 += hi_bin - j >= sure ? others[j & 3] : 0u;
+    if (top != 0u)
+      segments(part, [&](uint32_t k) { more0 += k > least ? 1 : 0, same0 += k == least ? 1 : 0; });
+  } else if (listed_all) {
+    // what the wavefront keeps: from the list where there is one
     for (uint32_t at = 0; at < listed; at += 64) {
       const bool own = at + lane < listed && s_from[min(at + lane, listed - 1u)] == wave;
       const uint32_t k = s_list[min(at + lane, listed - 1u)];
@@ -300,23 +487,23 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
     }
   } else {
     more = 0;
-    pass_over([&](int, const uint64_t* gt, const uint64_t* eq) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        more += mine(gt[j]) ? 1 : 0;
-        same += mine(eq[j]) ? 1 : 0;
-      }
-    });
+    count_over(q0, q1, more, same);
   }
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) more += __shfl_xor(more, off, 64), same += __shfl_xor(same, off, 64);
+  for (int off = 32; off >= 1; off >>= 1) {
+    more += __shfl_xor(more, off, 64), same += __shfl_xor(same, off, 64);
+    if constexpr (PARTS) more0 += __shfl_xor(more0, off, 64), same0 += __shfl_xor(same0, off, 64);
+  }
   if (lane == 0) s_wave[0][wave] = more, s_wave[1][wave] = same;
+  if (PARTS && lane == 0) s_wave[2][wave] = more0, s_wave[3][wave] = same0;
   __syncthreads();
-  int at = 0, tied = 0;                               // kept and tied tokens of the wavefronts before
+  int at = base, tied = 0;                            // kept and tied tokens before this wavefront's
   for (int w = 0; w < wave; ++w) at += s_wave[0][w], tied += s_wave[1][w];
+  if constexpr (PARTS)
+    for (int w = 0; w < kPickWaves; ++w) at += s_wave[2][w], tied += s_wave[3][w];
   at = __builtin_amdgcn_readfirstlane(at + min(tied, static_cast<int>(ties)));
   tied = __builtin_amdgcn_readfirstlane(tied);
-  pass_over([&](int i, const uint64_t* gt, const uint64_t* eq) __attribute__((always_inline)) {
+  pass_over(w0, w1, [&](int i, const uint64_t* gt, const uint64_t* eq) __attribute__((always_inline)) {
     uint64_t stay[4] = {gt[0], gt[1], gt[2], gt[3]};
     if (ties != 0u && tied < static_cast<int>(ties) && (eq[0] | eq[1] | eq[2] | eq[3]) != 0) {
       // the first `ties` of the row
@@ -341,6 +528,7 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
       }
   });
   const int end = max_pages * kBlock;
+  if (part > 0) return;
   for (int i = count + tid; i < keep; i += kPickThreads) out[i] = end;
 }
 
@@ -447,21 +635,45 @@ __global__ __launch_bounds__(256) void paged_move_kernel(
   }
 }
 
+// Parts of a row, 0 where a workgroup has it whole.  Few long rows leave most CUs idle: with
+// the move, 4 rows of 64K tokens take 38 us in parts and 58 whole, of 128K 45 and 93, 32 rows
+// of 32K 44 and 51.  At 64 rows of 64K they meet (124 and 123); 128 rows of 32K take 122 and
+// 110, 4 rows of 16K 30 and 29.
+static int paged_evict_parts(int B, int Hk, int max_pages) {
+  const int parts = (max_pages + kPickPart / kBlock - 1) / (kPickPart / kBlock);
+  return max_pages > 256 && parts <= kPickMaxParts && static_cast<int64_t>(B) * Hk <= 64 ? parts : 0;
+}
+
+int64_t paged_evict_ws_elems(int B, int Hk, int max_pages) {
+  return B * static_cast<int64_t>(Hk) * paged_evict_parts(B, Hk, max_pages) * kPickRecord;
+}
+
 hipError_t launch_paged_evict(const PagedCache& c, const float* mass, int64_t sm_b, int64_t sm_h,
                               const int32_t* lens, const int32_t* table, int64_t st_b, int B, int max_pages,
                               const int32_t* new_table, int64_t sn_b, int new_pages, int keep, int recent, int first,
                               int32_t* kept, int32_t* new_lens, float* new_mass, int64_t so_b, int64_t so_h,
-                              hipStream_t stream) {
-  // Rows of up to 2048 tokens have four wavefronts, whose barriers are shorter and several of
-  // which share a CU (512 rows of 1000 tokens 10.8 us, 128 of 4096 12.4; with 16 wavefronts the
-  // 512 took 18.9); 8192 and 32768 weights fit the LDS of half a CU and of one.
-  const int threads = max_pages <= 32 ? 256 : 1024;
-  const auto pick = max_pages <= 32    ? paged_pick_kernel<2048, 256>
-                    : max_pages <= 128 ? paged_pick_kernel<8192, 1024>
-                    : max_pages <= 512 ? paged_pick_kernel<32768, 1024>
-                                       : paged_pick_kernel<0, 1024>;
-  pick<<<dim3(c.Hk, B), threads, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages, c.num_pages, keep,
-                                              recent, first, kept, new_lens);
+                              float* workspace, hipStream_t stream) {
+  const int rows = B * c.Hk;
+  if (const int parts = paged_evict_parts(B, c.Hk, max_pages); parts > 0) {
+    uint32_t* const records = reinterpret_cast<uint32_t*>(workspace);
+    paged_digits_kernel<<<rows * parts, kPickPart / 8, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages,
+                                                                    c.num_pages, recent, first, c.Hk, rows, parts,
+                                                                    records);
+    paged_pick_kernel<0, 512, true><<<rows * parts, 512, 0, stream>>>(
+        mass, sm_b, sm_h, lens, table, st_b, max_pages, c.num_pages, keep, recent, first, kept, new_lens, c.Hk, rows,
+        parts, records);
+  } else {
+    // Rows of up to 2048 tokens have four wavefronts, whose barriers are shorter and several of
+    // which share a CU (512 rows of 1000 tokens 10.8 us, 128 of 4096 12.4; with 16 wavefronts the
+    // 512 took 18.9); 8192 and 32768 weights fit the LDS of half a CU and of one.
+    const int threads = max_pages <= 32 ? 256 : 1024;
+    const auto pick = max_pages <= 32    ? paged_pick_kernel<2048, 256>
+                      : max_pages <= 128 ? paged_pick_kernel<8192, 1024>
+                      : max_pages <= 512 ? paged_pick_kernel<32768, 1024>
+                                         : paged_pick_kernel<0, 1024>;
+    pick<<<rows, threads, 0, stream>>>(mass, sm_b, sm_h, lens, table, st_b, max_pages, c.num_pages, keep, recent,
+                                       first, kept, new_lens, c.Hk, rows, 0, nullptr);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid(new_pages, c.Hk, B);

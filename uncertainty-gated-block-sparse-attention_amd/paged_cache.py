@@ -419,7 +419,11 @@ def paged_evict(cache, mass, block_table, seq_lens, new_table, keep, recent=0, f
     kept = torch.empty((B, Hk, max(keep, 0)), dtype=torch.int32, device=device)
     lens = torch.empty(B, dtype=torch.int32, device=device)
     new_mass = torch.empty((B, Hk, PAGE * new_pages), dtype=torch.float32, device=device)
-    _launch(cache, "paged_evict", _capi.lib().ugbsa_paged_evict, mass.data_ptr(), sm_b, sm_h, seq_lens.data_ptr(),
+    lib = _capi.lib()
+    n = lib.ugbsa_paged_evict_workspace_elems(B, Hk, max_pages)
+    ws = torch.empty(n, dtype=torch.float32, device=device) if n else None
+    _launch(cache, "paged_evict", lib.ugbsa_paged_evict, mass.data_ptr(), sm_b, sm_h, seq_lens.data_ptr(),
             block_table.data_ptr(), st_b, B, max_pages, new_table.data_ptr(), new_table.stride(0), new_pages, keep,
-            recent, first, kept.data_ptr(), lens.data_ptr(), new_mass.data_ptr(), *new_mass.stride()[:2])
+            recent, first, kept.data_ptr(), lens.data_ptr(), new_mass.data_ptr(), *new_mass.stride()[:2],
+            _capi.ptr(ws), n)
     return PagedEviction(kept, lens, new_mass)
