@@ -117,18 +117,19 @@ def _check_unwatched(*tensors):
 
 
 def _operand(name, t, rot, like):
-    """A 16-bit tensor of q's dtype, tokens and head_dim that the kernel reads in place."""
+    """A 16-bit tensor of q's dtype, tokens and head_dim that the kernel reads in place, and its (b, h, m, d)
+    strides."""
     assert t.dtype in (torch.bfloat16, torch.float16) and t.dtype is like.dtype, \
         f"{name}: bf16 or fp16 required, q's, got {t.dtype}"
     assert t.get_device() == rot._call[1], f"{name} must be on the table's device"
-    st = t.stride()
-    if st[-1] == 1 and not (t.data_ptr() & 15 or t.is_neg() or any(s & 7 for s in st[:-1])):
-        return t
+    st = _strides(t)
+    if st[3] == 1 and not (t.data_ptr() & 15 or (st[0] | st[1] | st[2]) & 7 or t.is_neg()):
+        return t, st
     if t.is_neg():
         t = t.resolve_neg()
     if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]):
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    return t, _strides(t)
 
 
 def _span(t):
@@ -240,12 +241,12 @@ def _turn(rot, positions, q, k, out, inverse):
         "positions: int32 on the table's device expected"
     assert positions.shape == want, f"positions {list(want)} expected, got {list(positions.shape)}"
     assert M <= 1 or positions.stride(-1) == 1, "positions: a row's entries must be contiguous"
-    qc, kc, Hk = _operand("q", q, rot, q), None, 0
+    (qc, q_st), kc, Hk = _operand("q", q, rot, q), None, 0
     if k is not None:
         Hk = k.shape[1] if k.dim() == len(shape) else 0
         assert Hk >= 1 and tuple(k.shape) == ((M, Hk, D) if len(shape) == 3 else (B, Hk, M, D)), \
             f"k {'[T, Hk, D]' if len(shape) == 3 else '[B, Hk, M, D]'} with q's tokens expected, got {list(k.shape)}"
-        kc = _operand("k", k, rot, q)
+        kc, k_st = _operand("k", k, rot, q)
     if out is None:
         qo, ko = _like(qc), None if k is None else _like(kc)
     else:
@@ -257,9 +258,9 @@ def _turn(rot, positions, q, k, out, inverse):
                 torch.autograd.graph.increment_version(o)
         qo, ko = (*outs, None)[:2]
     if M:
-        kv = _NONE if k is None else (kc.data_ptr(), *_strides(kc), ko.data_ptr(), *_strides(ko), Hk)
+        kv = _NONE if k is None else (kc.data_ptr(), *k_st, ko.data_ptr(), *_strides(ko), Hk)
         _launch(rot, "rotary", _capi.lib().ugbsa_rotary, positions.data_ptr(),
-                positions.stride(0) if len(want) == 2 else 0, qc.data_ptr(), *_strides(qc), qo.data_ptr(),
+                positions.stride(0) if len(want) == 2 else 0, qc.data_ptr(), *q_st, qo.data_ptr(),
                 *_strides(qo), H, *kv, B, M, D, _capi.dtype_code(q.dtype), inverse)
     return qo if k is None else (qo, ko)
 
