@@ -74,8 +74,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads 
   if (turns) {
     const double pos = positions[b * sp_b + m];
     float cs[8], sn[8];
+    // all bits of the pairs past the table's, which keep theirs (by branches the compiler made 27 KB
+    // of code of this, at one wavefront per SIMD: 8192 tokens 104 us, now 33)
+    uint32_t passes[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
+      passes[i] = LAYOUT == kPairs && (i < 4 ? da : db) / 2 + i % 4 >= pairs ? ~0u : 0u;
       const int j = LAYOUT == kPairs ? min((i < 4 ? da : db) / 2 + i % 4, pairs - 1) : da + i;
       turn_cos_sin(pos, t.turns[j], t.attention, cs[i], sn[i]);
       sn[i] *= sign;
@@ -87,9 +91,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads 
         if constexpr (LAYOUT == kPairs) {
           float a, c;
           turn_pair(E::to_f32(va[i][w] & 0xFFFFu), E::to_f32(va[i][w] >> 16), cs[w], sn[w], a, c);
-          if (da / 2 + w < pairs) va[i][w] = E::pack2(a, c);
+          va[i][w] = (va[i][w] & passes[w]) | (E::pack2(a, c) & ~passes[w]);
           turn_pair(E::to_f32(vb[i][w] & 0xFFFFu), E::to_f32(vb[i][w] >> 16), cs[4 + w], sn[4 + w], a, c);
-          if (db / 2 + w < pairs) vb[i][w] = E::pack2(a, c);
+          vb[i][w] = (vb[i][w] & passes[4 + w]) | (E::pack2(a, c) & ~passes[4 + w]);
         } else {
           uint32_t lo = va[i][w], hi = vb[i][w];
           turn_words<E>(lo, hi, cs + 2 * w, sn + 2 * w);
@@ -105,7 +109,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads 
 
 // Half layout whose halves are no whole vectors: a thread has W neighbouring pairs of a token
 // and its heads, or W dims that pass (vectors at addresses of four bytes' alignment, with
-// the pairs that are left one by one, took 94 us for 134 MB where this takes XX).
+// the pairs that are left one by one, took 94 us for 134 MB where this takes 38).
 template <typename E, int W, int HPT>
 __global__ __launch_bounds__(256) void rotary_odd_kernel(RotaryHeads q, RotaryHeads k, RotaryTable t,
                                                          const int32_t* __restrict__ positions, int64_t sp_b,
@@ -155,10 +159,11 @@ __global__ __launch_bounds__(256) void rotary_odd_kernel(RotaryHeads q, RotaryHe
     }
 }
 
-// A thread takes four heads where that leaves the card some thousand wavefronts, else one
-// (512 tokens, 28/4 heads XX us).  Tensors of more than 320 MB, in and out, go past the
-// memory-side cache: 2 x 8191 tokens, 40/8 heads, head_dim 128 (402 MB a launch) 79 -> 70 us;
-// 67 MB 21 -> 23, 300 MB 70 -> 74.
+// Where it leaves the card some thousand wavefronts a thread takes two heads (512 tokens, 28/4
+// heads 5.2 us of one each; 32K tokens, 537 MB, 95 us of two, 98 of four, 103 of one), or four where
+// halves are no whole vectors (8192 tokens, 100 of 128 dims, 38 and 68 of one).  Tensors of more
+// than 320 MB, in and out, go past the memory-side cache: 2 x 8191 tokens, 40/8 heads,
+// head_dim 128 (402 MB a launch) 79 -> 70 us; 67 MB 21 -> 23, 300 MB 70 -> 74.
 template <typename E>
 static hipError_t launch_rotary_t(const RotaryTable& t, const int32_t* positions, int64_t sp_b,
                                   const RotaryHeads& q, const RotaryHeads& k, int B, int M, int D, bool inverse,
@@ -167,8 +172,9 @@ static hipError_t launch_rotary_t(const RotaryTable& t, const int32_t* positions
   const float sign = inverse ? -1.f : 1.f;
   const int bits = D == 64 ? 2 : (D == 128 ? 3 : 4);
   const bool many = (static_cast<uint64_t>(toks) * heads << bits) >= 1u << 21;
-  const uint32_t groups = many ? (heads + 3) / 4 : heads, rows = toks * groups;
-  if (!t.interleaved && t.pairs % 8) {
+  const bool odd = !t.interleaved && t.pairs % 8;
+  const uint32_t each = !many ? 1 : (odd ? 4 : 2), groups = (heads + each - 1) / each, rows = toks * groups;
+  if (odd) {
     const uint32_t items = (D - t.pairs) / (t.pairs % 2 ? 1 : 2);
     const uint32_t grid = static_cast<uint32_t>((static_cast<uint64_t>(rows) * items + 255) / 256);
     const auto kernel = t.pairs % 2 ? (many ? rotary_odd_kernel<E, 1, 4> : rotary_odd_kernel<E, 1, 1>)
@@ -179,7 +185,7 @@ static hipError_t launch_rotary_t(const RotaryTable& t, const int32_t* positions
   const uint32_t units = rows << bits;
   const bool past = many && static_cast<uint64_t>(toks) * heads * D * 4 > 320ull << 20;
 #define UGBSA_ROT(L_) \
-  (past ? rotary_kernel<E, L_, 4, true> : (many ? rotary_kernel<E, L_, 4, false> : rotary_kernel<E, L_, 1, false>))
+  (past ? rotary_kernel<E, L_, 2, true> : (many ? rotary_kernel<E, L_, 2, false> : rotary_kernel<E, L_, 1, false>))
   const auto kernel = t.interleaved ? UGBSA_ROT(kPairs) : UGBSA_ROT(kHalves);
 #undef UGBSA_ROT
   kernel<<<(units + 255) / 256, 256, 0, stream>>>(q, k, t, positions, sp_b, M, D, bits, groups, units, sign);
