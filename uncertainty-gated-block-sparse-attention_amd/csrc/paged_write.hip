@@ -3,7 +3,8 @@
 // Both are copies bound by HBM: a written token costs 4 D bytes read and 2 D
 // (e4m3) or 4 D written per head, a read one the reverse.  Six prompts of up to 32K
 // tokens, 4 heads, into e4m3 (232 MB): 48 us, 4.8 TB/s; 64K tokens of 8 heads back
-// (404 MB): 74.7 us, 5.4 TB/s; a copy of 256 MiB runs at 5.3.
+// (404 MB): 74.7 us, 5.4 TB/s; a copy of 256 MiB runs at 5.3.  37K tokens of 4
+// heads into e2m1 (97 MB) 27 us, and back into six rows of 17K (211 MB) 31.
 #include "paged.h"
 #include "rotary.h"
 
@@ -17,7 +18,8 @@ __device__ __forceinline__ int touched_pages(int len, int n_new) {
 // A thread's eight dims d0 .. of the token at src + 0 .. (raw: their 16-bit values, src
 // their address), turned.
 template <typename E>
-__device__ __forceinline__ u32x4 turned8(u32x4 raw, const uint16_t* src, int d0, const RotaryTable& t, int position) {
+__device__ __forceinline__ u32x4 turned8(u32x4 raw, const uint16_t* src, int d0, const RotaryTable& t, int position,
+                                         int lane) {
   const int pairs = t.pairs;
   if (d0 >= 2 * pairs) return raw;
   const double pos = position;
@@ -32,16 +34,37 @@ __device__ __forceinline__ u32x4 turned8(u32x4 raw, const uint16_t* src, int d0,
     }
     return raw;
   }
-  // the other halves: eight values in a row where the halves are whole vectors
-  u32x4 other = {0u, 0u, 0u, 0u};
   if (pairs % 8 == 0) {
-    other = *reinterpret_cast<const u32x4*>(src + (d0 < pairs ? pairs : -pairs));
-  } else {
+    // halves that are whole vectors: the lane with the pairs' other halves works out four of the
+    // eight turns, this one the others (37K tokens of 4 heads in 16 bits: 59 us where each worked
+    // out all, 49 so)
+    const bool low = d0 < pairs;
+    const int peer = lane + (low ? pairs : -pairs) / 8, j0 = low ? d0 : d0 - pairs + 4;
+    float cs[8], sn[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = d0 + i, o = d < pairs ? d + pairs : d - pairs;
-      if (d < 2 * pairs) other[i / 2] |= static_cast<uint32_t>(src[o - d0]) << (16 * (i % 2));
+    for (int i = 0; i < 4; ++i) {
+      float c, s;
+      turn_cos_sin(pos, t.turns[j0 + i], t.attention, c, s);
+      const float pc = __shfl(c, peer, 64), ps = __shfl(s, peer, 64);
+      cs[i] = low ? c : pc, cs[4 + i] = low ? pc : c;
+      sn[i] = low ? -s : ps, sn[4 + i] = low ? -ps : s;
     }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t other = __shfl(raw[w], peer, 64);
+      // fma(a, cos, -(b sin)) of the lower half, fma(b, cos, a sin) of the upper, as turn_pair
+      float y0 = __builtin_fmaf(E::to_f32(raw[w] & 0xFFFFu), cs[2 * w], E::to_f32(other & 0xFFFFu) * sn[2 * w]);
+      float y1 = __builtin_fmaf(E::to_f32(raw[w] >> 16), cs[2 * w + 1], E::to_f32(other >> 16) * sn[2 * w + 1]);
+      asm("" : "+v"(y0), "+v"(y1));
+      raw[w] = E::pack2(y0, y1);
+    }
+    return raw;
+  }
+  u32x4 other = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = d0 + i, o = d < pairs ? d + pairs : d - pairs;
+    if (d < 2 * pairs) other[i / 2] |= static_cast<uint32_t>(src[o - d0]) << (16 * (i % 2));
   }
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -68,7 +91,7 @@ __device__ __forceinline__ u32x4 turned8(u32x4 raw, const uint16_t* src, int d0,
 // the summary needs no atomics.  A thread takes 8 dims of every (256 / (D / 8))-th
 // token; a scale is a maximum over neighbouring lanes, the D / 8 of a token or the four
 // of 32 dims.  TURN: keys are turned by their positions first (rotary.h) and rounded to
-// the 16-bit format, as ugbsa_rotary does: a thread loads its pairs' other halves too.
+// the 16-bit format, as ugbsa_rotary does.
 template <typename E, int D, int KIND, bool TURN>
 __global__ __launch_bounds__(256) void paged_write_kernel(
     PagedCache c, const uint16_t* __restrict__ k, int64_t sk_t, int64_t sk_h,
@@ -135,16 +158,34 @@ __global__ __launch_bounds__(256) void paged_write_kernel(
 #pragma unroll
   for (int j = 0; j < 8; ++j) mx[j] = -INFINITY, mn[j] = INFINITY;
   const int64_t head = static_cast<int64_t>(page) * c.Hk + h;
-  for (int s = s0 + rg; s < s1; s += RG) {
+  auto source = [&](int kv, int64_t tok) {
+    return (kv ? v + tok * sv_t + h * sv_h : k + tok * sk_t + h * sk_h) + 8 * ch;
+  };
+  // TURN: the next token's values and position are on the way while this one's are turned (the
+  // same call 49 -> 44 us; 34 without turning)
+  u32x4 ahead[2];
+  int at_ahead = 0;
+  auto fetch = [&](int s) __attribute__((always_inline)) {
+    if (s >= s1) return;
     const int64_t tok = t + s - s0;
 #pragma unroll
+    for (int kv = 0; kv < 2; ++kv) ahead[kv] = stream_load<true>(reinterpret_cast<const u32x4*>(source(kv, tok)));
+    at_ahead = positions != nullptr ? positions[tok] : blk * kBlock + s;
+  };
+  if constexpr (TURN) fetch(s0 + rg);
+  for (int s = s0 + rg; s < s1; s += RG) {
+    const int64_t tok = t + s - s0;
+    u32x4 now[2];
+    if constexpr (TURN) {
+      now[0] = turned8<E>(ahead[0], source(0, tok), 8 * ch, rot, at_ahead, tid & 63);
+      now[1] = ahead[1];
+      fetch(s + RG);
+    }
+#pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      const uint16_t* src = (kv ? v + tok * sv_t + h * sv_h : k + tok * sk_t + h * sk_h) + 8 * ch;
-      u32x4 raw = stream_load<true>(reinterpret_cast<const u32x4*>(src));
-      if constexpr (TURN) {
-        if (kv == 0)
-          raw = turned8<E>(raw, src, 8 * ch, rot, positions != nullptr ? positions[tok] : blk * kBlock + s);
-      }
+      u32x4 raw;
+      if constexpr (TURN) raw = now[kv];
+      else raw = stream_load<true>(reinterpret_cast<const u32x4*>(source(kv, tok)));
       const int64_t at = page * (kv ? c.sv_p : c.sk_p) + h * (kv ? c.sv_h : c.sk_h) +
                          s * (kv ? c.sv_n : c.sk_n) + (KIND == kPagesE2m1 ? 4 * ch : 8 * ch);
       float x[8];
