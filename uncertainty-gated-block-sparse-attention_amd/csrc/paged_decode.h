@@ -8,8 +8,10 @@
 // 16-bit format.
 //
 // Bound by memory: 32 sequences of 64K tokens, 40/8 heads, e4m3 (4.3 GB) 698 us, 6.2
-// TB/s; 24 of up to 16K, bf16 (375 MB) 69.5 us, 5.4 TB/s with the joining launch; one of
-// 1000 tokens 11 us, two launches of about 4 us.
+// TB/s; e2m1 (2.3 GB) 364 us, 6.3; 24 of up to 16K, bf16 (375 MB) 69.5 us, 5.4 TB/s with the
+// joining launch; 24 of up to 16K, 16/2 heads of 256 dims, e2m1 (50 MB) 20.5 us, where starting
+// (lengths, table, pages: reads one behind another) and joining take as long as the pages; one
+// of 1000 tokens 11 us, two launches of about 4 us, e2m1 9.5, one launch.
 //
 // MASS: each cached token of a KV head gets the sum over its query heads of the weight
 // that the token had,

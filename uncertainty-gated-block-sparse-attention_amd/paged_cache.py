@@ -15,6 +15,10 @@ before they are rounded to codes), kept up to date as tokens are written:
     out = paged_decode(q, cache, block_table, seq_lens, scale, sel.kv_idx, sel.counts)
     k, v = paged_read(cache, block_table, seq_lens, N)             # [B, Hk, N, D], contiguous
 
+A cache that has to stay within its pages follows the attention weights of its tokens
+(``paged_decode(..., mass=)``) and is cut back to the heaviest by ``paged_evict``; keys can be turned by
+their positions on the way in (``paged_write(..., rotary=, positions=)``).
+
 ``block_table`` [B, max_pages] int32 and ``seq_lens`` [B] int32 live on the device: no call reads
 them on the host, and every call is asynchronous on the current stream and can be captured in a
 graph.  Lengths outside [0, 64 * max_pages] are taken as the nearer end; table entries outside the
