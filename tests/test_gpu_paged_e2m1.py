@@ -252,6 +252,28 @@ def poison(cache, table, lens):
         t.masked_fill_(dead.view(P, 1, 1, 64), 255)
 
 
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("D,r", [(64, 64), (64, 16), (64, 48), (128, 128), (128, 48), (256, 256), (256, 16), (256, 176)])
+def test_keys_whose_lanes_share_their_turns(hip_lib, D, r, dtype):
+    """Halves of whole vectors, from the ends of a page and one token a sequence: the bits of ``rotary``."""
+    g = gen(D + r)
+    rot = ro.Rotary.make(r, DEV, base=500.0, attention=1.3)
+    for lens, new in (([0, 63, 200, 7], [64, 2, 77, 1]), ([5, 63, 0, 128], None)):
+        T = 4 if new is None else sum(new)
+        table, P = tables([a + b for a, b in zip(lens, new or [1] * 4)], g)
+        cu = None if new is None else i32([sum(new[:i]) for i in range(5)])
+        k, v = (torch.randn(T, 3, D, generator=g, device=DEV).to(dtype) for _ in range(2))
+        pos = torch.randint(-(1 << 31), (1 << 31) - 1, (T,), generator=g, device=DEV).to(torch.int32)
+        kw = dict(dtype=dtype, device=DEV)
+        caches = [pc.PagedCache.empty(P, 3, D, **kw) for _ in range(2)]
+        for cache in caches:
+            cache.k_pages.zero_(), cache.v_pages.zero_(), cache.planes.zero_()
+        pc.paged_write(caches[0], k, v, table, i32(lens), cu_new=cu, rotary=rot, positions=pos)
+        pc.paged_write(caches[1], ro.rotary(rot, pos, k), v, table, i32(lens), cu_new=cu)
+        for n in ("k_pages", "v_pages", "planes"):
+            assert torch.equal(bits(getattr(caches[0], n)), bits(getattr(caches[1], n)))
+
+
 @pytest.mark.parametrize("lens", [[1], [0, 31, 32, 33, 63, 64, 65], [511, 0, 1000, 2], [4097], [300] * 40,
                                   [130, 0, 256, 1] * 33])
 @pytest.mark.parametrize("H,Hk,D,dtype", SHAPES)

@@ -372,6 +372,39 @@ def test_evict_rows_of_many_pages(hip_lib, width, B, Hk):
                     assert (r.kept[b, h, len(want[h]):] == W).all()
 
 
+def test_eviction_of_long_rows_replayed(hip_lib):
+    """Captured at one set of lengths and weights, replayed at others beside another graph's replay."""
+    g = gen(44)
+    W, keep, B, Hk = 300, 700, 2, 2
+    caches = [filled(gen(45), 40, Hk, 64, BF, "e4m3") for _ in range(2)]
+    table = torch.randint(0, 20, (B, W), generator=g, device=DEV, dtype=torch.int32)
+    new_table = torch.full((B, (keep + 63) // 64), -1, dtype=torch.int32, device=DEV)
+    held = [(torch.rand(B, Hk, 64 * W, generator=g, device=DEV), i32([64 * W, 9000])) for _ in range(2)]
+    pc.paged_evict(caches[0], *held[0][:1], table, held[0][1], new_table, keep, recent=9, first=3)
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for cache, (mass, lens) in zip(caches, held):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(pc.paged_evict(cache, mass, table, lens, new_table, keep, recent=9, first=3))
+        graphs.append(graph)
+    for lengths in ([64 * W, 12345], [100, 4096], [0, 8193], [64 * W - 1, 1]):
+        for mass, lens in held:
+            mass.copy_(torch.randint(0, 50, mass.shape, generator=g, device=DEV))
+            lens.copy_(i32(lengths))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for cache, (mass, lens), r in zip(caches, held, results):
+            want = pc.paged_evict(cache, mass, table, lens, new_table, keep, recent=9, first=3)
+            for got, x in ((r.kept, want.kept), (r.seq_lens, want.seq_lens), (r.mass, want.mass)):
+                assert torch.equal(got, x)
+            for b, n in enumerate(lengths):
+                for h in range(Hk):
+                    ref = pick_ref(mass[b, h], torch.ones(n, dtype=torch.bool, device=DEV), n, keep, 9, 3)
+                    assert torch.equal(r.kept[b, h, :len(ref)].long(), ref)
+
+
 def test_evict_of_a_shared_prefix(hip_lib):
     """Two sequences that share pages keep different tokens of them; the pages stay as they are."""
     g = gen(36)

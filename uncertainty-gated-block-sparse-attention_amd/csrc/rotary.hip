@@ -188,7 +188,7 @@ static hipError_t launch_rotary_t(const RotaryTable& t, const int32_t* positions
   (past ? rotary_kernel<E, L_, 2, true> : (many ? rotary_kernel<E, L_, 2, false> : rotary_kernel<E, L_, 1, false>))
   const auto kernel = t.interleaved ? UGBSA_ROT(kPairs) : UGBSA_ROT(kHalves);
 #undef UGBSA_ROT
-  kernel<<<(units + 255) / 256, 256, 0, stream>>>(q, k, t, positions, sp_b, M, D, bits, groups, units, sign);
+  kernel<<<static_cast<uint32_t>((units + 255ull) / 256), 256, 0, stream>>>(q, k, t, positions, sp_b, M, D, bits, groups, units, sign);
   return hipGetLastError();
 }
 
