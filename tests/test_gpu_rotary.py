@@ -110,6 +110,24 @@ def test_many_tokens(hip_lib):
         check(y, *turned(rot, pos[:, None], a))
 
 
+@pytest.mark.parametrize("r,interleaved", [(128, True), (100, True), (64, False), (98, False), (36, False)])
+def test_calls_of_any_size_agree(hip_lib, r, interleaved):
+    """A call that streams past the caches, one with several heads a thread and short ones give the same
+    bits; those of the short one are the formula's."""
+    g = gen(r)
+    T = 23000
+    rot = ro.Rotary.make(r, DEV, interleaved=interleaved)
+    x = torch.randn(T, 31, 128, generator=g, device=DEV).to(BF)
+    pos = torch.randint(0, 1 << 20, (T,), generator=g, device=DEV, dtype=torch.int32)
+    y = ro.rotary(rot, pos, x)
+    assert 2 * x.numel() * 2 > 320 << 20
+    for a, b in ((0, 9000), (9000, T), (T - 700, T)):
+        assert torch.equal(ro.rotary(rot, pos[a:b], x[a:b]), y[a:b])
+    check(y[-700:], *turned(rot, pos[-700:, None], x[-700:]))
+    z = x.clone()
+    assert torch.equal(ro.rotary(rot, pos, z, out=z), y)
+
+
 def test_far_and_negative_positions(hip_lib):
     """A turn of the first pair is 2 pi positions: 32 bits would not hold the angle."""
     pos = i32([0, 1, -1, -77777, 1 << 20, (1 << 24) + 1, (1 << 31) - 1, -(1 << 31)])
