@@ -274,6 +274,32 @@ def test_keys_whose_lanes_share_their_turns(hip_lib, D, r, dtype):
             assert torch.equal(bits(getattr(caches[0], n)), bits(getattr(caches[1], n)))
 
 
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("r,interleaved", [(128, False), (48, False), (128, True), (90, False)])
+def test_keys_turned_without_a_number(hip_lib, r, interleaved, dtype):
+    """Infinities, NaN and zeros of either sign among the keys: what ``rotary`` makes of them, NaN where it has one."""
+    g = gen(r)
+    rot = ro.Rotary.make(r, DEV, interleaved=interleaved)
+    special = torch.tensor([float("nan"), float("inf"), -float("inf"), 0.0, -0.0, 1.0, -2.0, 0.5], device=DEV)
+    k = special[torch.randint(0, 8, (100, 2, 128), generator=g, device=DEV)].to(dtype)
+    pos = torch.randint(0, 1000, (100,), generator=g, device=DEV).to(torch.int32)
+    pos[::3] = 0
+    table = i32([[0, 1]])
+    caches = [pc.PagedCache.empty(2, 2, 128, dtype, DEV) for _ in range(2)]
+    for cache in caches:
+        cache.k_pages.zero_(), cache.v_pages.zero_(), cache.planes.zero_()
+    cu = i32([0, 100])
+    pc.paged_write(caches[0], k, k, table, i32([0]), cu_new=cu, rotary=rot, positions=pos)
+    pc.paged_write(caches[1], ro.rotary(rot, pos, k), k, table, i32([0]), cu_new=cu)
+    for n in ("k_pages", "v_pages", "planes"):
+        x, y = (getattr(c, n) for c in caches)
+        assert torch.equal(x.isnan(), y.isnan())
+        if n != "planes":
+            assert torch.equal(bits(x.masked_fill(x.isnan(), 7.0)), bits(y.masked_fill(y.isnan(), 7.0)))
+        else:
+            assert torch.equal(x.nan_to_num(nan=7.0), y.nan_to_num(nan=7.0))
+
+
 @pytest.mark.parametrize("lens", [[1], [0, 31, 32, 33, 63, 64, 65], [511, 0, 1000, 2], [4097], [300] * 40,
                                   [130, 0, 256, 1] * 33])
 @pytest.mark.parametrize("H,Hk,D,dtype", SHAPES)
