@@ -137,6 +137,32 @@ def test_strides_that_reach_the_kernel(monkeypatch):
     assert len(calls) == 2
 
 
+def test_backward_turns_what_needs_a_gradient(monkeypatch):
+    """One launch over the operand that asks for it, whatever gradients come in; both in one launch where
+    both ask."""
+    calls = []
+    no_launch(monkeypatch, calls)
+    bf = torch.bfloat16
+    pos = torch.zeros(5, dtype=torch.int32)
+    for grads, heads in (((True, False), (4, 0)), ((False, True), (2, 0)), ((True, True), (4, 2))):
+        q, k = (torch.zeros(5, h, 64, dtype=bf, requires_grad=g) for h, g in zip((4, 2), grads))
+        out = ro.rotary(table(), pos, q, k)
+        assert [t.requires_grad for t in out] == [True, True]
+        calls.clear()
+        leaves = [t for t, g in zip((q, k), grads) if g]
+        got = torch.autograd.grad(out, leaves, [torch.zeros_like(t) for t in out])
+        assert [g.shape for g in got] == [t.shape for t in leaves]
+        args = calls[0][4:]
+        assert len(calls) == 1 and (args[11], args[22]) == heads and args[27] is True
+    # and to the second order
+    q = torch.zeros(5, 4, 64, dtype=bf, requires_grad=True)
+    d = [torch.zeros(5, h, 64, dtype=bf, requires_grad=True) for h in (4, 2)]
+    gq, = torch.autograd.grad(ro.rotary(table(), pos, q, torch.zeros(5, 2, 64, dtype=bf)), q, d, create_graph=True)
+    calls.clear()
+    got = torch.autograd.grad(gq, d, torch.zeros_like(q), allow_unused=True)
+    assert got[0].shape == d[0].shape and got[1] is None and len(calls) == 1 and calls[0][4:][22] == 0
+
+
 @pytest.mark.filterwarnings("ignore")
 def test_tangents_and_traces_are_refused(monkeypatch):
     no_launch(monkeypatch)

@@ -217,6 +217,8 @@ class _Turn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk=None):
         positions, = ctx.saved_tensors
+        # an operand that needs no gradient is not turned back, though its result has one to give
+        dq, dk = (d if need else None for d, need in zip((dq, dk), ctx.needs_input_grad[3:]))
         if dq is None and dk is None:
             return None, None, None, None, None
         if dq is None:
@@ -275,6 +277,8 @@ def rotary(rot, positions, q, k=None, out=None, inverse=False):
     attention factor, which is applied again)
 
     Returns the turned q, or (q, k) (``out`` if given).  Differentiable in q and k, to any order, unless ``out`` is given.
+    Where one of q and k requires a gradient, both results do, and the gradient of the other's is left
+    out: ``detach()`` that result before a call that takes none, such as ``paged_write``.
     A backward pass that is captured in a graph needs leaves that no eager graph holds.
     """
     if forward_ad._current_level >= 0 or _tracing_state() is not None:
