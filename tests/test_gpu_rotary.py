@@ -128,6 +128,34 @@ def test_calls_of_any_size_agree(hip_lib, r, interleaved):
     assert torch.equal(ro.rotary(rot, pos, z, out=z), y)
 
 
+def test_calls_of_several_launches(hip_lib):
+    """More rows than a grid has threads for: the bits of calls over some of them, where the launches meet
+    and at the ends."""
+    def same(rot, pos, x, meet):
+        T = x.shape[0]
+        parts = [slice(max(a - 300, 0), min(a + 300, T)) for a in (0, *meet, T)]
+        for p in parts:
+            x[p].normal_(generator=gen(p.start))
+        want = [ro.rotary(rot, pos[p], x[p].clone()) for p in parts]
+        check(want[-1], *turned(rot, pos[parts[-1], None], x[parts[-1]]))
+        assert ro.rotary(rot, pos, x, out=x) is x
+        for p, w in zip(parts, want):
+            assert torch.equal(x[p], w)
+            x[p].zero_()
+        step = 1 << 22
+        assert not any(x[i:i + step].any() for i in range(0, T, step))
+    print("[case] 63 threads a row", flush=True)          # one pair turns, 62 dims pass, a thread each
+    T = 70_000_000
+    assert T * 63 > 1 << 32
+    same(table(2), torch.arange(T, device=DEV, dtype=torch.int32), torch.zeros(T, 1, 64, dtype=BF, device=DEV),
+         ((1 << 31) // 63, (1 << 31) // 63 * 2))
+    print("[case] 16 threads a row", flush=True)
+    T = (1 << 27) + 1000
+    same(table(256), torch.arange(T, device=DEV, dtype=torch.int32), torch.zeros(T, 1, 256, dtype=BF, device=DEV),
+         (1 << 27,))
+    torch.cuda.empty_cache()
+
+
 def test_far_and_negative_positions(hip_lib):
     """A turn of the first pair is 2 pi positions: 32 bits would not hold the angle."""
     pos = i32([0, 1, -1, -77777, 1 << 20, (1 << 24) + 1, (1 << 31) - 1, -(1 << 31)])

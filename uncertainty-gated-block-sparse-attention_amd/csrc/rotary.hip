@@ -2,6 +2,8 @@
 // the gradient is the same with sin negated.
 //
 // Bound by memory: 4 bytes a value, read and written once.
+#include <algorithm>
+
 #include "rotary.h"
 
 namespace ugbsa {
@@ -51,11 +53,11 @@ template <typename E, int LAYOUT, int HPT, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads k, RotaryTable t,
                                                      const int32_t* __restrict__ positions, int64_t sp_b,
                                                      uint32_t M, int D, int chunk_bits, uint32_t groups,
-                                                     uint32_t units, float sign) {
+                                                     uint32_t row0, uint32_t units, float sign) {
   const uint32_t unit = blockIdx.x * 256u + threadIdx.x;
   if (unit >= units) return;
   const int chunk = unit & ((1u << chunk_bits) - 1), pairs = t.pairs;
-  const uint32_t row = unit >> chunk_bits, tok = row / groups, g = row - tok * groups;
+  const uint32_t row = row0 + (unit >> chunk_bits), tok = row / groups, g = row - tok * groups;
   const uint32_t b = tok / M, m = tok - b * M;
   // half layout: dims da .. of the lower half and db .. of the upper, of the dims that turn or of
   // those that pass; else two vectors half a head apart
@@ -113,14 +115,13 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryHeads q, RotaryHeads 
 template <typename E, int W, int HPT>
 __global__ __launch_bounds__(256) void rotary_odd_kernel(RotaryHeads q, RotaryHeads k, RotaryTable t,
                                                          const int32_t* __restrict__ positions, int64_t sp_b,
-                                                         uint32_t M, uint32_t items, uint32_t groups, uint32_t rows,
-                                                         float sign) {
+                                                         uint32_t M, uint32_t items, uint32_t groups, uint32_t row0,
+                                                         uint32_t rows, float sign) {
   using Bits = std::conditional_t<W == 2, uint32_t, uint16_t>;
-  const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * 256u + threadIdx.x;
-  const uint32_t row = static_cast<uint32_t>(unit / items);
-  if (row >= rows) return;
-  const int item = static_cast<int>(unit - static_cast<uint64_t>(row) * items), pairs = t.pairs;
-  const uint32_t tok = row / groups, g = row - tok * groups, b = tok / M, m = tok - b * M;
+  const uint32_t unit = blockIdx.x * 256u + threadIdx.x, at = unit / items;
+  if (at >= rows) return;
+  const int item = static_cast<int>(unit - at * items), pairs = t.pairs;
+  const uint32_t row = row0 + at, tok = row / groups, g = row - tok * groups, b = tok / M, m = tok - b * M;
   const bool turns = W * item < pairs;
   const int da = W * item, dc = pairs + da;          // past the pairs: dims from 2 pairs on
   Bits va[HPT], vb[HPT];
@@ -174,22 +175,33 @@ static hipError_t launch_rotary_t(const RotaryTable& t, const int32_t* positions
   const bool many = (static_cast<uint64_t>(toks) * heads << bits) >= 1u << 21;
   const bool odd = !t.interleaved && t.pairs % 8;
   const uint32_t each = !many ? 1 : (odd ? 4 : 2), groups = (heads + each - 1) / each, rows = toks * groups;
+  // A grid holds fewer than 2^32 threads: the rows of the longest calls go in several launches.
+  const auto in_pieces = [&](uint32_t threads, auto launch) {        // of a row; launch(first row, rows, grid)
+    const uint32_t most = (1u << 31) / threads;
+    for (uint32_t row0 = 0; row0 < rows; row0 += most) {
+      const uint32_t n = std::min(most, rows - row0);
+      launch(row0, n, (n * threads + 255) / 256);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  };
   if (odd) {
     const uint32_t items = (D - t.pairs) / (t.pairs % 2 ? 1 : 2);
-    const uint32_t grid = static_cast<uint32_t>((static_cast<uint64_t>(rows) * items + 255) / 256);
     const auto kernel = t.pairs % 2 ? (many ? rotary_odd_kernel<E, 1, 4> : rotary_odd_kernel<E, 1, 1>)
                                     : (many ? rotary_odd_kernel<E, 2, 4> : rotary_odd_kernel<E, 2, 1>);
-    kernel<<<grid, 256, 0, stream>>>(q, k, t, positions, sp_b, M, items, groups, rows, sign);
-    return hipGetLastError();
+    return in_pieces(items, [&](uint32_t row0, uint32_t n, uint32_t grid) {
+      kernel<<<grid, 256, 0, stream>>>(q, k, t, positions, sp_b, M, items, groups, row0, n, sign);
+    });
   }
-  const uint32_t units = rows << bits;
   const bool past = many && static_cast<uint64_t>(toks) * heads * D * 4 > 320ull << 20;
 #define UGBSA_ROT(L_) \
   (past ? rotary_kernel<E, L_, 2, true> : (many ? rotary_kernel<E, L_, 2, false> : rotary_kernel<E, L_, 1, false>))
   const auto kernel = t.interleaved ? UGBSA_ROT(kPairs) : UGBSA_ROT(kHalves);
 #undef UGBSA_ROT
-  kernel<<<static_cast<uint32_t>((units + 255ull) / 256), 256, 0, stream>>>(q, k, t, positions, sp_b, M, D, bits, groups, units, sign);
-  return hipGetLastError();
+  return in_pieces(1u << bits, [&](uint32_t row0, uint32_t n, uint32_t grid) {
+    kernel<<<grid, 256, 0, stream>>>(q, k, t, positions, sp_b, M, D, bits, groups, row0, n << bits, sign);
+  });
 }
 
 hipError_t launch_rotary(const RotaryTable& t, const int32_t* positions, int64_t sp_b, const RotaryHeads& q,
