@@ -465,7 +465,7 @@ int ugbsa_paged_decode_mass(const ugbsa_paged_cache* cache, const void* q, int64
  * ascending, then 64 * max_pages; new_lens [B] int32; new_mass [B, Hk, 64 * new_pages], the
  * kept tokens' mass, then zeros (mass and new_mass: rows as above).  Keys keep the
  * positions they were turned by: a later token's position is no longer its length.
- * 1 <= keep <= 64 * new_pages; recent + first <= keep.
+ * 1 <= keep <= 64 * new_pages, new_pages < 2^24; recent + first <= keep; B * Hk < 2^22.
  * workspace: 16-byte aligned floats, as many as the query says (none for most sizes). */
 int64_t ugbsa_paged_evict_workspace_elems(int B, int Hk, int max_pages);
 int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t sm_b,

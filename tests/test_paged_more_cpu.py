@@ -76,6 +76,17 @@ def test_evict_refusals(lib):
         refused(lib, evict_call(lib, four(), max_pages=512, **kw), code, "workspace")
 
 
+def test_evictions_past_a_grid_are_refused(lib):
+    """A workgroup of up to 1024 threads a row, and one of 256 a new page: 2^32 threads or more do not start."""
+    def evict(Hk=2, B=1, new_pages=4):
+        c = four(Hk=Hk)
+        return lib.ugbsa_paged_evict(ctypes.addressof(c), 16, 0, 0, 16, 16, 8, B, 8, 16, 4, new_pages, 100, 0, 0, 16, 16,
+                                     16, 256, 256, None, 0, None)
+    refused(lib, evict(new_pages=1 << 24), -1, "new_pages")
+    refused(lib, evict(Hk=65, B=65535), -1, "2^22")
+    refused(lib, evict(Hk=65535, B=65535), -1, "2^22")
+
+
 def test_write_rotary_refusals(lib):
     c = four()
 

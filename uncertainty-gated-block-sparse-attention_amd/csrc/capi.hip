@@ -830,7 +830,10 @@ int ugbsa_paged_evict(const ugbsa_paged_cache* cache, const float* mass, int64_t
   if (new_table == nullptr || kept == nullptr || new_lens == nullptr)
     return fail(UGBSA_EARG, "new_table, kept or new_lens is null");
   if (sn_b < 0) return fail(UGBSA_ELAYOUT, "new_table: negative row stride");
-  if (new_pages < 1 || new_pages > 1 << 24) return fail(UGBSA_EARG, "new_pages must lie in [1, 2^24] (%d)", new_pages);
+  // a workgroup a row and one a new page: grids of fewer than 2^32 threads
+  if (static_cast<int64_t>(B) * cache->Hk >= 1 << 22)
+    return fail(UGBSA_EARG, "B * Hk must be below 2^22 (B=%d, Hk=%d)", B, cache->Hk);
+  if (new_pages < 1 || new_pages >= 1 << 24) return fail(UGBSA_EARG, "new_pages must lie in [1, 2^24) (%d)", new_pages);
   if (keep < 1 || keep > static_cast<int64_t>(new_pages) * ugbsa::kBlock)
     return fail(UGBSA_EARG, "keep must lie in [1, 64 * new_pages] (%d, new_pages %d)", keep, new_pages);
   if (recent < 0 || first < 0 || static_cast<int64_t>(recent) + first > keep)
