@@ -76,6 +76,18 @@ def test_evict_refusals(lib):
         refused(lib, evict_call(lib, four(), max_pages=512, **kw), code, "workspace")
 
 
+def test_followed_weights_past_a_grid_are_refused(lib):
+    """B * H workgroups of 256 threads join pieces and B * Hk or more add weights, in one launch: 2^32
+    threads do not start."""
+    def call(B, H, pages, **kw):
+        c = struct(D=64, Hk=1, **kw)
+        return lib.ugbsa_paged_decode_mass(ctypes.addressof(c), 16, 64, 64, 64, 1, H, 16, 16, 8, B, pages, 0.1, None, None, 0,
+                                           16, 4096, 4096, 16, 64, 64, 1, 16, 0, None)
+    refused(lib, call(65535, 256, 17), -1, "too large")          # 16776960 + 65535 workgroups
+    refused(lib, call(65535, 255, 17), -1, "workspace")          # 16711425 + 65535: as far as the next check
+    refused(lib, call(65535, 256, 16), -1, "workspace")          # rows of one workgroup: the grids have two dimensions
+
+
 def test_evictions_past_a_grid_are_refused(lib):
     """A workgroup of up to 1024 threads a row, and one of 256 a new page: 2^32 threads or more do not start."""
     def evict(Hk=2, B=1, new_pages=4):

@@ -801,6 +801,8 @@ int ugbsa_paged_decode_mass(const ugbsa_paged_cache* cache, const void* q, int64
   int rc = check_paged_decode(cache, q, sq_b, sq_h, sq_m, sq_d, H, lens, table, st_b, B, max_pages, scale, kv_idx,
                               counts, k_slots, out, so_b, so_h, so_d);
   if (rc || (rc = check_mass("mass", mass, sm_b, sm_h))) return rc;
+  if (!ugbsa::paged_mass_fits(B, H, cache->Hk, cache->D, cache->cache_dtype, kv_idx != nullptr ? k_slots : max_pages))
+    return fail(UGBSA_EARG, "B * H and B * Hk * pages are too large to follow weights (B=%d, H=%d)", B, H);
   const int64_t need = ugbsa_paged_decode_mass_workspace_elems(B, H, cache->Hk, cache->D,
                                                                kv_idx != nullptr ? k_slots : max_pages,
                                                                cache->cache_dtype);

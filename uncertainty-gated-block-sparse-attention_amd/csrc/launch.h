@@ -220,7 +220,9 @@ hipError_t launch_paged_decode(const PagedCache& c, const uint16_t* q, int64_t s
                                hipStream_t stream);
 
 // The same, the weights added to mass [B, Hk, 64 max_pages] fp32; ws holds
-// paged_mass_ws_elems fp32.
+// paged_mass_ws_elems fp32.  fits: whether the launch that joins and adds has fewer than
+// 2^24 workgroups of 256 threads, and so a grid.
+bool paged_mass_fits(int B, int H, int Hk, int D, int kind, int units);
 int64_t paged_mass_ws_elems(int B, int H, int Hk, int D, int kind, int units);
 hipError_t launch_paged_mass(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h, int B, int H,
                              const int32_t* lens, const int32_t* table, int64_t st_b, int max_pages,

@@ -803,6 +803,18 @@ inline int paged_decode_workgroups(int B, int H, int Hk, int D, int kind, int un
   return static_cast<int>(most < resident ? most : resident);
 }
 
+// The launch after a MASS call on the line: tiles of a workgroup that adds weights, such workgroups of
+// a row, and all workgroups, those that join pieces first.
+struct PagedFinish {
+  int count, parts;
+  int64_t grid;
+};
+inline PagedFinish paged_finish(int B, int H, int Hk, int units) {
+  const int tiles = (units + 15) / 16, count = pd_mass_tiles(static_cast<int64_t>(tiles) * Hk * B);
+  const int parts = (tiles + count - 1) / count;
+  return {count, parts, static_cast<int64_t>(B) * H + static_cast<int64_t>(parts) * Hk * B};
+}
+
 template <typename E, int D, int KIND, bool MASS>
 hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& rows, const uint16_t* q, int64_t sq_b,
                                  int64_t sq_h, int B, int H, float scale, uint16_t* out, int64_t so_b, int64_t so_h,
@@ -846,11 +858,9 @@ hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& rows, con
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if constexpr (MASS) {
-    const int tiles = (units + 15) / 16, count = pd_mass_tiles(static_cast<int64_t>(tiles) * c.Hk * B);
-    const int parts = (tiles + count - 1) / count;
-    const int64_t grid = static_cast<int64_t>(B) * H + static_cast<int64_t>(parts) * c.Hk * B;
-    paged_finish_kernel<E, D><<<dim3(static_cast<uint32_t>(grid)), kPdCombineThreads, 0, stream>>>(
-        starts, part, ml, rows, gr, grp, chunks, B, parts, count, out, so_b, so_h, sc);
+    const PagedFinish f = paged_finish(B, H, c.Hk, units);
+    paged_finish_kernel<E, D><<<dim3(static_cast<uint32_t>(f.grid)), kPdCombineThreads, 0, stream>>>(
+        starts, part, ml, rows, gr, grp, chunks, B, f.parts, f.count, out, so_b, so_h, sc);
   } else {
     paged_combine_kernel<E, D><<<dim3(B * H), kPdCombineThreads, 0, stream>>>(starts, part, ml, gr, grp, chunks,
                                                                               lists, out, so_b, so_h);

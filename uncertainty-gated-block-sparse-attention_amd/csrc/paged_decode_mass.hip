@@ -23,6 +23,10 @@ int64_t paged_mass_ws_elems(int B, int H, int Hk, int D, int kind, int units) {
   return decode_elems(B, H, Hk, D, kind, units) + (2 * rows + 3) / 4 * 4 + rows * units * kBlock;
 }
 
+bool paged_mass_fits(int B, int H, int Hk, int D, int kind, int units) {
+  return paged_decode_one(D, kind, units) || paged_finish(B, H, Hk, units).grid < 1 << 24;
+}
+
 hipError_t launch_paged_mass(const PagedCache& c, const uint16_t* q, int64_t sq_b, int64_t sq_h, int B, int H,
                              const int32_t* lens, const int32_t* table, int64_t st_b, int max_pages,
                              const int32_t* kv_idx, const int32_t* counts, int k_slots, float scale, float* mass,
