@@ -372,6 +372,36 @@ def test_evict_rows_of_many_pages(hip_lib, width, B, Hk):
                     assert (r.kept[b, h, len(want[h]):] == W).all()
 
 
+@pytest.mark.parametrize("width,B,Hk", [(20, 2, 2), (100, 1, 3), (500, 40, 2), (900, 2, 3), (2100, 8, 8)])
+def test_evict_weights_that_agree(hip_lib, width, B, Hk):
+    """Rows most of whose weights were never added to, or lie within one bin or at a few values in it, in
+    every form of the pick: cuts among the zeros, among the others, and between the two."""
+    print(f"[case] weights that agree, {width} pages, {B} x {Hk}", flush=True)
+    g = gen(width)
+    W = 64 * width
+    cache = filled(g, 40, Hk, 64, BF, "e4m3")
+    pages = torch.randint(0, 40, (B, width), generator=g, device=DEV, dtype=torch.int32)
+    lens = [W - 7 * b if b % 3 < 2 else W // 2 + b for b in range(B)]
+    some = torch.rand(B, Hk, W, generator=g, device=DEV)
+
+    def masses():
+        yield torch.where(some < 0.03, torch.exp(3 * torch.randn(B, Hk, W, generator=g, device=DEV)), 0.0)
+        yield torch.where(some < 0.03, 1e-42, 0.0)                      # of the zeros' bin
+        yield torch.where(torch.arange(W, device=DEV) % 1024 < 960, 0.0, some)      # whole wavefronts alike
+        yield 1 + 0.2 * some
+        yield torch.where(some < 0.6, 1.125, 1 + 0.2 * some)
+        yield torch.where(torch.arange(W, device=DEV) < W // 2, 2.0, 2.25).expand(B, Hk, W).contiguous()
+    for mass in masses():
+        for keep, recent, first in ((W // 100, 0, 2), (W // 30, 5, 0), (W // 2, W // 8, 4)):
+            new_table = torch.full((B, (keep + 63) // 64), -1, dtype=torch.int32, device=DEV)
+            r = pc.paged_evict(cache, mass, pages, i32(lens), new_table, keep, recent=recent, first=first)
+            for b in {0, 1 % B, 2 % B, B - 1}:
+                there = torch.ones(lens[b], dtype=torch.bool, device=DEV)
+                for h in range(Hk):
+                    want = pick_ref(mass[b, h], there, lens[b], keep, recent, first)
+                    assert int(r.seq_lens[b]) == len(want) and torch.equal(r.kept[b, h, :len(want)].long(), want)
+
+
 def test_eviction_of_long_rows_replayed(hip_lib):
     """Captured at one set of lengths and weights, replayed at others beside another graph's replay."""
     g = gen(44)

@@ -33,10 +33,37 @@ __device__ __forceinline__ bool one_digit(const uint32_t* d) {
   return __ballot(d[0] != d0) == 0 && __ballot(d[1] != d0 || d[2] != d0 || d[3] != d0) == 0;
 }
 
+// Weights that nothing was added to are zeros, often most of a row's, and 64 lanes that add to one
+// word of LDS do so one behind the other: 128 rows of 32K tokens, 5 in 100 of them not 0, 126 us
+// so and 75 with the lanes that agree found first (zeros alone 105 and 69).  Among
+// weights over many binades the search would cost 5 in 100 of the call.  Whether enough agree:
+__device__ __forceinline__ bool many(uint64_t lanes) { return __builtin_popcountll(lanes) >= 24; }
+__device__ __forceinline__ bool alike_digits(const uint32_t* d) {
+  return many(__ballot(d[0] == __builtin_amdgcn_readfirstlane(d[0])));
+}
+
+
+// One more in its bin for each lane with `in`; the lane's place there.  The lanes that agree with the
+// first of them go with one addition.
+__device__ __forceinline__ uint32_t add_to_bin(uint32_t* hist, uint32_t bin, bool in, int lane) {
+  const uint64_t have = __ballot(in);
+  if (have == 0) return 0u;
+  const int lead = __builtin_ctzll(have);
+  const uint32_t one = __builtin_amdgcn_readlane(bin, lead);
+  const uint64_t same = __ballot(in && bin == one);
+  uint32_t at = 0u;
+  if (lane == lead) at = atomicAdd(&hist[one], static_cast<uint32_t>(__builtin_popcountll(same)));
+  at = __builtin_amdgcn_readlane(at, lead) + lanes_below(same);
+  if (in && bin != one) at = atomicAdd(&hist[bin], 1u);
+  return at;
+}
+
 // A row cut into parts of kPickPart tokens, a workgroup each, and what a part leaves for the
 // others: how many of its competing tokens each bin of the top digit holds and where they
 // begin, two bins a word; how many tokens stay in any case, and whether a page is absent; and
-// the keys, bin by bin.
+// the keys, bin by bin.  Of 2048 / 4096 / 8192 tokens, us of a call with the move: 64 rows of 32K
+// 52.6 / 43.0 / 41.8 (nearly all alike in their top digit 82 / 60 / 72), 4 of 32K 25.6 / 25.9 / 29.1 (43
+// / 44 / 61), 4 of 64K 28.3 / 26.9 / 29.9, 64 of 64K 83 / 60 / 52.
 constexpr int kPickPart = 4096, kPickWords = kPickBins / 2;
 constexpr int kPickStarts = kPickWords, kPickStay = 2 * kPickWords, kPickKeys = kPickStay + 4;
 constexpr int kPickRecord = kPickKeys + kPickPart;
@@ -87,6 +114,9 @@ __global__ __launch_bounds__(kPickPart / 8) void paged_digits_kernel(
       at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
       for (int j = 0; j < 4; ++j) rank[r][j] = at + 4 * lane + j;
+    } else if (alike_digits(d[r])) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rank[r][j] = add_to_bin(s_hist, d[r][j], in[r][j], lane);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -279,13 +309,37 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
       }
     }
   };
-  // f(key) over the cut's bin of the first `upto` parts
-  auto segments = [&](int upto, auto f) __attribute__((always_inline)) {
+  // over the cut's bin of the first `upto` parts: f(key, whether many of the wavefront's agree in these
+  // bits), or all(key, how many) where all that it has at once do (4 rows of 128K zeros: a load and a
+  // search after the other 229 us, so 63)
+  constexpr uint32_t SEG = 8;
+  auto segments = [&](int upto, uint32_t bits, auto all, auto f) __attribute__((always_inline)) {
 #pragma unroll 1
     for (int p = wave; p < upto; p += kPickWaves) {
       const uint32_t seg = s_seg[p], size = seg >> 16;
       const uint32_t* keys = records + static_cast<int64_t>(p) * kPickRecord + kPickKeys + (seg & 0xFFFFu);
-      for (uint32_t i = lane; i < size; i += 64) f(keys[i]);
+      uint32_t i = 0;
+#pragma unroll 1
+      for (; i + 64 * SEG <= size; i += 64 * SEG) {             // SEG loads on the way together
+        uint32_t k[SEG], other = 0u;
+#pragma unroll
+        for (uint32_t j = 0; j < SEG; ++j) k[j] = keys[i + 64 * j + lane];
+        const uint32_t one = __builtin_amdgcn_readfirstlane(k[0]);
+#pragma unroll
+        for (uint32_t j = 0; j < SEG; ++j) other |= k[j] ^ one;
+        if (__ballot((other & bits) != 0u) == 0) {
+          all(one, 64 * SEG);
+          continue;
+        }
+        const bool alike = many(__ballot(((k[0] ^ one) & bits) == 0u));
+#pragma unroll
+        for (uint32_t j = 0; j < SEG; ++j) f(k[j], alike);
+      }
+#pragma unroll 1
+      for (i += lane; i < size; i += 64) {
+        const uint32_t k = keys[i];
+        f(k, many(__ballot(((k ^ __builtin_amdgcn_readfirstlane(k)) & bits) == 0u)));
+      }
     }
   };
   int more = 0, same = 0;                             // of this lane's: above the cut, and tied
@@ -310,31 +364,38 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
         visit([&](f32x4 x, const uint64_t* in, bool all) __attribute__((always_inline)) {
           uint32_t d[4];
           top_digits(x, d);
-          if (all && one_digit(d)) {
+          const bool alike = alike_digits(d);
+          if (alike && all && one_digit(d)) {
             if (lane == 0) atomicAdd(&s_hist[d[0]], 256u);
             return;
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (mine(in[j])) atomicAdd(&s_hist[d[j]], 1u);
+          for (int j = 0; j < 4; ++j) {
+            if (alike) add_to_bin(s_hist, d[j], mine(in[j]), lane);
+            else if (mine(in[j])) atomicAdd(&s_hist[d[j]], 1u);
+          }
         });
       }
     } else if (PARTS) {
-      segments(parts, [&](uint32_t k) {
-        if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+      segments(parts, mask | static_cast<uint32_t>(bins - 1) << shift, [&](uint32_t k, uint32_t n) {
+        if ((k & mask) == prefix && lane == 0) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], n);
+      }, [&](uint32_t k, bool alike) __attribute__((always_inline)) {
+        const bool one = (k & mask) == prefix;
+        if (alike) add_to_bin(s_hist, (k >> shift) & (bins - 1), one, lane);
+        else if (one) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
       });
     } else if (top <= kPickList) {
       const uint32_t listed = min(s_listed, static_cast<uint32_t>(kPickList));
       for (uint32_t i = tid; i < listed; i += kPickThreads) {
         const uint32_t k = s_list[i];
-        if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+        add_to_bin(s_hist, (k >> shift) & (bins - 1), (k & mask) == prefix, lane);
       }
     } else {
       visit([&](f32x4 x, const uint64_t* in, bool) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t k = pick_key(x[j]);
-          if (mine(in[j]) && (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+          add_to_bin(s_hist, (k >> shift) & (bins - 1), mine(in[j]) && (k & mask) == prefix, lane);
         }
       });
     }
@@ -476,7 +537,11 @@ __global__ __launch_bounds__(kPickThreads) void paged_pick_kernel(
 #pragma unroll
     for (int j = 0; j < kEach; ++j) more0 += hi_bin - j >= sure ? others[j & 3] : 0u;
     if (top != 0u)
-      segments(part, [&](uint32_t k) { more0 += k > least ? 1 : 0, same0 += k == least ? 1 : 0; });
+      segments(part, ~0u, [&](uint32_t k, uint32_t n) {
+        if (lane == 0) more0 += k > least ? n : 0, same0 += k == least ? n : 0;
+      }, [&](uint32_t k, bool) __attribute__((always_inline)) {
+        more0 += k > least ? 1 : 0, same0 += k == least ? 1 : 0;
+      });
   } else if (listed_all) {
     // what the wavefront keeps: from the list where there is one
     for (uint32_t at = 0; at < listed; at += 64) {
@@ -643,13 +708,17 @@ __global__ __launch_bounds__(256) void paged_move_kernel(
   }
 }
 
-// Parts of a row, 0 where a workgroup has it whole.  Few long rows leave most CUs idle: with
-// the move, 4 rows of 64K tokens take 38 us in parts and 58 whole, of 128K 45 and 93, 32 rows
-// of 32K 44 and 51.  At 64 rows of 64K they meet (124 and 123); 128 rows of 32K take 122 and
-// 110, 4 rows of 16K 30 and 29.
+// Parts of a row, 0 where a workgroup has it whole.  Few long rows leave most CUs idle in that
+// form; in this one each part reads the keys of the cut's bin in all parts, which may be most of the
+// row.  us with the move, in parts / whole, of weights over many binades, all 0, and all within one
+// bin: 4 rows of 64K tokens 27 / 47, 46 / 80, 59 / 73; of 128K 31 / 73, 63 / 134, 91 / 123; of 1M 125 /
+// 371, 634 / 916, 1124 / 794; 64 of 32K 43 / 45, 54 / 61, 60 / 57; of 64K 60 / 58, 93 / 89, 120 / 83.  From
+// 2048 parts on they lose: 64 rows of 128K 93 / 87, 210 / 148, 311 / 138; 16 of 512K 151 / 213, 555 /
+// 474, 981 / 427.  128 rows of 32K take 122 and 110, 4 rows of 16K 30 and 29.
 static int paged_evict_parts(int B, int Hk, int max_pages) {
   const int parts = (max_pages + kPickPart / kBlock - 1) / (kPickPart / kBlock);
-  return max_pages > 256 && parts <= kPickMaxParts && static_cast<int64_t>(B) * Hk <= 64 ? parts : 0;
+  const int64_t rows = static_cast<int64_t>(B) * Hk;
+  return max_pages > 256 && parts <= kPickMaxParts && rows <= 64 && rows * parts <= 1024 ? parts : 0;
 }
 
 int64_t paged_evict_ws_elems(int B, int Hk, int max_pages) {
