@@ -51,6 +51,17 @@ def test_scaled_between_two_turn_counts():
     assert any(p / factor < x < p for x, p in zip(f, plain))
 
 
+def test_given_frequencies_keep_64_bits(monkeypatch):
+    """Numbers are not taken through 32 bits, which would move the angle of position 2^20 by 2^-5."""
+    monkeypatch.setattr(ro.Rotary, "__post_init__", lambda self: None)
+    f = [0.1, 1.0, 1 / 3]
+    for given in (f, tuple(f), torch.tensor(f, dtype=torch.float64)):
+        assert ro.Rotary.from_frequencies(given).turns.tolist() == [x / (2 * math.pi) for x in f]
+    for half in (torch.float32, torch.bfloat16):        # a tensor's values as they are
+        t = torch.tensor(f, dtype=half)
+        assert ro.Rotary.from_frequencies(t).turns.tolist() == [x / (2 * math.pi) for x in t.tolist()]
+
+
 def test_bad_tables_are_refused():
     for kw in (dict(r=3), dict(r=0), dict(r=64, base=0.0), dict(r=64, base=math.inf), dict(r=64, scaling="other"),
                dict(r=64, scaling="linear", factor=0.0), dict(r=64, factor=2.0), dict(r=2, scaling="ntk", factor=2.0),

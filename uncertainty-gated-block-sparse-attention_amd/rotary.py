@@ -75,7 +75,7 @@ class Rotary:
     @classmethod
     def from_frequencies(cls, frequencies, device=None, interleaved=False, attention=1.0):
         """The table of given f_j [rotary_dim / 2] (radians a position), as model code computes them."""
-        f = torch.as_tensor(frequencies, device=device).detach().to(torch.float64)
+        f = torch.as_tensor(frequencies, dtype=torch.float64, device=device).detach()
         return cls((f / (2 * math.pi)).contiguous(), interleaved, attention)
 
 
