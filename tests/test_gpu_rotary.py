@@ -1,6 +1,7 @@
 """Rotary positions against the formula in 64 bits on the same inputs, and their gradients."""
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -163,6 +164,33 @@ def test_far_and_negative_positions(hip_lib):
     x[:, 1] = 0.75
     for rot in (table(64), ro.Rotary.from_frequencies([1.0, 3.5, 0.25, 100.0, 7e-9], DEV, interleaved=True)):
         check(ro.rotary(rot, pos, x), *turned(rot, pos[:, None], x))
+
+
+def test_far_positions_exactly(hip_lib):
+    """Angles from exact rationals: the positions of each frequency whose cosine is nearest to zero, where
+    bf16 shows absolute errors of some 2^-24, up to 2^31.  Off by the series' 2^-22 and by 2.4 |pos| f 2^-53
+    (the product's rounding 2^-53, the table's 2^-53, its 2 pi's 2^-54.5)."""
+    pi = Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899863")
+    freqs = [1.0, 0.8659643233600653, 3.5, 0.25, 2.0 ** -20]
+    rot = ro.Rotary.from_frequencies(freqs, DEV)
+    rows = []
+    for top in (1 << 12, 1 << 20, 1 << 26, 1 << 30, (1 << 31) - 1):
+        for j, f in enumerate(freqs):
+            near = [min(max(round((2 * k + 1) * math.pi / (2 * f)), 0), top)
+                    for k in range(max(int(top * f / math.pi) - 5000, 0), int(top * f / math.pi))] or [top]
+            rest = [abs(Fraction(f) * p / pi % 1 - Fraction(1, 2)) for p in near]
+            pos = near[rest.index(min(rest))]
+            rows += [(pos, j), (-pos, j)]
+    pos = i32([p for p, _ in rows])
+    x = torch.zeros(len(rows), 1, 64, dtype=BF, device=DEV)
+    x[..., :len(freqs)] = 1
+    y = ro.rotary(rot, pos, x)[:, 0].double().cpu()
+    for i, (p, j) in enumerate(rows):
+        angle = float(Fraction(freqs[j]) * p % (2 * pi))
+        for got, want in ((y[i, j].item(), math.cos(angle)), (y[i, j + len(freqs)].item(), math.sin(angle))):
+            slack = 2.0 ** -22 + 2.4 * abs(p) * freqs[j] * 2.0 ** -53
+            # bf16's half step: 2^-8 of values in [.5, 1) apart are 2^-9 off at most, which is 2^-8 of .5
+            assert abs(got - want) <= 2.0 ** -8 * (abs(want) + slack) + slack, (p, freqs[j], got, want)
 
 
 def test_unusual_operands(hip_lib):

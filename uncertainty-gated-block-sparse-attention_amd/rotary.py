@@ -8,7 +8,8 @@ with or cached.
 
 Pair j of a head's first ``rotary_dim`` dims is turned by the angle position * f_j: (j, j + rotary_dim
 / 2), or (2 j, 2 j + 1) where the table is interleaved; the other dims pass unchanged.  Angles are
-reduced in 64 bits, so positions may be far apart; the products are fp32, rounded once.  ``rotary`` is
+reduced in 64 bits: cos and sin are off by less than 2^-22 + 2.4 |position| f_j 2^-53, whose second
+part is the smaller up to angles of 2^29; the products are fp32, rounded once.  ``rotary`` is
 differentiable in q and k.
 """
 
