@@ -131,6 +131,34 @@ def test_weights_absent_pages_and_wide_tables(hip_lib, kind):
         check_weights(q, cache, table, [0, -5, 200, 1], 0.09, start)
 
 
+@pytest.mark.parametrize("H,Hk,D,dtype,kind", [(8, 2, 64, BF, "model"), (34, 2, 128, FH, "e2m1"), (9, 1, 256, FH, "e2m1"),
+                                               (16, 2, 128, BF, "e4m3"), (40, 8, 128, BF, "e2m1")])
+def test_weights_of_several_live_tiles(hip_lib, H, Hk, D, dtype, kind):
+    """Wide tables and lists, where a workgroup adds the weights of several runs of 1024 tokens, in rows
+    that fill some of them, one or none."""
+    print(f"[case] live tiles H={H}/{Hk} D={D} {dtype} {kind}", flush=True)
+    g = gen(H + D)
+    lens, width = [9001, 1025, 5120, 0, 6200, 1024], 20000
+    B = len(lens)
+    tiles = (width + 15) // 16 * Hk * B
+    assert tiles > 2 * 1024                                  # a workgroup has three at least
+    table, P = tables(lens, g, width=width)
+    cache = filled(g, P, Hk, D, dtype, kind)
+    poison(cache, table, lens)
+    q = torch.randn(B, H, 1, D, generator=g, device=DEV).to(dtype)
+    start = torch.rand(B, Hk, 64 * width, generator=g, device=DEV)
+    check_weights(q, cache, table, lens, D ** -0.5, start)
+    slots = 4096
+    for counts in (None, torch.randint(17, 160, (B, Hk), generator=g, device=DEV, dtype=torch.int32)):
+        idx = torch.full((B, Hk, slots), width, dtype=torch.int32, device=DEV)
+        for b in range(B):
+            n = (lens[b] + 63) // 64
+            for h in range(Hk):                              # pages in any order, some that are none between
+                order = torch.randperm(n + 20, generator=g, device=DEV)
+                idx[b, h, :n + 20] = torch.where(order < n, order, width + 3).to(torch.int32)
+        check_weights(q, cache, table, lens, D ** -0.5, start, kv_idx=idx, counts=counts)
+
+
 def test_weights_of_nan_and_infinite_scores(hip_lib):
     """A NaN score makes its KV head's row NaN up to the length, and nothing past it."""
     g = gen(22)
