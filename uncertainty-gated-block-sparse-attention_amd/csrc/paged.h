@@ -8,9 +8,10 @@
 //           scale byte per 32 dims of a token's head ([P, Hk, D / 32, 64], so that the
 //           keys which a lane reads lie side by side; byte 255: the 32 are NaN)
 //   planes  [P, Hk, 2, D] in the 16-bit format: K-max and K-min of a page's keys as
-//           they were given, the Quest summary of kernel 1, one block a page.  What an
-//           e4m3 page holds of them is rounded, and may lie past the planes by half a
-//           step: 1/16 of its magnitude, or 2^-10 of the token's scale if that is more
+//           they were given, the Quest summary of kernel 1, one block a page.  What a
+//           page of codes holds of them is rounded, and may lie past the planes by half a
+//           step: of e4m3 1/16 of its magnitude, or 2^-10 of the token's scale if that is
+//           more; of e2m1 a quarter of its magnitude or of its scale
 //
 // Power-of-two scales keep every step exact but one: x 2^-e is exact, the
 // rounding to e4m3's four significant bits is the only one, and what the write
