@@ -445,7 +445,9 @@ int ugbsa_paged_decode(const ugbsa_paged_cache* cache, const void* q, int64_t sq
  * 64 * max_pages] fp32 (rows b and h at strides sm_b and sm_h, 16-byte aligned, each its
  * own memory): mass[b][h][i] grows by the sum over the KV head's query heads of the
  * softmax weight of token i (fp32, unrounded, in the heads' order).  Tokens that a row
- * does not attend to, and entries from lens[b] on, keep theirs.
+ * does not attend to, and entries from lens[b] on, keep theirs.  The workspace holds the
+ * scores, B * H * 64 * max_pages (or k_slots) floats, whatever the lengths are: 1.3 GB of 64
+ * sequences of 40 heads in tables of 2048 pages.  Cut the table to the longest sequence.
  * B * (H + Hk * (1 + max_pages (or k_slots) / 128)) must be below 2^24 - 2^13 where a row's
  * K and V in that many pages are more than 256 KB. */
 int64_t ugbsa_paged_decode_mass_workspace_elems(int B, int H, int Hk, int D, int units,

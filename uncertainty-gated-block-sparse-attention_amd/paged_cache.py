@@ -337,11 +337,12 @@ def paged_decode(q, cache, block_table, seq_lens, scale, kv_idx=None, counts=Non
     that the KV head's query heads attend to; counts [B, Hk] int32: how many entries count (None:
     all).  Entries that are no page of the sequence are skipped.
     mass : [B, Hk, >= 64 * max_pages] fp32, what each cached token's weight adds up to, for ``paged_evict``:
-    entry i of a row grows by the sum over the KV head's query heads of token i's softmax weight
+    entry i of a row grows by the sum over the KV head's query heads of token i's softmax weight.  The
+    call then keeps its scores meanwhile, B * H * 64 * (max_pages or k_slots) fp32 whatever the lengths are
     Returns [B, 1, H, D] contiguous, the dispatcher's layout (``out`` if given).  A sequence without
-    a key gives zeros.  Weights are rounded to ``dtype`` before the product with V.  The launch is
-    shaped by the table's (or list's) width: pass a table cut to the longest sequence where the batch
-    is short.
+    a key gives zeros.  Weights are rounded to ``dtype`` before the product with V.  The launch,
+    and the scores' memory with ``mass``, are shaped by the table's (or list's) width: pass a table cut to the
+    longest sequence where the batch is short.
     """
     assert cache.k_pages is not None, "a cache of planes alone has no pages"
     B, max_pages, st_b = _table(cache, block_table, seq_lens)
