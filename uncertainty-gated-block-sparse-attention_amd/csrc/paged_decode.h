@@ -22,8 +22,10 @@
 // scaled scores in a scratch [B, H, units, 64] on the way (units: the row's pages or list
 // entries), and the (m, l) of the rows it writes whole; the launch that joins the others'
 // pieces adds the weights up, in the heads' order and without atomics: a sequence has its
-// own row of mass.  Scores again from K instead would read 2 D bytes a token in 16 bits,
-// this writes and reads 8 a query head.
+// own row of mass.  This writes and reads 8 bytes a token and query head; scores again from K
+// would read 2 D bytes a token and KV head in 16 bits (256 at head_dim 128: up to 32 heads a
+// KV head), but 132 of e4m3's (16) and 68 of e2m1's (8), and make the products again.  34 / 2
+// heads over e2m1, 136 bytes for 68, 4 x 64K tokens: 47 us a call, 31 without mass.
 #pragma once
 
 #include <algorithm>
@@ -469,7 +471,12 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       if (moved)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-      // P rounded once to the element format, as the other attention kernels do
+      // P rounded once to the element format, which the products take, as in the other attention
+      // kernels: each weight is off by half a step at most, 2^-8 of it in bf16, and the errors of
+      // many tokens are independent, so the result's own rounding stays the larger part (norm of the
+      // error against 64 bits 2.1e-3 in bf16, 1.7e-3 where weights keep 32 bits; fp16 2.6e-4, 2.1e-4).
+      // The rest of P as a second piece gives the latter for a second product with V: e2m1, 32 x 64K
+      // tokens 360 -> 372 us, 24 of up to 16K at head_dim 256 25.6 -> 25.9, 32 x 64K at 64 125 -> 131.
       u32x4 pw;
 #pragma unroll
       for (int j = 0; j < 4; ++j) pw[j] = E::pack2(p[2 * j], p[2 * j + 1]);
@@ -708,7 +715,9 @@ __device__ __forceinline__ void add_mass(const PagedRows& rows, int Hk, int grp,
     *reinterpret_cast<f32x4*>(to) = old;
   }
 }
-// Tiles of a workgroup: some thousand workgroups in all, which start faster than more do.
+// Tiles of a workgroup: some thousand workgroups in all.  us a call with one tile / by this rule / up
+// to 16 for some 4 thousand tiles: 64 sequences of 2000 tokens in a table of 2048 pages, 40/8 heads, 117
+// / 79 / 72; 16 x 32K 167 / 166 / 176; 4 x 64K, 34/2 heads, 52 / 53 / 58; 4K tokens the same.
 inline int pd_mass_tiles(int64_t tiles) { return static_cast<int>(std::min<int64_t>((tiles + 1023) / 1024, 8)); }
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
@@ -849,7 +858,10 @@ hipError_t launch_paged_decode_t(const PagedCache& c, const PagedRows& rows, con
   // times as much and they would only displace each other there (32 x 16K tokens,
   // 40/8 heads, bf16 362 -> 336 us; 32 x 64K in e4m3 725 -> 698; 24 of up to 16K 77 ->
   // 72); smaller calls may find theirs in it (4 of up to 64K, head_dim 256, 41.1 and
-  // 42.2).  The table's width bounds the lengths, which are on the device.
+  // 42.2).  Of e2m1 from half as much again on: one cache of 204 / 272 / 340 / 408 / 544 MB read over
+  // and over 46 / 57 / 75 / 89 / 113 us through the cache, 50 / 59 / 69 / 81 / 104 past it (two caches in
+  // turn 52 / 65 / 76 / 89 / 113 and 48 / 59 / 69 / 80 / 101).  The table's width bounds the lengths,
+  // which are on the device.
   const int64_t most = static_cast<int64_t>(B) * c.Hk * units * paged_bytes(D, KIND);
   const auto kernel = most > (KIND == kPagesE2m1 ? 384ll : 768ll) << 20 ? paged_decode_kernel<E, D, KIND, true, 0, MASS>
                                          : paged_decode_kernel<E, D, KIND, false, 0, MASS>;

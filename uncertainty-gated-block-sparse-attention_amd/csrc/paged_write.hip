@@ -5,6 +5,10 @@
 // tokens, 4 heads, into e4m3 (232 MB): 48 us, 4.8 TB/s; 64K tokens of 8 heads back
 // (404 MB): 74.7 us, 5.4 TB/s; a copy of 256 MiB runs at 5.3.  37K tokens of 4
 // heads into e2m1 (97 MB) 27 us, and back into six rows of 17K (211 MB) 31.
+//
+// Where keys are turned, by their arithmetic: the (page, KV head) workgroups of a page each work
+// its tokens' angles out in 64 bits.  37K tokens of 4 heads, us turned / as given: into 16 bits
+// 38 / 29, e4m3 44 / 31, e2m1 36 / 27.
 #include "paged.h"
 #include "rotary.h"
 
