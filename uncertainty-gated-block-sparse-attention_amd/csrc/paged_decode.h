@@ -474,7 +474,7 @@ __global__ __launch_bounds__(64 * (ONE ? ONE : kPdWaves), ONE ? 2 : pd_occupancy
       // P rounded once to the element format, which the products take, as in the other attention
       // kernels: each weight is off by half a step at most, 2^-8 of it in bf16, and the errors of
       // many tokens are independent, so the result's own rounding stays the larger part (norm of the
-      // error against 64 bits 2.1e-3 in bf16, 1.7e-3 where weights keep 32 bits; fp16 2.6e-4, 2.1e-4).
+      // error against 64 bits 2.0e-3 to 2.3e-3 in bf16, 1.7e-3 where weights keep 32 bits; fp16 2.6e-4, 2.1e-4).
       // The rest of P as a second piece gives the latter for a second product with V: e2m1, 32 x 64K
       // tokens 360 -> 372 us, 24 of up to 16K at head_dim 256 25.6 -> 25.9, 32 x 64K at 64 125 -> 131.
       u32x4 pw;
